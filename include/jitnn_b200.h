@@ -344,6 +344,84 @@ JQ_API int jq_gguf_meta_number(const jq_gguf* f, const char* key, double* value,
 JQ_API int jq_gguf_meta_string(const jq_gguf* f, const char* key, const char** bytes, int64_t* length);
 JQ_API int jq_gguf_upload(const jq_gguf* f, int64_t index, int device, int64_t row_begin, int64_t row_end, jq_weight** out);
 
+/*
+ * ---- operators of paged decoding ---------------------------------------------------------------------------------
+ * All of them take device pointers of the handle's GPU, only enqueue work on `stream`, allocate nothing, and may be captured into a graph; what workspace they need the
+ * caller gives, one for each call that may overlap another. Element types of rows and pages: */
+#define JQ_ELEM_F32 0
+#define JQ_ELEM_F16 1
+#define JQ_ELEM_BF16 2
+
+/*
+ * Rotary positions (ops/Rope.java:84-149; RopeScaling.linear and llama3, and YaRN of Peng et al. 2023).
+ *
+ * jq_rope_frequencies  (host only) freqs[dim / 2] = the angle per position of every pair, base^(-2 i / dim) rescaled, and *magnitude, what the rotated values are multiplied
+ *                      with. params: LINEAR {factor}; LLAMA3 {factor, low, high, context}: pairs with fewer than `low` turns in `context` positions are slowed down by
+ *                      `factor`, those with more than `high` stay, linear between; YARN {factor, context, fast, slow, magnitude}: the same between the pairs that
+ *                      make `fast` and `slow` turns, a magnitude of 0 stands for 0.1 ln(factor) + 1.
+ * jq_rope_create       the table of cosines and sines (made in double) for positions 0 .. positions - 1 on `device`. Pairs are (x[i], x[i + dim / 2]), or
+ *                      (x[2 i], x[2 i + 1]) where `interleaved`.
+ * jq_rope_apply        y = x with the first dim elements of every head rotated, for one tensor or two (queries and keys) in one launch: x[c] is [batch, seq, heads[c],
+ *                      head_dim] with the element strides strides[6 c ..] = {batch, token, head of x, batch, token, head of y}, elements of a head next to each other;
+ *                      y[c] may be x[c], and must not overlap it otherwise. positions: int32 or int64 (position_bytes 4 or 8) with strides, or NULL: offset + token. A position outside the table gives NaN and
+ *                      status 97 (jq_device_status). inverse: by the negative angle, which makes the gradient of x out of that of y.
+ */
+#define JQ_ROPE_NONE 0
+#define JQ_ROPE_LINEAR 1
+#define JQ_ROPE_LLAMA3 2
+#define JQ_ROPE_YARN 3
+typedef struct jq_rope jq_rope;
+JQ_API int jq_rope_frequencies(int dim, double base, int scaling, const double* params, double* freqs, double* magnitude);
+JQ_API int jq_rope_create(int device, int64_t positions, int dim, const double* freqs, double magnitude, int interleaved, jq_rope** out);
+JQ_API int jq_rope_free(jq_rope* r);
+JQ_API int jq_rope_apply(const jq_rope* r, int elem, int count, const void* const* x, void* const* y, const int* heads, int head_dim, const int64_t* strides, int64_t batch,
+                         int64_t seq, const void* positions, int position_bytes, int64_t position_batch_stride, int64_t position_stride, int64_t offset, int inverse,
+                         void* stream);
+
+/*
+ * A paged cache of keys and values (the reference has no cache). k and v are the caller's memory, [pages][kv_heads][page_size][head_dim] of type `elem`, page_size a power
+ * of two from 16 to 1024; the handle borrows them.
+ *
+ * A batch: rows starts[s] .. starts[s + 1] - 1 (int32 [sequences + 1], ascending) are the newest of sequence s, which has lengths[s] keys of its own once they are
+ * appended, key i on page tables[s * table_stride + i / page_size]. In front of their own keys all sequences see the prefix_length keys on the pages prefix[0 ..].
+ * A row's own position is lengths[s] - (starts[s + 1] - row); where that is negative the row has no keys of its own and none is stored. Rows outside
+ * starts[0] .. starts[sequences] - 1 belong to no sequence: their outputs are left as they were, or become zero where `fill`. tables, starts, lengths and prefix are read on the device, at
+ * every replay of a graph anew. A page id outside the cache, or a position outside the table of pages, is not touched (its keys are not seen, its rows not stored) and leaves status 96
+ * for jq_device_status. Where two rows of a call have the same page and slot, either is stored.
+ *
+ * jq_pages_append     k and v [tokens, kv_heads, head_dim] to their pages, k rotated at prefix_length + own position first, and q_out [tokens, heads, head_dim] = q rotated
+ *                     likewise (heads 0: no queries; rope NULL: no rotation). strides (elements): token and head of q, k, v, q_out. Rows are FP32, or of the pages' type.
+ *                     q_out may be q. A position that the table of rotations does not have gives NaN queries, stores nothing and leaves status 97.
+ * jq_pages_attention  out [tokens, heads, head_dim]: softmax(scale q . k) v over the prefix and the own keys up to the row's position; a row that sees no key gives zeros.
+ *                     strides: token and head of q and out. heads is a multiple of kv_heads, which neighbouring heads share. prefix has prefix_width pages.
+ *                     workspace: jq_pages_attention_bytes of device memory at a 256-byte aligned address.
+ */
+typedef struct jq_pages jq_pages;
+JQ_API int jq_pages_create(int device, int elem, int64_t pages, int page_size, int kv_heads, int head_dim, void* k, void* v, jq_pages** out);
+JQ_API int jq_pages_free(jq_pages* p);
+JQ_API int jq_pages_append(const jq_pages* p, const jq_rope* rope, int elem, int heads, const void* q, const void* k, const void* v, void* q_out, const int64_t* strides,
+                           int64_t tokens, const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences,
+                           int64_t prefix_length, int fill, void* stream);
+JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens, int64_t prefix_length, int64_t* nbytes);
+JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void* q, void* out, const int64_t* strides, int64_t tokens, const int32_t* tables,
+                              int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, const int32_t* prefix,
+                              int64_t prefix_width, int64_t prefix_length, float scale, int fill, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Verification of drafted tokens (speculative sampling; the reference has no generation loop). target [sequences, drafts_most + 1, vocab] are the target's logits (`logits` non-zero, at
+ * `temperature`) or probabilities behind each draft, draft_probs [sequences, drafts_most, vocab] FP32 the drafter's (NULL: all on the draft), drafts and counts (NULL:
+ * drafts_most each) int32, uniforms FP32 [sequences, drafts_most + 1] numbers in [0, 1). Strides are elements; drafts and uniforms are contiguous.
+ * Draft i is kept while uniforms[i] q_i(x_i) < p_i(x_i); then one token comes by the inverse distribution function at uniforms[drafts_most]: behind the first refused draft j from
+ * max(p_j - q_j, 0) over its sum (p_j where that is zero), behind the last draft from p. accepted[s] = the drafts kept, tokens [sequences, drafts_most + 1] = those, the
+ * further token, and -1 in the rest. Temperature 0: the likeliest token (the first of equal ones) instead, uniforms and draft_probs are not read. No drafts at
+ * all is sampling. All in double. A weight that is NaN counts as zero; where no weight is left the token is the last. A draft outside the vocabulary is refused and leaves status 98.
+ * workspace: jq_verify_bytes (which also holds the limits of the sizes) of device memory at a 16-byte aligned address.
+ */
+JQ_API int jq_verify_bytes(int64_t sequences, int64_t drafts_most, int64_t vocab, int logits, int64_t* nbytes);
+JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t target_stride, int64_t target_row_stride, const int32_t* drafts, const float* draft_probs,
+                            int64_t draft_stride, int64_t draft_row_stride, const float* uniforms, const int32_t* counts, int64_t sequences, int64_t drafts_most,
+                            int64_t vocab, int logits, double temperature, int32_t* accepted, int32_t* tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Pinned host memory for activations and results (faster and truly asynchronous copies). */
 JQ_API int jq_host_alloc(void** ptr, int64_t nbytes);
 JQ_API int jq_host_free(void* ptr);

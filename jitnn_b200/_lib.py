@@ -18,7 +18,7 @@ JQ_ERR_INVALID, JQ_ERR_OOM, JQ_ERR_CUDA, JQ_ERR_NCCL, JQ_ERR_TIMEOUT, JQ_ERR_UNS
 JQ_MEM_HOST, JQ_MEM_DEVICE = 0, 1
 JQ_LAYOUT_AUTO = 0
 
-c_i64, c_int, vp = ctypes.c_int64, ctypes.c_int, ctypes.c_void_p
+c_i64, c_int, c_double, vp = ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.c_void_p
 
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
@@ -71,6 +71,17 @@ SIGNATURES = {
     "jq_gguf_meta_number": (c_int, [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_i64)]),
     "jq_gguf_meta_string": (c_int, [vp, ctypes.c_char_p, ctypes.POINTER(vp), ctypes.POINTER(c_i64)]),
     "jq_gguf_upload": (c_int, [vp, c_i64, c_int, c_i64, c_i64, ctypes.POINTER(vp)]),
+    "jq_rope_frequencies": (c_int, [c_int, c_double, c_int, vp, vp, ctypes.POINTER(c_double)]),
+    "jq_rope_create": (c_int, [c_int, c_i64, c_int, vp, c_double, c_int, ctypes.POINTER(vp)]),
+    "jq_rope_free": (c_int, [vp]),
+    "jq_rope_apply": (c_int, [vp, c_int, c_int, vp, vp, vp, c_int, vp, c_i64, c_i64, vp, c_int, c_i64, c_i64, c_i64, c_int, vp]),
+    "jq_pages_create": (c_int, [c_int, c_int, c_i64, c_int, c_int, c_int, vp, vp, ctypes.POINTER(vp)]),
+    "jq_pages_free": (c_int, [vp]),
+    "jq_pages_append": (c_int, [vp, vp, c_int, c_int, vp, vp, vp, vp, vp, c_i64, vp, c_i64, c_i64, vp, vp, c_int, c_i64, c_int, vp]),
+    "jq_pages_attention_bytes": (c_int, [vp, c_int, c_i64, c_i64, ctypes.POINTER(c_i64)]),
+    "jq_pages_attention": (c_int, [vp, c_int, c_int, vp, vp, vp, c_i64, vp, c_i64, c_i64, vp, vp, c_int, vp, c_i64, c_i64, ctypes.c_float, c_int, vp, c_i64, vp]),
+    "jq_verify_bytes": (c_int, [c_i64, c_i64, c_i64, c_int, ctypes.POINTER(c_i64)]),
+    "jq_verify_drafts": (c_int, [c_int, c_int, vp, c_i64, c_i64, vp, vp, c_i64, c_i64, vp, vp, c_i64, c_i64, c_i64, c_int, c_double, vp, vp, vp, c_i64, vp]),
     "jq_host_alloc": (c_int, [ctypes.POINTER(vp), c_i64]),
     "jq_host_free": (c_int, [vp]),
     "jq_launch_count": (c_i64, []),

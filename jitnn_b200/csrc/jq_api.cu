@@ -34,27 +34,6 @@ int check_launch(const char* kernel) {
     return JQ_OK;
 }
 
-// Makes `device` current for the scope and restores the caller's device afterwards.
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int device) {
-        if (cudaGetDevice(&prev) != cudaSuccess) {
-            prev = -1;
-        }
-        if (prev != device) {
-            ok = cudaSetDevice(device) == cudaSuccess;
-        } else {
-            prev = -1;
-        }
-    }
-    ~DeviceGuard() {
-        if (prev >= 0) {
-            cudaSetDevice(prev);
-        }
-    }
-};
-
 // Per-thread, per-device staging for calls whose data lives on the host: a device buffer that grows on
 // demand and a private stream, so that concurrent callers never share scratch.
 struct Staging {

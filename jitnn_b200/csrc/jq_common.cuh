@@ -30,6 +30,27 @@ inline void count_launch(int n = 1) { g_launches.fetch_add(n, std::memory_order_
 // Checks the launch that was just issued.
 int check_launch(const char* kernel);
 
+// Makes `device` current for the scope and restores the caller's device afterwards.
+struct DeviceGuard {
+    int prev = -1;
+    bool ok = true;
+    explicit DeviceGuard(int device) {
+        if (cudaGetDevice(&prev) != cudaSuccess) {
+            prev = -1;
+        }
+        if (prev != device) {
+            ok = cudaSetDevice(device) == cudaSuccess;
+        } else {
+            prev = -1;
+        }
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) {
+            cudaSetDevice(prev);
+        }
+    }
+};
+
 // ---- block geometry (DType.java:75-98 of the reference) ---------------------------------------
 inline int block_values(int type) {
     switch (type) {
