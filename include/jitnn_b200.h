@@ -392,7 +392,8 @@ JQ_API int jq_rope_apply(const jq_rope* r, int elem, int count, const void* cons
  * jq_pages_append     k and v [tokens, kv_heads, head_dim] to their pages, k rotated at prefix_length + own position first, and q_out [tokens, heads, head_dim] = q rotated
  *                     likewise (heads 0: no queries; rope NULL: no rotation). strides (elements): token and head of q, k, v, q_out. Rows are FP32, or of the pages' type.
  *                     q_out may be q. A position that the table of rotations does not have gives NaN queries, stores nothing and leaves status 97.
- * jq_pages_attention  out [tokens, heads, head_dim]: softmax(scale q . k) v over the prefix and the own keys up to the row's position; a row that sees no key gives zeros.
+ * jq_pages_attention  out [tokens, heads, head_dim]: softmax(scale q . k) v over the prefix and the own keys up to the row's position; a row that sees no key, or only keys whose
+ *                     scores are negative infinities, gives zeros.
  *                     strides: token and head of q and out. heads is a multiple of kv_heads, which neighbouring heads share. prefix has prefix_width pages.
  *                     workspace: jq_pages_attention_bytes of device memory at a 256-byte aligned address.
  */
@@ -402,7 +403,7 @@ JQ_API int jq_pages_free(jq_pages* p);
 JQ_API int jq_pages_append(const jq_pages* p, const jq_rope* rope, int elem, int heads, const void* q, const void* k, const void* v, void* q_out, const int64_t* strides,
                            int64_t tokens, const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences,
                            int64_t prefix_length, int fill, void* stream);
-JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens, int64_t prefix_length, int64_t* nbytes);
+JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes);
 JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void* q, void* out, const int64_t* strides, int64_t tokens, const int32_t* tables,
                               int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, const int32_t* prefix,
                               int64_t prefix_width, int64_t prefix_length, float scale, int fill, void* workspace, int64_t workspace_bytes, void* stream);

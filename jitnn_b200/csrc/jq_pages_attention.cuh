@@ -1,0 +1,137 @@
+// What the paged attention's kernels share: the arguments, and how the work is cut.
+#pragma once
+
+#include "jq_pages.cuh"
+
+namespace jq {
+
+// The work of a launch: items (sequence, key/value head, block of rows), each of as many units as its sequence has runs of keys. Rows are token * group + head of the
+// group. The prefix is one more sequence behind the others, all tokens its rows. Units are numbered through all items, a sequence's blocks of rows next to one another (they read the
+// same keys), and thread block c has units c * per .. (c + 1) * per - 1: sequences of any lengths share the GPU evenly, and nobody on the host needs to know the lengths.
+// An item that lies in one thread block is complete there; of the others a thread block leaves partial results in its two slots, the first for the item that
+// began in front of it, the second for the one that goes on behind it.
+struct Work {
+    int first, last;   // sequences first .. last - 1; number b.sequences is the prefix
+    int rows_shift;    // rows of a block, keys of a unit: powers of two
+    int keys_shift;
+    int ctas;          // thread blocks at most
+    int least;         // units that make a thread block worth while
+    float* part;       // [slot][rows of a block][head_dim]
+    float2* part_ml;   // maxima (of scores times log2 e) and sums
+};
+
+struct AttendArgs {
+    const void* q;
+    void* out;
+    int64_t qt, qh, ot, oh;  // strides of token and head, in elements
+    const void *k_pages, *v_pages;
+    int64_t pages;
+    int page_size, page_shift, heads, kv_heads, head_dim, group;
+    Batch b;
+    float scale;
+    int fill;
+    int* status;
+    Work own, pre;     // whose the own keys' items are, and whose the prefix's
+    float* whole;      // of complete items, where own keys and a prefix are to be joined: over own keys and over the prefix, [2][token][head][head_dim]
+    float2* whole_ml;
+    int joined;        // whether they are
+    long long wait_clocks;
+};
+
+struct Sequence {
+    int row0, rows;    // tokens
+    int keys;          // that its last row sees
+    int reach;         // the same before it is cut to what the table of pages has, or below zero
+    int blocks;        // of rows, per key/value head
+    int chunks;        // units of a block
+    __device__ int64_t units(int kv_heads) const { return (int64_t)kv_heads * blocks * chunks; }
+};
+
+__device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int s, int rows_shift, int keys_shift) {
+    Sequence q;
+    if (s == a.b.sequences) {
+        q.row0 = 0;
+        q.rows = a.b.tokens;
+        q.keys = q.reach = a.b.prefix_length;
+    } else {
+        const int from = a.b.starts[s], to = a.b.starts[s + 1], length = a.b.lengths[s];
+        q.row0 = from < 0 ? 0 : from;
+        const int end = to < a.b.tokens ? to : a.b.tokens;
+        q.rows = end > q.row0 ? end - q.row0 : 0;
+        // the keys that the sequence's last row here sees; a row's position is counted from the end that the sequence names
+        const int64_t keys = (int64_t)length - ((int64_t)to - end);
+        const int64_t most = (int64_t)a.b.table_width << a.page_shift;
+        if (q.rows > 0 && keys > most) {
+            note_status(a.status, STATUS_PAGE);
+        }
+        q.reach = (int)(keys < -0x40000000 ? -0x40000000 : keys);
+        q.keys = q.rows == 0 || keys < 0 ? 0 : (int)(keys < most ? keys : most);
+    }
+    q.blocks = (int)(((int64_t)q.rows * a.group + (1 << rows_shift) - 1) >> rows_shift);
+    q.chunks = (int)(((int64_t)q.keys + (1 << keys_shift) - 1) >> keys_shift);
+    return q;
+}
+
+// Keys that the row of token `i` of the sequence sees.
+__device__ __forceinline__ int keys_seen(const AttendArgs& a, const Sequence& q, int s, int i) {
+    if (s == a.b.sequences) {
+        return q.keys;
+    }
+    const int64_t n = (int64_t)q.reach - (q.rows - 1 - i);
+    return n < 0 ? 0 : (n < q.keys ? (int)n : q.keys);
+}
+
+struct Cut {
+    int64_t total, per;
+    __device__ __forceinline__ int thread_block_of(int64_t unit) const { return (int)(unit / per); }
+};
+
+// By a whole warp: the units of sequences first .. end - 1 of a work, all of them together, and the units of a thread block.
+__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+__device__ __forceinline__ int64_t units_before(const AttendArgs& a, const Work& w, int end, int lane) {
+    int64_t sum = 0;
+    for (int s = w.first + lane; s < end; s += 32) {
+        sum += sequence_at(a, s, w.rows_shift, w.keys_shift).units(a.kv_heads);
+    }
+    return warp_sum(sum);
+}
+__device__ __forceinline__ Cut cut_of(const Work& w, int64_t total) {
+    Cut c;
+    c.total = total;
+    int64_t used = (total + w.least - 1) / w.least;
+    used = used < w.ctas ? used : w.ctas;
+    c.per = used > 0 ? (total + used - 1) / used : 1;
+    return c;
+}
+// The sequence that a unit is in, and the first unit of that sequence; by a whole warp.
+__device__ __forceinline__ int find_unit(const AttendArgs& a, const Work& w, int64_t unit, int lane, int64_t& base) {
+    int64_t before = 0;
+    for (int s0 = w.first; s0 < w.last; s0 += 32) {
+        const int s = s0 + lane;
+        const int64_t mine = s < w.last ? sequence_at(a, s, w.rows_shift, w.keys_shift).units(a.kv_heads) : 0;
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t n = __shfl_up_sync(0xffffffffu, upto, o);
+            upto += lane >= o ? n : 0;
+        }
+        upto += before;
+        const unsigned hit = __ballot_sync(0xffffffffu, unit < upto);
+        if (hit != 0u) {
+            const int at = __ffs(hit) - 1;
+            base = __shfl_sync(0xffffffffu, upto - mine, at);
+            return s0 + at;
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    base = before;
+    return w.last;
+}
+
+}  // namespace jq

@@ -400,6 +400,9 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     if (rc != JQ_OK) {
         return rc;
     }
+    if (sequences == 0) {
+        return JQ_OK;
+    }
     if (!elem_ok(elem) || target == nullptr || (drafts == nullptr && drafts_most > 0) || accepted == nullptr || tokens == nullptr) {
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: null pointer, or element type %d", elem);
     }
@@ -412,9 +415,6 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     }
     if (workspace_bytes < need || (need > 0 && (workspace == nullptr || ((uintptr_t)workspace & 15) != 0))) {
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: a workspace of %lld bytes at a 16-byte aligned address is needed, got %lld", (long long)need, (long long)workspace_bytes);
-    }
-    if (sequences == 0) {
-        return JQ_OK;
     }
     int count = 0;
     JQ_CUDA(cudaGetDeviceCount(&count));

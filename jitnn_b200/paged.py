@@ -266,7 +266,7 @@ class PagedCache:
 
     def attention(self, q, batch, scale=None, out=None):
         """softmax(scale q . k) v [tokens, heads, head_dim] of each row over the prefix and its sequence's keys up to its own; ``scale`` is 1 / sqrt(head_dim) where it
-        is None. Neighbouring heads share a key/value head. A row that sees no key gives zeros; rows of no sequence become zero in a new tensor, and stay as they are in ``out``."""
+        is None. Neighbouring heads share a key/value head. A row that sees no key, or only keys with scores of negative infinity, gives zeros; rows of no sequence become zero in a new tensor, and stay as they are in ``out``."""
         torch = _t()
         h = self._handle()
         self._on_pages(batch)
@@ -279,7 +279,7 @@ class PagedCache:
         if q.shape[0]:
             L = _lib.load()
             need = ctypes.c_int64()
-            check(L.jq_pages_attention_bytes(h, q.shape[1], q.shape[0], batch.prefix_length, ctypes.byref(need)))
+            check(L.jq_pages_attention_bytes(h, q.shape[1], q.shape[0], batch._rows[5], batch.prefix_length, ctypes.byref(need)))
             space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
             strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), y.stride(0), y.stride(1))
             check(L.jq_pages_attention(h, code, q.shape[1], q.data_ptr(), y.data_ptr(), strides, q.shape[0], *batch._rows, *batch._ahead,

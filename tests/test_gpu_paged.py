@@ -227,19 +227,29 @@ def check_attention(t, q, heads, kv, hd, act, cache, scale=None):
 @pytest.mark.parametrize("hd", [64, 128, 256, 40])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 def test_what_a_row_does_not_see_does_not_reach_it(act, cache, hd, bad):
-    """The newest keys and values of a run of drafts are not finite: the rows in front of them stay as they were, the last sees them."""
+    """The newest keys and values of a run of drafts are not finite: the rows in front of them are what they were, the last sees them.
+
+    Where values are not finite the kernels may add them up one by one, in another order than otherwise: two results that are each within attention_bound of the same 64-bit
+    value are within twice that of each other, which is what is asked of the rows (the bits need not be the same)."""
     t = Setup([1, 4, 1], [50, 61, 16], 2, hd, 16, cache, prefix=20, hole=bad, seed=3)
     q = normal(t.tokens, 4, hd, dtype=act, seed=3)
     clean = check_attention(t, q, 4, 2, hd, act, cache)
+    rest, bounds = [0, 1, 2, 3, 5], []
+    for row, s, at in t.each_row():
+        k, v = (torch.cat((oracle.keys_of(x, t.prefix, 16, 20), oracle.keys_of(x, t.tables[s], 16, at + 1))) for x in (t.k, t.v))
+        want, size, score = oracle.attention(q[row], k, v, 1 / math.sqrt(hd))
+        bounds.append(2 * oracle.attention_bound(want, size, score, hd, len(k), act, cache))
+    bounds = torch.stack(bounds)[rest]
     page, slot = int(t.tables[1, 60 // 16]), 60 % 16
     t.cache.k[page, :, slot] = bad
     t.cache.v[page, :, slot] = bad
     got = t.cache.attention(q.cuda(), t.batch)
-    assert torch.equal(got[[0, 1, 2, 3, 5]], clean[[0, 1, 2, 3, 5]])
+    within(got[rest], clean[rest].double().cpu(), bounds)
     assert not torch.isfinite(got[4]).any() if not (bad == -math.inf) else True
     t.cache.k[page, :, slot] = 0.0  # only the value is not finite: what sees it is that
     got = t.cache.attention(q.cuda(), t.batch)
-    assert torch.equal(got[[0, 1, 2, 3, 5]], clean[[0, 1, 2, 3, 5]]) and not torch.isfinite(got[4]).any()
+    within(got[rest], clean[rest].double().cpu(), bounds)
+    assert not torch.isfinite(got[4]).any()
     no_status()
 
 
@@ -337,8 +347,8 @@ def test_bad_pages_are_not_touched():
     t.cache.append(None, k.cuda(), v.cuda(), batch)
     assert device_status(0) == 96
     batch = PagedBatch(t.tables.cuda(), t.batch.starts, torch.tensor([100, 20], dtype=torch.int32, device="cuda"))
-    assert torch.isfinite(t.cache.attention(q.cuda(), batch)).all()
-    assert device_status(0) == 96
+    got = t.cache.attention(q.cuda(), batch)  # (the row sees what lies behind key 40 on its last page, where nothing finite is, and nothing of pages that are not in the table)
+    assert device_status(0) == 96 and torch.isnan(got[0]).all() and torch.isfinite(got[1]).all()
     for starts in ([0, 5, 9], [-3, 1, 2], [2, 1, 0], [7, 8, 9]):  # rows that are not there, or backwards
         batch = PagedBatch(t.tables.cuda(), torch.tensor(starts, dtype=torch.int32, device="cuda"), t.batch.lengths, prefix=t.batch.prefix, prefix_length=20)
         assert torch.isfinite(t.cache.attention(q.cuda(), batch)).all()
@@ -403,7 +413,8 @@ def test_streams_and_graphs():
             with torch.cuda.stream(s):
                 g.replay()
     torch.cuda.synchronize()
-    assert torch.equal(outs[0], plain[0]) and torch.equal(outs[1], plain[1]) and not torch.equal(outs[0], outs[1])
+    bits = [[x.view(torch.int32) for x in xs] for xs in (outs, plain)]  # (the other lengths reach what nobody has written: NaN)
+    assert torch.equal(bits[0][0], bits[1][0]) and torch.equal(bits[0][1], bits[1][1]) and not torch.equal(bits[0][0], bits[0][1])
     no_status()
 
 
