@@ -403,7 +403,7 @@ JQ_API int jq_pages_free(jq_pages* p);
 JQ_API int jq_pages_append(const jq_pages* p, const jq_rope* rope, int elem, int heads, const void* q, const void* k, const void* v, void* q_out, const int64_t* strides,
                            int64_t tokens, const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences,
                            int64_t prefix_length, int fill, void* stream);
-JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes);
+JQ_API int jq_pages_attention_bytes(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes);
 JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void* q, void* out, const int64_t* strides, int64_t tokens, const int32_t* tables,
                               int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, const int32_t* prefix,
                               int64_t prefix_width, int64_t prefix_length, float scale, int fill, void* workspace, int64_t workspace_bytes, void* stream);

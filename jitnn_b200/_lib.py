@@ -78,7 +78,7 @@ SIGNATURES = {
     "jq_pages_create": (c_int, [c_int, c_int, c_i64, c_int, c_int, c_int, vp, vp, ctypes.POINTER(vp)]),
     "jq_pages_free": (c_int, [vp]),
     "jq_pages_append": (c_int, [vp, vp, c_int, c_int, vp, vp, vp, vp, vp, c_i64, vp, c_i64, c_i64, vp, vp, c_int, c_i64, c_int, vp]),
-    "jq_pages_attention_bytes": (c_int, [vp, c_int, c_i64, c_i64, c_i64, ctypes.POINTER(c_i64)]),
+    "jq_pages_attention_bytes": (c_int, [vp, c_int, c_int, c_i64, c_i64, c_i64, ctypes.POINTER(c_i64)]),
     "jq_pages_attention": (c_int, [vp, c_int, c_int, vp, vp, vp, c_i64, vp, c_i64, c_i64, vp, vp, c_int, vp, c_i64, c_i64, ctypes.c_float, c_int, vp, c_i64, vp]),
     "jq_verify_bytes": (c_int, [c_i64, c_i64, c_i64, c_int, ctypes.POINTER(c_i64)]),
     "jq_verify_drafts": (c_int, [c_int, c_int, vp, c_i64, c_i64, vp, vp, c_i64, c_i64, vp, vp, c_i64, c_i64, c_i64, c_int, c_double, vp, vp, vp, c_i64, vp]),

@@ -6,6 +6,7 @@
 #include "jq_pages_attention.cuh"
 #include "jq_pages_join.cuh"
 #include "jq_pages_stream.cuh"
+#include "jq_pages_tile.cuh"
 
 namespace jq {
 namespace {
@@ -111,89 +112,130 @@ __global__ void __launch_bounds__(128) attend_row_kernel(AttendArgs a) {
     }
 }
 
+// Who does what, and where in the workspace.
 struct Plan {
-    int rows = 0;   // of a block; 0: the row kernel
-    int ctas = 0;
-    int64_t part = 0, part_ml = 0, whole = 0, whole_ml = 0, bytes = 0;  // where in the workspace
+    int rows = 0;              // of the stream kernel's blocks; 0: it is not launched
+    int workers = 0;           // its warps
+    int tile_workers = 0;      // the tile kernel's thread blocks; 0: it is not launched
+    bool tile_own = false;     // whether it takes own keys too, not the prefix alone
+    int64_t part = 0, part_ml = 0, tile_part = 0, tile_part_ml = 0, whole = 0, whole_ml = 0, bytes = 0;
 };
 
-// How many thread blocks of an instance an SM holds (registers), and with it the share of the work that each gets.
-template <typename C, int HD, int NB>
-constexpr int resident() {
-    return HD * sizeof(C) >= 512 ? 2 : 3;
-}
+// How many thread blocks of the stream kernel an SM holds (by its registers).
+constexpr int stream_resident(int head_dim, int bytes) { return head_dim * bytes >= 512 ? 2 : 3; }
 
-int resident_of(int elem, int head_dim) { return head_dim * elem_bytes(elem) >= 512 ? 2 : 3; }
+// Rows of a key/value head that read the same keys: up to 16 go to the stream kernel, which reads the keys once for 8 or 16 rows; more go to the tile kernel, which takes 128 at
+// a time. It is made for 16-bit pages and heads of 64 and 128.
+constexpr int STREAM_ROWS = 16;
 
-Plan plan_of(const jq_pages* p, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length) {
+Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length) {
     Plan plan;
-    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256) {
+    const int hd = p->head_dim;
+    if ((hd != 64 && hd != 128 && hd != 256) || tokens == 0) {
         return plan;
     }
-    const int64_t group = heads / p->kv_heads, rows = (tokens + sequences - 1) / sequences * group;
-    plan.rows = rows <= 8 || p->head_dim == 256 ? 8 : 16;
-    plan.ctas = 148 * resident_of(p->elem, p->head_dim);
+    const int64_t group = heads / p->kv_heads, own = (tokens + sequences - 1) / sequences * group, shared = tokens * group;
+    const bool tile = p->elem != JQ_ELEM_F32 && hd <= 128;
+    plan.tile_own = tile && own > STREAM_ROWS;
+    if (plan.tile_own || (tile && prefix_length > 0 && shared > STREAM_ROWS)) {
+        const int resident = elem == p->elem ? 2 : 1;
+        // (the prefix's units are known here; of the own keys the device knows)
+        const int64_t units = (int64_t)p->kv_heads * ((shared + pages::TILE_BLOCK - 1) / pages::TILE_BLOCK) * ((prefix_length + pages::TILE_KEYS - 1) / pages::TILE_KEYS);
+        plan.tile_workers = (int)(!plan.tile_own && units < 148 * resident ? units : 148 * resident);
+    }
+    if (!plan.tile_own) {
+        plan.rows = own <= 8 || hd == 256 ? 8 : 16;
+        plan.workers = 148 * stream_resident(hd, elem_bytes(p->elem)) * pages::STREAM_WARPS;
+    }
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    plan.part = take((int64_t)2 * plan.ctas * plan.rows * p->head_dim * 4);
-    plan.part_ml = take((int64_t)2 * plan.ctas * plan.rows * 8);
+    plan.part = take((int64_t)2 * plan.workers * plan.rows * hd * 4);
+    plan.part_ml = take((int64_t)2 * plan.workers * plan.rows * 8);
+    plan.tile_part = take((int64_t)2 * plan.tile_workers * pages::TILE_BLOCK * hd * 4);
+    plan.tile_part_ml = take((int64_t)2 * plan.tile_workers * pages::TILE_BLOCK * 8);
     if (prefix_length > 0) {
-        plan.whole = take(2 * tokens * heads * p->head_dim * 4);
+        plan.whole = take(2 * tokens * heads * hd * 4);
         plan.whole_ml = take(2 * tokens * heads * 8);
     }
     plan.bytes = at;
     return plan;
 }
 
-template <typename T, typename C, int HD, int NB>
-int launch_stream(const AttendArgs& a, cudaStream_t s) {
-    constexpr int smem = pages::Stream<T, C, HD, NB>::SMEM, RESIDENT = resident<C, HD, NB>();
-    auto kernel = pages::attend_stream_kernel<T, C, HD, NB, RESIDENT>;
-    static std::atomic<uint64_t> configured{0};  // the opt-in for large dynamic shared memory is per device
+template <typename K>
+int large_smem(K kernel, int smem, std::atomic<uint64_t>& configured) {  // the opt-in is per device
     int dev = 0;
     JQ_CUDA(cudaGetDevice(&dev));
-    if (smem > 48 * 1024 && (configured.load(std::memory_order_relaxed) >> (dev & 63) & 1) == 0) {
+    if ((configured.load(std::memory_order_relaxed) >> (dev & 63) & 1) == 0) {
         JQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
         configured.fetch_or((uint64_t)1 << (dev & 63));
     }
-    kernel<<<a.own.ctas, pages::STREAM_THREADS, smem, s>>>(a);
-    count_launch();
-    int rc = check_launch("attend_stream_kernel");
-    if (rc != JQ_OK) {
-        return rc;
-    }
+    return JQ_OK;
+}
+
+// Behind a kernel of this call (`behind`): programmatically, all of this call's kernels but the joining one work at the same time.
+template <typename K>
+int launch_part(K kernel, dim3 grid, int threads, int smem, bool behind, const AttendArgs& a, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3((unsigned)a.b.tokens, (unsigned)((a.heads + pages::JOIN_HEADS - 1) / pages::JOIN_HEADS));
-    cfg.blockDim = dim3(pages::JOIN_THREADS);
+    cfg.numAttrs = behind ? 1 : 0;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    JQ_CUDA(cudaLaunchKernelEx(&cfg, pages::attend_join_kernel<T, HD>, a));
+    JQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
     count_launch();
     return JQ_OK;
 }
 
+template <typename T, typename C, int HD, int NB>
+int launch_stream(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
+    static std::atomic<uint64_t> configured{0};
+    constexpr int smem = pages::Stream<T, C, HD, NB>::SMEM;
+    auto kernel = pages::attend_stream_kernel<T, C, HD, NB, stream_resident(HD, sizeof(C))>;
+    const int rc = smem > 48 * 1024 ? large_smem(kernel, smem, configured) : JQ_OK;
+    return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, plan.tile_workers > 0, a, s);
+}
+
+template <typename T, typename C, int HD>
+int launch_attend_head(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
+    int rc = JQ_OK;
+    if constexpr (sizeof(C) == 2 && HD <= 128) {
+        if (plan.tile_workers > 0) {
+            static std::atomic<uint64_t> configured{0};
+            constexpr int smem = pages::Tile<T, C, HD>::SMEM;
+            rc = large_smem(pages::attend_tile_kernel<T, C, HD>, smem, configured);
+            rc = rc != JQ_OK ? rc : launch_part(pages::attend_tile_kernel<T, C, HD>, dim3((unsigned)plan.tile_workers), pages::TILE_THREADS, smem, false, a, s);
+        }
+    }
+    if (rc == JQ_OK && plan.rows == 8) {
+        rc = launch_stream<T, C, HD, 1>(a, plan, s);
+    }
+    if constexpr (HD <= 128) {
+        if (rc == JQ_OK && plan.rows == 16) {
+            rc = launch_stream<T, C, HD, 2>(a, plan, s);
+        }
+    }
+    return rc != JQ_OK ? rc : launch_part(pages::attend_join_kernel<T, HD>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, a, s);
+}
+
 template <typename T, typename C>
 int launch_attend(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
-    if (plan.rows == 0) {
-        attend_row_kernel<T, C><<<dim3((unsigned)a.b.tokens, (unsigned)a.heads), 128, 0, s>>>(a);
-        count_launch();
-        return check_launch("attend_row_kernel");
+    switch (a.head_dim) {
+        case 64: return launch_attend_head<T, C, 64>(a, plan, s);
+        case 128: return launch_attend_head<T, C, 128>(a, plan, s);
+        case 256: return launch_attend_head<T, C, 256>(a, plan, s);
+        default: break;
     }
-    if (a.head_dim == 64) {
-        return plan.rows == 8 ? launch_stream<T, C, 64, 1>(a, s) : launch_stream<T, C, 64, 2>(a, s);
-    }
-    if (a.head_dim == 128) {
-        return plan.rows == 8 ? launch_stream<T, C, 128, 1>(a, s) : launch_stream<T, C, 128, 2>(a, s);
-    }
-    return launch_stream<T, C, 256, 1>(a, s);
+    attend_row_kernel<T, C><<<dim3((unsigned)a.b.tokens, (unsigned)a.heads), 128, 0, s>>>(a);
+    count_launch();
+    return check_launch("attend_row_kernel");
 }
 
 }  // namespace
@@ -203,7 +245,7 @@ using namespace jq;
 
 extern "C" {
 
-JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes) {
+JQ_API int jq_pages_attention_bytes(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes) {
     const int rc = check_pages(p, "jq_pages_attention_bytes");
     if (rc != JQ_OK) {
         return rc;
@@ -212,7 +254,7 @@ JQ_API int jq_pages_attention_bytes(const jq_pages* p, int heads, int64_t tokens
         return fail(JQ_ERR_INVALID, "jq_pages_attention: %lld rows of %lld sequences, %d heads on %d key/value heads", (long long)tokens, (long long)sequences, heads,
                     p->kv_heads);
     }
-    *nbytes = plan_of(p, heads, tokens, sequences, prefix_length).bytes;
+    *nbytes = plan_of(p, elem, heads, tokens, sequences, prefix_length).bytes;
     return JQ_OK;
 }
 
@@ -220,7 +262,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
                               int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, const int32_t* prefix,
                               int64_t prefix_width, int64_t prefix_length, float scale, int fill, void* workspace, int64_t workspace_bytes, void* stream) {
     int64_t need = 0;
-    int rc = jq_pages_attention_bytes(p, heads, tokens, sequences, prefix_length, &need);
+    int rc = jq_pages_attention_bytes(p, elem, heads, tokens, sequences, prefix_length, &need);
     if (rc != JQ_OK) {
         return rc;
     }
@@ -252,11 +294,16 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     while (1 << a.page_shift < p->page_size) {
         a.page_shift++;
     }
-    const Plan plan = plan_of(p, heads, tokens, sequences, prefix_length);
+    const Plan plan = plan_of(p, elem, heads, tokens, sequences, prefix_length);
     uint8_t* const space = static_cast<uint8_t*>(workspace);
-    a.own = Work{0, sequences + (prefix_length > 0 ? 1 : 0), plan.rows == 8 ? 3 : 4, 4, plan.ctas, pages::STREAM_WARPS, reinterpret_cast<float*>(space + plan.part),
-                 reinterpret_cast<float2*>(space + plan.part_ml)};
-    a.pre = a.own;
+    auto floats = [&](int64_t at) { return reinterpret_cast<float*>(space + at); };
+    auto pairs = [&](int64_t at) { return reinterpret_cast<float2*>(space + at); };
+    const int ahead = prefix_length > 0 ? 1 : 0;
+    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 6, plan.tile_workers, 1, floats(plan.tile_part), pairs(plan.tile_part_ml)};
+    const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, 1, floats(plan.part), pairs(plan.part_ml)};
+    a.own = plan.tile_own ? tile : few;
+    a.pre = plan.tile_workers > 0 ? tile : few;
+    a.wait_clocks = (long long)g_opt_wait_limit_us.load(std::memory_order_relaxed) * 2000;  // about 2 GHz
     a.whole = reinterpret_cast<float*>(space + plan.whole);
     a.whole_ml = reinterpret_cast<float2*>(space + plan.whole_ml);
     a.joined = prefix_length > 0 ? 1 : 0;

@@ -7,15 +7,15 @@ namespace jq {
 
 // The work of a launch: items (sequence, key/value head, block of rows), each of as many units as its sequence has runs of keys. Rows are token * group + head of the
 // group. The prefix is one more sequence behind the others, all tokens its rows. Units are numbered through all items, a sequence's blocks of rows next to one another (they read the
-// same keys), and thread block c has units c * per .. (c + 1) * per - 1: sequences of any lengths share the GPU evenly, and nobody on the host needs to know the lengths.
-// An item that lies in one thread block is complete there; of the others a thread block leaves partial results in its two slots, the first for the item that
+// same keys), and worker c (a warp, or a thread block) has units c * per .. (c + 1) * per - 1: sequences of any lengths share the GPU evenly, and nobody on the host needs to know the lengths.
+// An item that one worker has all of is complete there; of the others a worker leaves partial results in its two slots, the first for the item that
 // began in front of it, the second for the one that goes on behind it.
 struct Work {
     int first, last;   // sequences first .. last - 1; number b.sequences is the prefix
     int rows_shift;    // rows of a block, keys of a unit: powers of two
     int keys_shift;
-    int ctas;          // thread blocks at most
-    int least;         // units that make a thread block worth while
+    int workers;       // at most
+    int least;         // units that make another worker worth while
     float* part;       // [slot][rows of a block][head_dim]
     float2* part_ml;   // maxima (of scores times log2 e) and sums
 };
@@ -83,10 +83,10 @@ __device__ __forceinline__ int keys_seen(const AttendArgs& a, const Sequence& q,
 
 struct Cut {
     int64_t total, per;
-    __device__ __forceinline__ int thread_block_of(int64_t unit) const { return (int)(unit / per); }
+    __device__ __forceinline__ int worker_of(int64_t unit) const { return (int)(unit / per); }
 };
 
-// By a whole warp: the units of sequences first .. end - 1 of a work, all of them together, and the units of a thread block.
+// By a whole warp: the units of sequences first .. end - 1 of a work, all of them together, and the units of a worker.
 __device__ __forceinline__ int64_t warp_sum(int64_t v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -105,7 +105,7 @@ __device__ __forceinline__ Cut cut_of(const Work& w, int64_t total) {
     Cut c;
     c.total = total;
     int64_t used = (total + w.least - 1) / w.least;
-    used = used < w.ctas ? used : w.ctas;
+    used = used < w.workers ? used : w.workers;
     c.per = used > 0 ? (total + used - 1) / used : 1;
     return c;
 }

@@ -1,5 +1,5 @@
-// Joins what the thread blocks have of a row: a warp has one head of one token. Which thread blocks those are it works out anew from the lengths, while the kernels in front
-// still run; up to 32 partial results are asked for at once, a lane each its maximum and sum.
+// Joins what the workers have of a row: a thread block has one head of one token. Which workers those are it works out anew from the lengths, while the kernels in front
+// still run. Its warps take the partial results in turn, eight each at once, a lane each the maximum and sum of 32.
 #pragma once
 
 #include "jq_pages_attention.cuh"
@@ -8,15 +8,14 @@
 namespace jq {
 namespace pages {
 
-constexpr int JOIN_THREADS = 256, JOIN_HEADS = JOIN_THREADS / 32;
+constexpr int JOIN_WARPS = 4, JOIN_THREADS = 32 * JOIN_WARPS;
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a) {
-    const int lane = threadIdx.x & 31, token = blockIdx.x, h = blockIdx.y * JOIN_HEADS + (threadIdx.x >> 5);
-    if (h >= a.heads) {
-        return;
-    }
     constexpr int V = HD / 32;  // elements of a lane
+    __shared__ float meet[JOIN_WARPS][HD];
+    __shared__ float2 meet_ml[JOIN_WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x, h = blockIdx.y;
     // the token's sequence: the last that has it
     int s = -1;
     for (int s0 = 0; s0 < a.b.sequences; s0 += 32) {
@@ -30,13 +29,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
         asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            if (a.fill) {
+            if (a.fill && warp == 0) {
                 out[lane * V + j] = from_float<T>(0.0f);
             }
         }
         return;
     }
-    // where the results over own keys and over the prefix are: `count` of them in slots of thread blocks first, first + 1 ..; or one complete
+    // where the results over own keys and over the prefix are: `count` of them in slots of workers first, first + 1 ..; or one complete
     int count[2], first[2], in_block[2];
     const bool one = a.joined == 0;
     const int kvh = h / a.group;
@@ -54,8 +53,8 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
         if (q.chunks > 0) {
             const int row = (token - q.row0) * a.group + h % a.group;
             const int64_t item0 = base + ((int64_t)kvh * q.blocks + (row >> w.rows_shift)) * q.chunks;
-            first[part] = cut.thread_block_of(item0);
-            count[part] = cut.thread_block_of(item0 + q.chunks - 1) - first[part] + 1;
+            first[part] = cut.worker_of(item0);
+            count[part] = cut.worker_of(item0 + q.chunks - 1) - first[part] + 1;
             in_block[part] = row & ((1 << w.rows_shift) - 1);
         }
     }
@@ -68,12 +67,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
     for (int j = 0; j < V; j++) {
         acc[j] = 0.0f;
     }
-    const int all = count[0] + count[1];
-    for (int n0 = 0; n0 < all; n0 += 32) {
+    const int all = count[0] + count[1], each = (all + JOIN_WARPS - 1) / JOIN_WARPS;
+    const int mine = each * warp < all ? each * warp : all, upto = mine + each < all ? mine + each : all;
+    for (int n0 = mine; n0 < upto; n0 += 32) {
         const int n = n0 + lane;
         const float* from = nullptr;
         float2 ml = make_float2(-INFINITY, 0.0f);
-        if (n < all) {
+        if (n < upto) {
             const int part = n < count[0] ? 0 : 1, i = part == 0 ? n : n - count[0];
             const Work& w = part == 0 ? a.own : a.pre;
             if (count[part] == 1) {
@@ -104,30 +104,58 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
         for (int j = 0; j < V; j++) {
             acc[j] *= shrink;
         }
-        const int here = all - n0 < 32 ? all - n0 : 32;
-#pragma unroll 4
-        for (int i = 0; i < here; i++) {
-            const float* const p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), i)) + lane * V;
-            const float x = __shfl_sync(0xffffffffu, weight, i);
+        const int here = upto - n0 < 32 ? upto - n0 : 32;
+        for (int i0 = 0; i0 < here; i0 += 8) {
+            float v[8][V], x[8];
 #pragma unroll
-            for (int j = 0; j < V; j += V >= 4 ? 4 : 2) {
-                if constexpr (V >= 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(p + j);
-                    acc[j] = fmaf(v.x, x, acc[j]);
-                    acc[j + 1] = fmaf(v.y, x, acc[j + 1]);
-                    acc[j + 2] = fmaf(v.z, x, acc[j + 2]);
-                    acc[j + 3] = fmaf(v.w, x, acc[j + 3]);
-                } else {
-                    const float2 v = *reinterpret_cast<const float2*>(p + j);
-                    acc[j] = fmaf(v.x, x, acc[j]);
-                    acc[j + 1] = fmaf(v.y, x, acc[j + 1]);
+            for (int i = 0; i < 8; i++) {
+                const int k = i0 + i < here ? i0 + i : i0;  // (the last ones twice, the second time for nothing)
+                const float* const p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), k)) + lane * V;
+                x[i] = __shfl_sync(0xffffffffu, weight, k);
+#pragma unroll
+                for (int j = 0; j < V; j += 2) {
+                    const float2 e = *reinterpret_cast<const float2*>(p + j);
+                    v[i][j] = e.x;
+                    v[i][j + 1] = e.y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                if (i0 + i < here) {
+#pragma unroll
+                    for (int j = 0; j < V; j++) {
+                        acc[j] = fmaf(v[i][j], x[i], acc[j]);
+                    }
                 }
             }
         }
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        out[lane * V + j] = from_float<T>(over(acc[j], l));
+        meet[warp][lane * V + j] = acc[j];
+    }
+    if (lane == 0) {
+        meet_ml[warp] = make_float2(m, l);
+    }
+    __syncthreads();
+    float top = -INFINITY, sum = 0.0f, weight[JOIN_WARPS];
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; w++) {
+        top = fmaxf(top, meet_ml[w].x);
+    }
+    const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int w = 0; w < JOIN_WARPS; w++) {
+        weight[w] = exp2_fast(meet_ml[w].x - base);
+        sum = fmaf(meet_ml[w].y, weight[w], sum);
+    }
+    for (int d = threadIdx.x; d < HD; d += JOIN_THREADS) {
+        float o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WARPS; w++) {
+            o = fmaf(meet[w][d], weight[w], o);
+        }
+        out[d] = from_float<T>(over(o, sum));
     }
 }
 

@@ -75,10 +75,53 @@ __device__ __forceinline__ uint4 load_once(const void* p) {
     return v;
 }
 
-__device__ __forceinline__ uint4 load_shared16(const void* p) {
+__device__ __forceinline__ uint4 load_shared16_at(uint32_t at) {
     uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
     return v;
+}
+__device__ __forceinline__ uint4 load_shared16(const void* p) { return load_shared16_at((uint32_t)__cvta_generic_to_shared(p)); }
+
+// Whether one of the numbers in sixteen bytes is infinite or none: words of FP32 (W = 2), or halves.
+template <int W>
+__device__ __forceinline__ bool not_finite(const uint4& x, bool bf) {
+    if constexpr (W == 2) {
+        const uint32_t e = 0x7f800000u;
+        return (x.x & e) == e || (x.y & e) == e || (x.z & e) == e || (x.w & e) == e;
+    } else {
+        const uint32_t e = bf ? 0x7f80u : 0x7c00u;
+        bool r = false;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t v = i == 0 ? x.x : (i == 1 ? x.y : (i == 2 ? x.z : x.w));
+            r = r || (v & e) == e || ((v >> 16) & e) == e;
+        }
+        return r;
+    }
+}
+
+// Eight neighbouring elements of a row of queries, zeros where there is none; at any address.
+template <typename T>
+__device__ __forceinline__ void load_queries(const T* x, bool there, bool wide, float (&v)[8]) {
+    if (wide && there) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(x), b = *reinterpret_cast<const float4*>(x + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 w = *reinterpret_cast<const uint4*>(x);
+            const T* const e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                v[j] = to_float(e[j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            v[j] = there ? to_float(x[j]) : 0.0f;
+        }
+    }
 }
 
 }  // namespace pages

@@ -5,8 +5,8 @@
 // a step adds up, and which key is which row, is free as long as both operands agree, so a lane takes eight neighbouring elements (16 bytes, 32 in FP32) of its
 // rows, and the eight or four lanes beside it the rest of the line. For V^T a lane has the same elements of four keys and pairs two keys' by a byte permute. P^T comes from
 // S^T's accumulators by transposing 8 x 8 pieces between lanes. A warp has chunks of 16 keys to itself, with its own maximum and sum; the values of a chunk are asked for
-// before its scores are worked out, the keys of the next one right after, so 8 KB (16-bit, head size 128) a warp are on their way all the time and no barrier is met
-// until the item ends. There the thread block's warps meet in shared memory.
+// before its scores are worked out, the keys of the next one right after, so 8 KB (16-bit, head size 128) a warp are on their way all the time. The work is cut among warps,
+// which never meet: an item of two chunks costs no barrier, and what the warps have of a long one the joining kernel adds up.
 //
 // Precision: 16-bit rows and pages are multiplied as they are, weights rounded to the pages' type (and added up as rounded, so that the rounding of a weight that
 // stands alone cancels). FP32 rows and weights are sums of three bfloat16 parts, or two half-precision parts with a power of two per row, against the pages' 16-bit
@@ -34,9 +34,8 @@ struct Stream {
     static constexpr int W = sizeof(C) / 2;                                  // 16-byte words of eight elements
     static constexpr int KB = HD / 32, VB = HD / 64;                         // runs of 32 elements (keys), of 64 (values)
     static constexpr bool AHEAD = HD * sizeof(C) <= 512;                     // whether a chunk's keys and values fit the registers; else they are asked for run by run
-    static constexpr int Q_BYTES = KB * QP * NB * 512;                       // queries in shared memory: [run][part][block of eight][lane] x 16 bytes
-    static constexpr int MERGE_BYTES = STREAM_WARPS * ROWS * (HD + 4) * 4;   // (rows of HD + 4 floats: eight lanes' columns fall into different banks)
-    static constexpr int SMEM = Q_BYTES > MERGE_BYTES ? Q_BYTES : MERGE_BYTES;
+    static constexpr int Q_BYTES = KB * QP * NB * 512;                       // a warp's queries in shared memory: [run][part][block of eight][lane] x 16 bytes
+    static constexpr int SMEM = STREAM_WARPS * Q_BYTES;
 };
 
 // Eight elements as pairs of numbers of the instruction: words of part `p`. FP32: x[0..1] hold them.
@@ -52,23 +51,6 @@ __device__ __forceinline__ void parts_of_run(const uint4 (&x)[W], uint32_t (&w)[
     }
 }
 
-template <int W>
-__device__ __forceinline__ bool not_finite(const uint4& x, bool bf) {
-    if constexpr (W == 2) {
-        const uint32_t e = 0x7f800000u;
-        return (x.x & e) == e || (x.y & e) == e || (x.z & e) == e || (x.w & e) == e;
-    } else {
-        const uint32_t e = bf ? 0x7f80u : 0x7c00u;
-        bool r = false;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t v = i == 0 ? x.x : (i == 1 ? x.y : (i == 2 ? x.z : x.w));
-            r = r || (v & e) == e || ((v >> 16) & e) == e;
-        }
-        return r;
-    }
-}
-
 template <typename T, typename C, int HD, int NB, int RESIDENT>
 __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel(AttendArgs a) {
     using S = Stream<T, C, HD, NB>;
@@ -77,25 +59,27 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
     constexpr int ROWS_SHIFT = NB == 1 ? 3 : 4, KEYS_SHIFT = 4;
     static_assert(ROWS == 1 << ROWS_SHIFT && CHUNK == 1 << KEYS_SHIFT, "");
     constexpr int PRODUCTS = KP > QP ? KP : QP;  // parts i and j meet where i + j < PRODUCTS
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ float2 ml[STREAM_WARPS][ROWS];
-    __shared__ float q_scale[ROWS];
+    extern __shared__ __align__(16) uint8_t all_smem[];
     asm volatile("griddepcontrol.launch_dependents;");
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    uint8_t* const smem = all_smem + warp * S::Q_BYTES;
     const Work& work = a.own;
+    const int worker = warp * (int)gridDim.x + (int)blockIdx.x;  // (few workers: on different SMs)
     const Cut cut = cut_of(work, units_before(a, work, work.last, lane));
-    int64_t begin = (int64_t)blockIdx.x * cut.per;
+    int64_t begin = (int64_t)worker * cut.per;
     if (begin >= cut.total) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     const int64_t end = begin + cut.per < cut.total ? begin + cut.per : cut.total;
     int64_t base;
     int s = find_unit(a, work, begin, lane, base);
     Sequence sq = sequence_at(a, s, ROWS_SHIFT, KEYS_SHIFT);
+    const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
     const C* const k_pages = static_cast<const C*>(a.k_pages);
     const C* const v_pages = static_cast<const C*>(a.v_pages);
     while (begin < end) {
-        // ---- the next item, or the part of it that is this thread block's
+        // ---- the next item, or the part of it that is this warp's
         while (begin >= base + sq.units(a.kv_heads)) {
             base += sq.units(a.kv_heads);
             sq = sequence_at(a, ++s, ROWS_SHIFT, KEYS_SHIFT);
@@ -107,58 +91,51 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
         const int rows = sq.rows * a.group, row0 = block * ROWS;  // rows of the group: token * group + head
         const int* const table = prefix ? a.b.prefix : a.b.tables + s * a.b.table_stride;
         auto limit_of = [&](int r) { return row0 + r < rows ? keys_seen(a, sq, s, (row0 + r) / a.group) : sq.keys; };  // keys that row r of the block sees
-        __syncthreads();  // (shared memory is free again)
-        // ---- queries: rows of the block as the instruction's second operand
-        if constexpr (QP == 2) {  // a power of two per row takes the largest magnitude to [2^9, 2^10)
-            for (int r = warp; r < ROWS; r += STREAM_WARPS) {
-                float top = 0.0f;
-                if (row0 + r < rows) {
-                    const T* x = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + (row0 + r) / a.group) * a.qt + (int64_t)(kvh * a.group + (row0 + r) % a.group) * a.qh;
-                    for (int d = lane; d < HD; d += 32) {
-                        top = fmaxf(top, fabsf(to_float(x[d])));
+        float q_scale[NB][2];
+        __syncwarp();  // (the last item's queries are done with)
+        // ---- queries: rows of the block as the instruction's second operand. A lane has eight elements of a run of row g of every block of eight
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const int r = row0 + nb * 8 + g;
+            const bool there = r < rows;
+            const T* const x = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + (there ? r / a.group : 0)) * a.qt + (int64_t)(kvh * a.group + (there ? r % a.group : 0)) * a.qh + t * 8;
+            float v[KB][8];
+            float top = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                load_queries<T>(x + kb * 32, there, wide, v[kb]);
+                if constexpr (QP == 2) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        top = fmaxf(top, fabsf(v[kb][j]));
                     }
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                }
-                if (lane == 0) {
-                    uint32_t e = __float_as_uint(top) >> 23;
-                    e = e < 20u ? 20u : (e > 250u ? 250u : e);
-                    q_scale[r] = __uint_as_float((e - 9u) << 23);
-                }
             }
-            __syncthreads();
-        }
-        for (int i = tid; i < KB * NB * 32; i += STREAM_THREADS) {
-            const int l = i & 31, nb = (i >> 5) % NB, kb = (i >> 5) / NB, r = nb * 8 + (l >> 2);
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                v[j] = 0.0f;
-            }
-            if (row0 + r < rows) {
-                const T* x = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + (row0 + r) / a.group) * a.qt + (int64_t)(kvh * a.group + (row0 + r) % a.group) * a.qh + kb * 32 + (l & 3) * 8;
-                float up = 1.0f;
-                if constexpr (QP == 2) {
-                    up = 1.0f / q_scale[r];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    v[j] = to_float(x[j]) * up;
-                }
-            }
-            uint32_t w[4][QP];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                split_pair<BF, QP>(v[2 * j], v[2 * j + 1], w[j]);
+            float up = 1.0f;
+            if constexpr (QP == 2) {  // a power of two per row takes the largest magnitude to [2^9, 2^10)
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                uint32_t e = __float_as_uint(top) >> 23;
+                e = e < 20u ? 20u : (e > 250u ? 250u : e);
+                up = __uint_as_float((263u - e) << 23);
+                const float down = __uint_as_float((e - 9u) << 23);
+                q_scale[nb][0] = __shfl_sync(0xffffffffu, down, 8 * t);  // of the rows that are this lane's columns
+                q_scale[nb][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
             }
 #pragma unroll
-            for (int p = 0; p < QP; p++) {
-                *reinterpret_cast<uint4*>(smem + (((kb * QP + p) * NB + nb) * 32 + l) * 16) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+            for (int kb = 0; kb < KB; kb++) {
+                uint32_t w[4][QP];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    split_pair<BF, QP>(v[kb][2 * j] * up, v[kb][2 * j + 1] * up, w[j]);
+                }
+#pragma unroll
+                for (int p = 0; p < QP; p++) {
+                    *reinterpret_cast<uint4*>(smem + (((kb * QP + p) * NB + nb) * 32 + lane) * 16) = make_uint4(w[0][p], w[1][p], w[2][p], w[3][p]);
+                }
             }
         }
-        __syncthreads();
+        __syncwarp();
         const float to_log2 = a.scale * LOG2E;
         float factor[NB][2];
         int limit[NB][2], least = sq.keys;
@@ -170,7 +147,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 limit[nb][c] = limit_of(r);
                 factor[nb][c] = to_log2;
                 if constexpr (QP == 2) {
-                    factor[nb][c] *= q_scale[r];
+                    factor[nb][c] *= q_scale[nb][c];
                 }
             }
         }
@@ -223,13 +200,13 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
             }
         };
-        int c = c0 + warp;
-        int page = page_of(c), page_next = page_of(c + STREAM_WARPS);
+        int c = c0;
+        int page = page_of(c), page_next = page_of(c + 1);
         int64_t at = rows_at(c, page);
         if (S::AHEAD && c < c1) {
             load_k(at, sq.keys - c * CHUNK, 0);
         }
-        for (; c < c1; c += STREAM_WARPS) {
+        for (; c < c1; c++) {
             const int left = sq.keys - c * CHUNK;  // keys from here on
             if constexpr (S::AHEAD) {
                 load_v(at, left, 0);
@@ -268,10 +245,10 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 note_status(a.status, STATUS_PAGE);
             }
             page = page_next;
-            page_next = page_of(c + 2 * STREAM_WARPS);
-            at = rows_at(c + STREAM_WARPS, page);
-            if (S::AHEAD && c + STREAM_WARPS < c1) {
-                load_k(at, left - CHUNK * STREAM_WARPS, 0);
+            page_next = page_of(c + 2);
+            at = rows_at(c + 1, page);
+            if (S::AHEAD && c + 1 < c1) {
+                load_k(at, left - CHUNK, 0);
             }
             const bool edge = c * CHUNK + CHUNK > least || at_now < 0;  // some row does not see all of the chunk
             // ---- scores that are not numbers: in parts an infinity is infinity - infinity too. They are worked out again, one product after the other
@@ -465,9 +442,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
             }
         }
-        // ---- the warps meet
-        __syncthreads();  // (the queries are done with)
-        float* const meet = reinterpret_cast<float*>(smem);
+        // ---- what the warp has of the item. A lane has elements 64 v + 8 g + 2 i and the one behind it of rows 2 t and 2 t + 1
+        const bool complete = c0 == 0 && c1 == sq.chunks;
+        constexpr float DOWN = QP == 2 ? 1.0f / 32768.0f : 1.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
@@ -477,66 +454,36 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                     l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], o);
                 }
                 const int r = nb * 8 + 2 * t + j;
-                if (g == 0) {
-                    ml[warp][r] = make_float2(m[nb][j], l[nb][j]);
+                if (row0 + r >= rows) {
+                    continue;
                 }
-                float* const to = meet + (warp * ROWS + r) * (HD + 4);
+                const int64_t token = sq.row0 + (row0 + r) / a.group;
+                const int head = kvh * a.group + (row0 + r) % a.group;
+                if (complete && !a.joined) {
+                    T* const y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
+#pragma unroll
+                    for (int i = 0; i < 2 * KB; i++) {
+                        const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
+                        y[d] = from_float<T>(over(acc[nb][i][j] * DOWN, l[nb][j]));
+                        y[d + 1] = from_float<T>(over(acc[nb][i][j + 2] * DOWN, l[nb][j]));
+                    }
+                    continue;
+                }
+                const int64_t at = complete ? ((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head : ((int64_t)worker * 2 + (c0 == 0 ? 1 : 0)) * ROWS + r;
+                float* const to = (complete ? a.whole : work.part) + at * HD;
+                if (g == 0) {
+                    (complete ? a.whole_ml : work.part_ml)[at] = make_float2(m[nb][j], l[nb][j]);
+                }
 #pragma unroll
                 for (int i = 0; i < 2 * KB; i++) {
-                    const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
-                    *reinterpret_cast<float2*>(to + d) = make_float2(acc[nb][i][j], acc[nb][i][j + 2]);
-                }
-            }
-        }
-        __syncthreads();
-        const bool complete = c0 == 0 && c1 == sq.chunks;
-        constexpr float DOWN = QP == 2 ? 1.0f / 32768.0f : 1.0f;
-        for (int i = tid; i < ROWS * (HD / 4); i += STREAM_THREADS) {
-            const int r = i / (HD / 4), d = i % (HD / 4) * 4;
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < STREAM_WARPS; w++) {
-                top = fmaxf(top, ml[w][r].x);
-            }
-            const float from = top == -INFINITY ? 0.0f : top;
-            float sum = 0.0f;
-            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < STREAM_WARPS; w++) {
-                const float f = exp2_fast(ml[w][r].x - from);
-                sum = fmaf(f, ml[w][r].y, sum);
-                const float4 v = *reinterpret_cast<const float4*>(meet + (w * ROWS + r) * (HD + 4) + d);
-                const float fd = f * DOWN;
-                o.x = fmaf(fd, v.x, o.x); o.y = fmaf(fd, v.y, o.y); o.z = fmaf(fd, v.z, o.z); o.w = fmaf(fd, v.w, o.w);
-            }
-            if (row0 + r < rows) {
-                if (!complete) {
-                    const int64_t slot = (int64_t)blockIdx.x * 2 + (c0 == 0 ? 1 : 0);
-                    *reinterpret_cast<float4*>(work.part + (slot * ROWS + r) * HD + d) = o;
-                    if (d == 0) {
-                        work.part_ml[slot * ROWS + r] = make_float2(top, sum);
-                    }
-                } else {
-                    const int64_t token = sq.row0 + (row0 + r) / a.group;
-                    const int head = kvh * a.group + (row0 + r) % a.group;
-                    if (a.joined) {
-                        const int64_t to = ((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head;
-                        *reinterpret_cast<float4*>(a.whole + to * HD + d) = o;
-                        if (d == 0) {
-                            a.whole_ml[to] = make_float2(top, sum);
-                        }
-                    } else {
-                        T* y = static_cast<T*>(a.out) + token * a.ot + head * a.oh + d;
-                        y[0] = from_float<T>(over(o.x, sum));
-                        y[1] = from_float<T>(over(o.y, sum));
-                        y[2] = from_float<T>(over(o.z, sum));
-                        y[3] = from_float<T>(over(o.w, sum));
-                    }
+                    *reinterpret_cast<float2*>(to + (i >> 2) * 64 + g * 8 + (i & 3) * 2) = make_float2(acc[nb][i][j] * DOWN, acc[nb][i][j + 2] * DOWN);
                 }
             }
         }
         begin = item0 + c1;
     }
+    // (behind the tile kernel: what waits for this kernel has waited for that one)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace pages

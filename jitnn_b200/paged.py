@@ -279,7 +279,7 @@ class PagedCache:
         if q.shape[0]:
             L = _lib.load()
             need = ctypes.c_int64()
-            check(L.jq_pages_attention_bytes(h, q.shape[1], q.shape[0], batch._rows[5], batch.prefix_length, ctypes.byref(need)))
+            check(L.jq_pages_attention_bytes(h, code, q.shape[1], q.shape[0], batch._rows[5], batch.prefix_length, ctypes.byref(need)))
             space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
             strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), y.stride(0), y.stride(1))
             check(L.jq_pages_attention(h, code, q.shape[1], q.data_ptr(), y.data_ptr(), strides, q.shape[0], *batch._rows, *batch._ahead,
