@@ -3,6 +3,7 @@
 #include <new>
 
 #include "jq_pages.cuh"
+#include "jq_tc.cuh"
 
 namespace jq {
 namespace {
@@ -212,7 +213,7 @@ JQ_API int jq_pages_create(int device, int elem, int64_t pages, int page_size, i
     if (!elem_ok(elem)) {
         return fail(JQ_ERR_INVALID, "jq_pages_create: element type %d", elem);
     }
-    if (pages < 1 || pages > 0x7fffffff || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
+    if (pages < 1 || pages > 0x7fffffff / (kv_heads > 0 ? kv_heads : 1) || page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0) {
         return fail(JQ_ERR_INVALID, "jq_pages_create: %lld pages of %d keys (a power of two from 16 to 1024)", (long long)pages, page_size);
     }
     if (kv_heads < 1 || kv_heads > 1024 || head_dim < 2 || head_dim % 2 != 0 || head_dim > 256) {
@@ -239,7 +240,23 @@ JQ_API int jq_pages_create(int device, int elem, int64_t pages, int page_size, i
     if (p == nullptr) {
         return fail(JQ_ERR_OOM, "jq_pages_create: out of host memory");
     }
-    *p = jq_pages{JQ_PAGES_MAGIC, device, elem, page_size, kv_heads, head_dim, pages, k, v};
+    *p = jq_pages{JQ_PAGES_MAGIC, device, elem, page_size, kv_heads, head_dim, pages, k, v, {}, {}};
+    if (elem != JQ_ELEM_F32 && (head_dim == 64 || head_dim == 128)) {
+        const EncodeTiledFn encode = encode_tiled();
+        bool made = encode != nullptr;
+        for (int i = 0; i < 2 && made; i++) {
+            const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)page_size, (cuuint64_t)pages * kv_heads};
+            const cuuint64_t strides[2] = {(cuuint64_t)head_dim * 2, (cuuint64_t)page_size * head_dim * 2};
+            const cuuint32_t box[3] = {64, (cuuint32_t)(page_size < BOX_KEYS ? page_size : BOX_KEYS), 1}, steps[3] = {1, 1, 1};
+            made = encode(i == 0 ? &p->k_map : &p->v_map, elem == JQ_ELEM_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, i == 0 ? k : v, dims,
+                          strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        }
+        if (!made) {
+            delete p;
+            return fail(JQ_ERR_CUDA, "jq_pages_create: no tensor map of %lld pages", (long long)pages);
+        }
+    }
     *out = p;
     return JQ_OK;
 }

@@ -1,12 +1,15 @@
 // What the operators of paged decoding share: element types, the handles, and how a row of a batch finds its sequence.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include "jq_common.cuh"
 
 namespace jq {
+
+constexpr int BOX_KEYS = 128;  // of a tensor map's box, where a page has as many
 
 inline int elem_bytes(int elem) { return elem == JQ_ELEM_F32 ? 4 : 2; }
 inline bool elem_ok(int elem) { return elem == JQ_ELEM_F32 || elem == JQ_ELEM_F16 || elem == JQ_ELEM_BF16; }
@@ -65,6 +68,7 @@ struct jq_pages {
     int page_size, kv_heads, head_dim;
     int64_t pages;
     void *k, *v;     // [pages][kv_heads][page_size][head_dim], the caller's
+    CUtensorMap k_map, v_map;  // of 16-bit pages with heads of 64 or 128: boxes of 64 elements of up to 128 keys
 };
 #define JQ_ROPE_MAGIC 0x4a51524fu
 #define JQ_PAGES_MAGIC 0x4a515047u

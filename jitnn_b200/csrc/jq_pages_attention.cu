@@ -177,8 +177,8 @@ int large_smem(K kernel, int smem, std::atomic<uint64_t>& configured) {  // the 
 }
 
 // Behind a kernel of this call (`behind`): programmatically, all of this call's kernels but the joining one work at the same time.
-template <typename K>
-int launch_part(K kernel, dim3 grid, int threads, int smem, bool behind, const AttendArgs& a, cudaStream_t s) {
+template <typename K, typename... More>
+int launch_part(K kernel, dim3 grid, int threads, int smem, bool behind, cudaStream_t s, const AttendArgs& a, const More&... more) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -189,7 +189,7 @@ int launch_part(K kernel, dim3 grid, int threads, int smem, bool behind, const A
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    JQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
+    JQ_CUDA(cudaLaunchKernelEx(&cfg, kernel, a, more...));
     count_launch();
     return JQ_OK;
 }
@@ -200,18 +200,18 @@ int launch_stream(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
     constexpr int smem = pages::Stream<T, C, HD, NB>::SMEM;
     auto kernel = pages::attend_stream_kernel<T, C, HD, NB, stream_resident(HD, sizeof(C))>;
     const int rc = smem > 48 * 1024 ? large_smem(kernel, smem, configured) : JQ_OK;
-    return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, plan.tile_workers > 0, a, s);
+    return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, plan.tile_workers > 0, s, a);
 }
 
 template <typename T, typename C, int HD>
-int launch_attend_head(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
+int launch_attend_head(const jq_pages* p, const AttendArgs& a, const Plan& plan, cudaStream_t s) {
     int rc = JQ_OK;
     if constexpr (sizeof(C) == 2 && HD <= 128) {
         if (plan.tile_workers > 0) {
             static std::atomic<uint64_t> configured{0};
             constexpr int smem = pages::Tile<T, C, HD>::SMEM;
             rc = large_smem(pages::attend_tile_kernel<T, C, HD>, smem, configured);
-            rc = rc != JQ_OK ? rc : launch_part(pages::attend_tile_kernel<T, C, HD>, dim3((unsigned)plan.tile_workers), pages::TILE_THREADS, smem, false, a, s);
+            rc = rc != JQ_OK ? rc : launch_part(pages::attend_tile_kernel<T, C, HD>, dim3((unsigned)plan.tile_workers), pages::TILE_THREADS, smem, false, s, a, p->k_map, p->v_map);
         }
     }
     if (rc == JQ_OK && plan.rows == 8) {
@@ -222,15 +222,15 @@ int launch_attend_head(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
             rc = launch_stream<T, C, HD, 2>(a, plan, s);
         }
     }
-    return rc != JQ_OK ? rc : launch_part(pages::attend_join_kernel<T, HD>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, a, s);
+    return rc != JQ_OK ? rc : launch_part(pages::attend_join_kernel<T, HD>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, s, a);
 }
 
 template <typename T, typename C>
-int launch_attend(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
+int launch_attend(const jq_pages* p, const AttendArgs& a, const Plan& plan, cudaStream_t s) {
     switch (a.head_dim) {
-        case 64: return launch_attend_head<T, C, 64>(a, plan, s);
-        case 128: return launch_attend_head<T, C, 128>(a, plan, s);
-        case 256: return launch_attend_head<T, C, 256>(a, plan, s);
+        case 64: return launch_attend_head<T, C, 64>(p, a, plan, s);
+        case 128: return launch_attend_head<T, C, 128>(p, a, plan, s);
+        case 256: return launch_attend_head<T, C, 256>(p, a, plan, s);
         default: break;
     }
     attend_row_kernel<T, C><<<dim3((unsigned)a.b.tokens, (unsigned)a.heads), 128, 0, s>>>(a);
@@ -299,7 +299,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(space + at); };
     auto pairs = [&](int64_t at) { return reinterpret_cast<float2*>(space + at); };
     const int ahead = prefix_length > 0 ? 1 : 0;
-    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 6, plan.tile_workers, 1, floats(plan.tile_part), pairs(plan.tile_part_ml)};
+    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 7, plan.tile_workers, 1, floats(plan.tile_part), pairs(plan.tile_part_ml)};
     const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, 1, floats(plan.part), pairs(plan.part_ml)};
     a.own = plan.tile_own ? tile : few;
     a.pre = plan.tile_workers > 0 ? tile : few;
@@ -319,15 +319,15 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     }
     const cudaStream_t s = (cudaStream_t)stream;
     if (elem == JQ_ELEM_F16) {
-        return launch_attend<__half, __half>(a, plan, s);
+        return launch_attend<__half, __half>(p, a, plan, s);
     }
     if (elem == JQ_ELEM_BF16) {
-        return launch_attend<__nv_bfloat16, __nv_bfloat16>(a, plan, s);
+        return launch_attend<__nv_bfloat16, __nv_bfloat16>(p, a, plan, s);
     }
     if (p->elem == JQ_ELEM_F16) {
-        return launch_attend<float, __half>(a, plan, s);
+        return launch_attend<float, __half>(p, a, plan, s);
     }
-    return p->elem == JQ_ELEM_BF16 ? launch_attend<float, __nv_bfloat16>(a, plan, s) : launch_attend<float, float>(a, plan, s);
+    return p->elem == JQ_ELEM_BF16 ? launch_attend<float, __nv_bfloat16>(p, a, plan, s) : launch_attend<float, float>(p, a, plan, s);
 }
 
 }  // extern "C"

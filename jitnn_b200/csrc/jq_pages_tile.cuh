@@ -1,14 +1,20 @@
 // The tile kernel of the paged attention: many rows a key/value head, on the tensor cores. Blocks of 128 rows (tokens and heads that share a key/value head: all of a batch, where
-// the keys are the prefix) against tiles of 64 keys.
+// the keys are the prefix) against tiles of 128 keys.
 //
-// A thread has a row, that is a lane of tensor memory. S = Q K^T (tcgen05.mma, 128 x 64, both from shared memory), the thread reads its scores, keeps its maximum and sum, writes
-// its weights over the scores, O = P V (weights from tensor memory, values as they lie on the pages: elements of a head are the second operand's columns), and adds O to its
-// sums in registers with the factor of the maximum: the instruction cuts off where it adds, so it only adds up a tile. O is read when the next weights are worked out, and the
-// scores of the tile behind that are made while those weights are written; keys and values come by asynchronous copies (16 bytes, through the table of pages) a tile or two ahead.
+// Warps 0 to 7, two threads a row (a lane of tensor memory), each half of a tile's keys and half of a head's elements: queries into shared memory, then per tile the maximum of
+// the row's scores, its weights and their sum; and the sums over the values in registers. (With one thread a row a warp alone on its scheduler took five clocks an instruction.)
+// Warp 8 brings keys and values by tensor-map copies, a box for every page that a tile touches, and issues the products: S = Q K^T (tcgen05.mma,
+// 128 x 128, both operands in shared memory), O = P V (weights from tensor memory; values as they lie on the pages, elements of a head are the second operand's columns).
+// The instruction cuts off where it adds, so O only adds up a tile, and the threads add the tiles with the factor of the maximum (a sum of 8192 keys held in it was 4e-6 off).
+// For 16-bit rows two thread blocks share an SM, one's products under the other's exponentials: weights take the place of the scores. FP32 rows are two half-precision
+// parts (with a power of two per row) or three bfloat16 parts, so many products for one, and weights likewise; their weights have columns of their own and, with
+// two parts, the scores two buffers, so that the next tile's are made meanwhile.
 //
-// Per tile and SM the products take 512 clocks at head size 128, the threads' part (64 exponentials, 128 sums, about 600 instructions a warp) as long as that and more,
-// the copies 1400 clocks where the pages come from memory: two thread blocks share an SM for 16-bit rows. FP32 rows are two half-precision parts (with a power of
-// two per row) or three bfloat16 parts, which are so many products for one, and weights likewise.
+// A row that does not see a key must not get anything of it, and 0 x NaN is one: in tiles that not every row sees whole, values that are not finite, and those behind the last key,
+// are cleared in shared memory, and the rows that do see such a key add it by themselves.
+//
+// Bound per tile and SM: the products' 1024 clocks at head size 128 (times the parts), the threads' 128 exponentials (1024 clocks at 16 a clock) and about 700 instructions a
+// warp, or 2800 clocks for 64 KB of pages where they come from memory.
 #pragma once
 
 #include "jq_pages_attention.cuh"
@@ -18,7 +24,7 @@
 namespace jq {
 namespace pages {
 
-constexpr int TILE_THREADS = 128, TILE_BLOCK = 128, TILE_KEYS = 64;
+constexpr int TILE_BLOCK = 128, TILE_KEYS = 128, TILE_ROW_THREADS = 2 * TILE_BLOCK, TILE_THREADS = TILE_ROW_THREADS + 32;
 
 template <typename T, typename C, int HD>
 struct Tile {
@@ -27,10 +33,16 @@ struct Tile {
     static constexpr int QP = sizeof(T) == 2 ? 1 : (BF ? 3 : 2);   // parts of queries and weights
     static constexpr int DB = HD / 64;                             // runs of 64 elements: 128-byte rows of the operands
     static constexpr int Q_PART = DB * TILE_BLOCK * 128, KV = DB * TILE_KEYS * 128;
-    static constexpr int SMEM = 1024 + QP * Q_PART + 4 * KV;       // queries, two tiles of keys, two of values, on a 1024-byte boundary
     static constexpr int RESIDENT = QP == 1 ? 2 : 1;
-    static constexpr int BUF = QP == 3 ? 96 : 64;                  // columns of a tile's scores, and of its weights after that
-    static constexpr int COLS = 2 * BUF + HD <= 256 ? 256 : 512;
+    static constexpr int KS = QP == 1 && HD == 128 ? 1 : 2, VS = QP != 2 && HD == 128 ? 1 : 2;  // tiles of keys, and of values, in shared memory
+    static constexpr int SMEM = 1024 + QP * Q_PART + (KS + VS) * KV;
+    static constexpr int BUFS = QP == 2 ? 2 : 1;                   // of scores
+    static constexpr bool ALIAS = QP == 1;                         // weights in the scores' columns
+    static constexpr int P_AT = ALIAS ? 0 : BUFS * TILE_KEYS, O_AT = ALIAS ? TILE_KEYS : P_AT + QP * (TILE_KEYS / 2);
+    // where the weights of the second half of the keys begin: in the scores' place, over scores that the same thread has read
+    static constexpr int P_HALF = ALIAS ? TILE_KEYS / 2 : TILE_KEYS / 4;
+    static constexpr int CHUNK = RESIDENT == 2 ? 16 : 32;          // scores that a thread holds at a time
+    static constexpr int COLS = O_AT + HD <= 256 ? 256 : 512;
     static constexpr uint32_t TYPES = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TILE_BLOCK >> 4) << 24);
     static constexpr uint32_t IDESC_S = TYPES | ((uint32_t)(TILE_KEYS >> 3) << 17);
     static constexpr uint32_t IDESC_O = TYPES | ((uint32_t)(HD >> 3) << 17) | (1u << 16);  // the second operand's columns are next to each other
@@ -71,6 +83,31 @@ __device__ __forceinline__ void tile_ld32(float* r, uint32_t addr) {
         r[i] = __uint_as_float(u[i]);
     }
 }
+__device__ __forceinline__ void tile_ld16(float* r, uint32_t addr) {
+    uint32_t u[16];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]),
+                   "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(addr)
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        r[i] = __uint_as_float(u[i]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void tile_ld(float* r, uint32_t addr) {
+    if constexpr (N == 32) {
+        tile_ld32(r, addr);
+    } else {
+        tile_ld16(r, addr);
+    }
+}
+__device__ __forceinline__ void tile_st8(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ float tile_ld1(uint32_t addr) {
     uint32_t u;
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(u) : "r"(addr) : "memory");
@@ -88,41 +125,79 @@ __device__ __forceinline__ void tile_st16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tile_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Sixteen bytes into shared memory, zeros where `there` is false (nothing is read then).
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_done() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// A box of the pages: 64 elements of a head's keys (or values) from key `slot` of page `page` on.
+__device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, uint32_t bar, int element, int slot, int page) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(to), "l"(map), "r"(bar), "r"(element),
+                 "r"(slot), "r"(page)
+                 : "memory");
 }
 
+// What all of a thread block's roles go through alike: its items, each a run of tiles.
+struct Item {
+    int s, kvh, row0, rows, c0, c1;
+    bool prefix, complete;
+};
+struct Items {
+    int64_t begin, end, base;
+    int s;
+    Sequence sq;
+    __device__ __forceinline__ bool next(const AttendArgs& a, Item& it) {
+        if (begin >= end) {
+            return false;
+        }
+        while (begin >= base + sq.units(a.kv_heads)) {
+            base += sq.units(a.kv_heads);
+            sq = sequence_at(a, ++s, 7, 7);
+        }
+        const int64_t item = (begin - base) / sq.chunks, item0 = base + item * sq.chunks;
+        it.s = s;
+        it.prefix = s == a.b.sequences;
+        it.kvh = (int)(item / sq.blocks);
+        it.row0 = (int)(item % sq.blocks) * TILE_BLOCK;
+        it.rows = sq.rows * a.group;
+        it.c0 = (int)(begin - item0);
+        it.c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
+        it.complete = it.c0 == 0 && it.c1 == sq.chunks;
+        begin = item0 + it.c1;
+        return true;
+    }
+};
+
 template <typename T, typename C, int HD>
-__global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT) attend_tile_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
+    attend_tile_kernel(AttendArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     using L = Tile<T, C, HD>;
     constexpr bool BF = L::BF;
-    constexpr int QP = L::QP, BUF = L::BUF;
+    constexpr int QP = L::QP, KS = L::KS, VS = L::VS;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ __align__(8) uint64_t bars[3];
+    __shared__ __align__(8) uint64_t bars[2 * (KS + VS) + 5];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_word;
+    __shared__ int abort_word, gone_ring[4];
+    __shared__ uint32_t bad_keys[2][4];
+    __shared__ float tops[2][2][TILE_BLOCK], sums[TILE_BLOCK];  // of either half
+    __shared__ int64_t row_q[TILE_BLOCK], row_out[TILE_BLOCK];  // where a row's queries are, and its results go; -1: there is no such row
     asm volatile("griddepcontrol.launch_dependents;");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Work& work = a.pre;
     const Cut cut = cut_of(work, units_before(a, work, work.last, lane));
-    int64_t begin = (int64_t)blockIdx.x * cut.per;
-    if (begin >= cut.total) {
+    Items items;
+    items.begin = (int64_t)blockIdx.x * cut.per;
+    if (items.begin >= cut.total) {
         return;
     }
-    const int64_t end = begin + cut.per < cut.total ? begin + cut.per : cut.total;
+    items.end = items.begin + cut.per < cut.total ? items.begin + cut.per : cut.total;
+    items.s = find_unit(a, work, items.begin, lane, items.base);
+    items.sq = sequence_at(a, items.s, 7, 7);
     const uint32_t smem = (tc::smem_u32(raw_smem) + 1023u) & ~1023u;
-    const uint32_t q_s = smem, k_s = smem + QP * L::Q_PART, v_s = k_s + 2 * L::KV;
-    const uint32_t s_bar = tc::smem_u32(&bars[0]), o_bar = tc::smem_u32(&bars[2]);  // scores of either buffer; O
+    const uint32_t q_s = smem, k_s = smem + QP * L::Q_PART, v_s = k_s + KS * L::KV;
+    auto bar = [&](int i) { return tc::smem_u32(&bars[i]); };
+    constexpr int REST = 2 * (KS + VS);
+    const uint32_t k_full = bar(0), k_free = bar(KS), v_full = bar(2 * KS), v_free = bar(2 * KS + VS);  // one for each stage
+    const uint32_t s_full = bar(REST), p_full = bar(REST + 2), o_full = bar(REST + 3), q_full = bar(REST + 4);
     volatile int* const abort_flag = &abort_word;
     if (tid == 0) {
-        for (int i = 0; i < 3; i++) {
-            tc::mbar_init(tc::smem_u32(&bars[i]), 1);
+        for (int i = 0; i < REST + 5; i++) {
+            tc::mbar_init(bar(i), i == REST + 2 || i == REST + 4 ? TILE_ROW_THREADS : 1);
         }
         abort_word = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -134,365 +209,495 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT) attend
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
-    const uint32_t tmem = tmem_slot, mine = tmem + ((uint32_t)warp << 21);  // (a warp's lanes: 32 from lane 32 warp on)
-    uint32_t s_phase = 0, o_phase = 0;  // s_phase: a bit for either buffer
-    int64_t base;
-    int s = find_unit(a, work, begin, lane, base);
-    Sequence sq = sequence_at(a, s, 7, 6);
-    const C* const k_pages = static_cast<const C*>(a.k_pages);
-    const C* const v_pages = static_cast<const C*>(a.v_pages);
-    const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
-    const float to_log2 = a.scale * 1.4426950408889634f;
-    bool ok = true;
-    while (begin < end && ok) {
-        while (begin >= base + sq.units(a.kv_heads)) {
-            base += sq.units(a.kv_heads);
-            sq = sequence_at(a, ++s, 7, 6);
-        }
-        const bool prefix = s == a.b.sequences;
-        const int64_t item = (begin - base) / sq.chunks, item0 = base + item * sq.chunks;
-        const int kvh = (int)(item / sq.blocks), block = (int)(item % sq.blocks);
-        const int c0 = (int)(begin - item0), c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
-        const int rows = sq.rows * a.group, row0 = block * TILE_BLOCK, r = row0 + tid;
-        const int* const table = prefix ? a.b.prefix : a.b.tables + s * a.b.table_stride;
-        const int limit = r < rows ? keys_seen(a, sq, s, r / a.group) : sq.keys, least = keys_seen(a, sq, s, row0 / a.group);
-        const T* const q = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + (r < rows ? r / a.group : 0)) * a.qt + (int64_t)(kvh * a.group + (r < rows ? r % a.group : 0)) * a.qh;
-        const int there = (c1 - c0);
-        // ---- copies: a thread has the same 16 bytes of every (128 / pieces of a row)th key
-        constexpr int PIECES = HD / 8, STEP = TILE_THREADS / PIECES, TIMES = TILE_KEYS / STEP;
-        const int piece = tid % PIECES, key_of = tid / PIECES;
-        auto copy_tile = [&](const C* pages, uint32_t to, int c) {
-            if (c < c1) {
-                int64_t at[TILE_KEYS / 16];
-#pragma unroll
-                for (int i = 0; i < TILE_KEYS / 16; i++) {
-                    const int key = c * TILE_KEYS + i * 16;
-                    const int page = key < sq.keys ? table[key >> a.page_shift] : -1;
-                    at[i] = page >= 0 && page < a.pages ? (((int64_t)page * a.kv_heads + kvh) * a.page_size + (key & (a.page_size - 1))) * HD : -1;
-                }
-#pragma unroll
-                for (int i = 0; i < TIMES; i++) {
-                    const int key = i * STEP + key_of;
-                    const int64_t from = at[i * STEP / 16];
-                    const bool real = from >= 0 && c * TILE_KEYS + key < sq.keys;
-                    copy16(to + (piece >> 3) * (TILE_KEYS * 128) + key * 128 + (((piece ^ key) & 7) << 4), pages + (real ? from + (key & 15) * HD + piece * 8 : 0), real);
-                }
-            }
-            copies_issued();
+    const uint32_t tmem = tmem_slot;
+    Item it;
+    // (a wait that gives up sets the abort flag, on which all others end too: every role goes on to its end without waiting or issuing anything)
+    auto wait = [&](uint32_t b, uint32_t parity, int code) { return tc::mbar_wait(b, parity, abort_flag, a.status, code, a.wait_clocks); };
+
+    if (warp == 8) {
+        // ---- copies and products. A lane has a box: 64 elements of the keys that a tile has of a page (of 128 of them), at most 16 boxes
+        const int box = a.page_size < TILE_KEYS ? a.page_size : TILE_KEYS, boxes = TILE_KEYS / box * L::DB;
+        const int my_run = lane % L::DB, my_key = lane / L::DB * box;
+        bool ok = true;
+        struct Cursor {  // the next tile whose keys, or values, are to be brought, numbered through the items
+            Items items;
+            Item it;
+            int c, n;
+            bool more;
         };
-        // (groups of copies: keys of tiles 0 and 1, values of 0, then keys of n + 2 and values of n + 1 in every turn n)
-        copy_tile(k_pages, k_s, c0);
-        copy_tile(k_pages, k_s + L::KV, c0 + 1);
-        copy_tile(v_pages, v_s, c0);
-        // ---- queries: a thread brings its row
-        float up = 1.0f, factor = to_log2;
-        if constexpr (QP == 2) {  // a power of two takes the row's largest magnitude to [2^9, 2^10)
-            float top = 0.0f;
-            for (int d = 0; d < HD; d += 8) {
-                float v[8];
-                load_queries<T>(q + d, r < rows, wide, v);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    top = fmaxf(top, fabsf(v[j]));
-                }
-            }
-            uint32_t e = __float_as_uint(top) >> 23;
-            e = e < 20u ? 20u : (e > 250u ? 250u : e);
-            up = __uint_as_float((263u - e) << 23);
-            factor *= __uint_as_float((e - 9u) << 23);
-        }
-#pragma unroll 4
-        for (int d = 0; d < HD; d += 8) {
-            float v[8];
-            load_queries<T>(q + d, r < rows, wide, v);
-            uint32_t w[4][QP];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                split_pair<BF, QP>(v[2 * j] * up, v[2 * j + 1] * up, w[j]);
-            }
-#pragma unroll
-            for (int p = 0; p < QP; p++) {
-                const uint32_t at = q_s + p * L::Q_PART + (d >> 6) * (TILE_BLOCK * 128) + tid * 128 + ((((d >> 3) ^ tid) & 7) << 4);
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0][p]), "r"(w[1][p]), "r"(w[2][p]), "r"(w[3][p]) : "memory");
-            }
-        }
-        // S of tile n (counted from the item's first) into its buffer
-        auto scores = [&](int n) {
-            const uint32_t kd = tile_desc(k_s + (n & 1) * L::KV), d = tmem + (n & 1) * BUF;
-            uint32_t more = 0;
-#pragma unroll
-            for (int p = QP - 1; p >= 0; p--) {  // smallest parts first
-                const uint32_t qd = tile_desc(q_s + p * L::Q_PART);
-#pragma unroll
-                for (int k = 0; k < HD / 16; k++) {
-                    tile_mma(d, qd + (k >> 2) * (TILE_BLOCK * 128 >> 4) + (k & 3) * 2, kd + (k >> 2) * (TILE_KEYS * 128 >> 4) + (k & 3) * 2, L::IDESC_S, more);
-                    more = 1;
-                }
-            }
-            tc::umma_commit(s_bar + 8 * (n & 1));
+        auto start = [&](Cursor& t) {
+            t.items = items;
+            t.n = 0;
+            t.more = t.items.next(a, t.it);
+            t.c = t.it.c0;
         };
-        copies_done<2>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
-        if (tid == 0) {
-            tc::fence_after_sync();
-            scores(0);
-        }
-        float acc[HD], m = -INFINITY, l = 0.0f, less = 0.0f;
-#pragma unroll
-        for (int i = 0; i < HD; i++) {
-            acc[i] = 0.0f;
-        }
-        // adds O of the tile before to the sums
-        auto add_o = [&]() {
-#pragma unroll
-            for (int h = 0; h < HD / 32; h++) {
-                float o[32];
-                tile_ld32(o, mine + 2 * BUF + 32 * h);
-                tile_ld_done();
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    acc[32 * h + i] = fmaf(acc[32 * h + i], less, o[i]);
-                }
+        auto bring = [&](Cursor& t, bool values) {
+            if (!ok || !t.more) {
+                return;
             }
-        };
-        bool pending = false;  // an O that has not been read
-        constexpr float UP = QP == 2 ? 32768.0f : 1.0f;  // (half-precision parts of weights: times 2^15)
-        for (int n = 0; n < there; n++) {
-            const int c = c0 + n, buf = n & 1;
-            // ---- scores are there, and the next tile's keys
-            ok = tc::mbar_wait(s_bar + 8 * buf, (s_phase >> buf) & 1, abort_flag, a.status, 10, a.wait_clocks);
-            s_phase ^= 1u << buf;
-            copies_done<1>();
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            tc::fence_before_sync();
-            ok = __syncthreads_and(ok);
-            if (!ok) {
-                break;
+            const int* const table = t.it.prefix ? a.b.prefix : a.b.tables + t.it.s * a.b.table_stride;
+            const int stages = values ? VS : KS, st = t.n % stages, key = t.c * TILE_KEYS + my_key;
+            const uint32_t full = (values ? v_full : k_full) + 8 * st;
+            int page = -1;
+            const bool mine = lane < boxes && key < t.items.sq.keys;
+            if (mine) {
+                page = table[key >> a.page_shift];
+                page = page >= 0 && page < a.pages ? page : -1;
             }
-            tc::fence_after_sync();
-            // (the keys' buffer of this tile is free: its scores are done. The tile behind the next follows)
-            copy_tile(k_pages, k_s + buf * L::KV, c + 2);
-            float x[TILE_KEYS];
-            tile_ld32(x, mine + buf * BUF);
-            tile_ld32(x + 32, mine + buf * BUF + 32);
-            tile_ld_done();
-            const int left = sq.keys - c * TILE_KEYS;  // keys from here on
-            const bool edge = c * TILE_KEYS + TILE_KEYS > least;
-            int holes = 0;  // a bit for every 16 keys whose page is not there
-#pragma unroll
-            for (int i = 0; i < TILE_KEYS / 16; i++) {
-                const int key = c * TILE_KEYS + i * 16;
-                const int page = key < sq.keys ? table[key >> a.page_shift] : 0;
-                holes |= page < 0 || page >= a.pages ? 1 << i : 0;
-            }
-            if constexpr (QP > 1) {  // in parts an infinity is infinity - infinity too: such scores are worked out again, one product after the other
-                bool odd = false;
-#pragma unroll
-                for (int i = 0; i < TILE_KEYS; i++) {
-                    odd = odd || x[i] != x[i];
-                }
-                if (__any_sync(0xffffffffu, odd)) {
-                    for (int key = 0; key < TILE_KEYS; key++) {
-                        float v = tile_ld1(mine + buf * BUF + key);
-                        if (v != v) {
-                            const int i = c * TILE_KEYS + key, page = i < sq.keys ? table[i >> a.page_shift] : -1;
-                            float sum = 0.0f;
-                            if (r < rows && page >= 0 && page < a.pages) {
-                                const C* const k = k_pages + (((int64_t)page * a.kv_heads + kvh) * a.page_size + (i & (a.page_size - 1))) * HD;
-                                for (int d = 0; d < HD; d++) {
-                                    sum = fmaf(to_float(q[d]) * up, to_float(k[d]), sum);
-                                }
-                            }
-                            v = sum;
-                        }
-                        tile_st1(mine + buf * BUF + key, v);
+            const unsigned there = __ballot_sync(0xffffffffu, page >= 0), missing = __ballot_sync(0xffffffffu, mine && page < 0);
+            if (lane == 0) {
+                ok = wait((values ? v_free : k_free) + 8 * st, ((t.n / stages) & 1) ^ 1, values ? 11 : 10);
+                if (!values) {
+                    int gone = 0;  // which keys are not there: a bit for each of the tile's sixteens
+                    for (int i = 0; i < TILE_KEYS / 16 && missing != 0u; i++) {
+                        gone |= (missing >> (i * 16 / box * L::DB) & 1) << i;
                     }
-                    tile_st_done();
-                    tile_ld32(x, mine + buf * BUF);
-                    tile_ld32(x + 32, mine + buf * BUF + 32);
-                    tile_ld_done();
+                    gone_ring[t.n & 3] = gone;
+                    if (gone != 0) {
+                        note_status(a.status, STATUS_PAGE);
+                    }
+                }
+                if (ok) {
+                    tc::mbar_expect_tx(full, (uint32_t)__popc(there) * box * 128);
                 }
             }
-            float f = factor;
-            if (!(factor > 0.0f)) {  // (the largest product is not that of the largest score)
-#pragma unroll
-                for (int i = 0; i < TILE_KEYS; i++) {
-                    x[i] *= factor;
-                }
-                f = 1.0f;
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (ok && page >= 0) {
+                copy_box((values ? v_s : k_s) + st * L::KV + my_run * (TILE_KEYS * 128) + my_key * 128, values ? &v_map : &k_map, full, my_run * 64,
+                         key & (a.page_size - 1), page * a.kv_heads + t.it.kvh);
             }
-            if (edge || holes != 0) {
-                if (holes != 0) {
-                    note_status(a.status, STATUS_PAGE);
-                }
-#pragma unroll
-                for (int i = 0; i < TILE_KEYS; i++) {
-                    x[i] = c * TILE_KEYS + i < limit && (holes >> (i / 16) & 1) == 0 ? x[i] : -INFINITY;
-                }
+            __syncwarp();
+            t.n++;
+            if (++t.c == t.it.c1) {
+                t.more = t.items.next(a, t.it);
+                t.c = t.it.c0;
             }
-            float top = x[0];
-#pragma unroll
-            for (int i = 1; i < TILE_KEYS; i++) {
-                top = fmaxf(top, x[i]);
-            }
-            top = fmaxf(top * f, m);
-            const float from = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(m - from);
-            m = top;
-            l *= shrink;
-#pragma unroll
-            for (int i = 0; i < TILE_KEYS; i++) {
-                x[i] = exp2_fast(fmaf(x[i], f, -from));
-            }
-            // ---- O of the tile before
-            if (pending) {
-                ok = tc::mbar_wait(o_bar, o_phase, abort_flag, a.status, 11, a.wait_clocks);
-                o_phase ^= 1;
+        };
+        Cursor kc, vc;
+        start(kc);
+        vc = kc;
+        bring(kc, false);
+        bring(vc, true);
+        if (KS > 1) {
+            bring(kc, false);
+        }
+        if (VS > 1) {
+            bring(vc, true);
+        }
+        int n = 0, ni = 0;
+        auto scores = [&](int k) {  // S of tile k
+            if (lane == 0) {
+                const int st = k % KS;
+                ok = ok && wait(k_full + 8 * st, (k / KS) & 1, 12);
                 tc::fence_after_sync();
-                if (__all_sync(0xffffffffu, ok)) {
-                    add_o();
-                }
-                pending = false;
-            }
-            // (the other buffer's weights have been used: the next tile's scores go there)
-            if (tid == 0 && ok && n + 1 < there) {
-                scores(n + 1);
-            }
-            less = shrink;
-            // ---- weights over the scores
-            uint32_t w[QP][16];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    uint32_t part[QP];
-                    split_pair<BF, QP>(x[32 * h + 2 * i] * UP, x[32 * h + 2 * i + 1] * UP, part);
-#pragma unroll
-                    for (int p = 0; p < QP; p++) {
-                        w[p][i] = part[p];
-                    }
-                    if constexpr (QP == 1) {
-                        if constexpr (BF) {
-                            l += __uint_as_float(part[0] << 16) + __uint_as_float(part[0] & 0xffff0000u);
-                        } else {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&part[0]));
-                            l += f.x + f.y;
-                        }
-                    } else {
-                        l += x[32 * h + 2 * i] + x[32 * h + 2 * i + 1];
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < QP; p++) {
-                    tile_st16(mine + buf * BUF + p * 32 + 16 * h, w[p]);
-                }
-            }
-            tile_st_done();
-            copies_done<1>();  // the tile's values
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            tc::fence_before_sync();
-            ok = __syncthreads_and(ok);
-            if (!ok) {
-                break;
-            }
-            tc::fence_after_sync();
-            // Where some row does not see a key whose value is not finite, its weight of zero would still make a NaN: then every thread adds the values up that its row sees
-            bool bad = false;
-            if (edge) {
-                for (int i = tid; i < L::KV / 16; i += TILE_THREADS) {
-                    const uint4 v = load_shared16_at(v_s + buf * L::KV + i * 16);
-                    bad = bad || not_finite<1>(v, BF);
-                }
-                bad = __syncthreads_or(bad);
-            }
-            if (!bad) {
-                if (tid == 0) {
-                    const uint32_t vd = tile_desc_values(v_s + buf * L::KV);
+                if (ok) {
+                    const uint32_t kd = tile_desc(k_s + st * L::KV), d = tmem + (k % L::BUFS) * TILE_KEYS;
                     uint32_t more = 0;
 #pragma unroll
-                    for (int p = QP - 1; p >= 0; p--) {
+                    for (int p = QP - 1; p >= 0; p--) {  // smallest parts first
+                        const uint32_t qd = tile_desc(q_s + p * L::Q_PART);
 #pragma unroll
-                        for (int k = 0; k < TILE_KEYS / 16; k++) {
-                            tile_mma_weights(tmem + 2 * BUF, tmem + buf * BUF + p * 32 + k * 8, vd + k * (16 * 128 >> 4), L::IDESC_O, more);
+                        for (int j = 0; j < HD / 16; j++) {
+                            tile_mma(d, qd + (j >> 2) * (TILE_BLOCK * 128 >> 4) + (j & 3) * 2, kd + (j >> 2) * (TILE_KEYS * 128 >> 4) + (j & 3) * 2, L::IDESC_S, more);
                             more = 1;
                         }
                     }
-                    tc::umma_commit(o_bar);
+                    tc::umma_commit(s_full + 8 * (k % L::BUFS));
+                    tc::umma_commit(k_free + 8 * st);
                 }
-                pending = true;
-            } else {
-#pragma unroll
-                for (int i = 0; i < HD; i++) {
-                    acc[i] *= less;
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        };
+        while (ok && items.next(a, it)) {
+            const int tiles = it.c1 - it.c0;
+            if (lane == 0) {
+                ok = wait(q_full, ni & 1, 13);
+            }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            scores(n);
+            for (int i = 0; i < tiles && ok; i++, n++) {
+                if (L::BUFS == 2 && i + 1 < tiles) {
+                    scores(n + 1);
                 }
-                for (int key = 0; key < TILE_KEYS && key < left; key++) {
-                    // (the parts of a weight, added up again)
-                    float p = 0.0f;
+                if (L::BUFS == 1) {
+                    bring(kc, false);  // (where the scores that are being made have their keys)
+                }
+                if (lane == 0) {
+                    const int st = n % VS;
+                    ok = ok && wait(p_full, n & 1, 14) && wait(v_full + 8 * st, (n / VS) & 1, 15);
+                    tc::fence_after_sync();
+                    if (ok) {
+                        const uint32_t vd = tile_desc_values(v_s + st * L::KV);
+                        uint32_t more = 0;
 #pragma unroll
-                    for (int i = 0; i < QP; i++) {
-                        const uint32_t pair = __float_as_uint(tile_ld1(mine + buf * BUF + i * 32 + (key >> 1)));
-                        const uint32_t half = (key & 1) != 0 ? pair >> 16 : pair & 0xffffu;
-                        p += BF ? __uint_as_float(half << 16) : __half2float(__ushort_as_half((unsigned short)half));
+                        for (int p = QP - 1; p >= 0; p--) {
+#pragma unroll
+                            for (int j = 0; j < TILE_KEYS / 16; j++) {
+                                tile_mma_weights(tmem + L::O_AT, tmem + L::P_AT + p * (TILE_KEYS / 2) + (j >> 2) * L::P_HALF + (j & 3) * 8, vd + j * (16 * 128 >> 4), L::IDESC_O,
+                                                 more);
+                                more = 1;
+                            }
+                        }
+                        tc::umma_commit(o_full);
+                        tc::umma_commit(v_free + 8 * st);
                     }
-                    if (c * TILE_KEYS + key < limit) {
+                }
+                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+                if (L::BUFS == 2) {
+                    bring(kc, false);
+                }
+                bring(vc, true);  // (waits for the product, with which the weights' columns are free as well)
+                if (L::BUFS == 1 && i + 1 < tiles) {
+                    if (L::ALIAS && lane == 0) {
+                        ok = ok && wait(o_full, n & 1, 16);
+                    }
+                    scores(n + 1);
+                }
+            }
+            ni++;
+        }
+        // copies that nobody has waited for are waited for here (with a limit): they write to this thread block's memory
+        if (!ok && lane == 0) {
+            const long long t0 = clock64();
+            for (int values = 0; values < 2; values++) {
+                const int stages = values ? VS : KS, upto = values ? vc.n : kc.n;
+                for (int i = upto > stages ? upto - stages : 0; i < upto; i++) {
+                    while (!tc::mbar_try((values ? v_full : k_full) + 8 * (i % stages), (i / stages) & 1) && clock64() - t0 < a.wait_clocks) {
+                    }
+                }
+            }
+        }
+    } else {
+        // ---- rows
+        const int half = warp >> 2, row = tid & (TILE_BLOCK - 1);
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // (a warp reaches 32 lanes, from lane 32 (warp % 4) on)
+        constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2, CH = L::CHUNK;  // of a thread
+        const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
+        auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(TILE_ROW_THREADS) : "memory"); };  // all of these warps
+        int n = 0;
+        bool ok = true;
+        while (items.next(a, it)) {
+            const Sequence& sq = items.sq;
+            const int r = it.row0 + row, tiles = it.c1 - it.c0, i_token = r / a.group, i_head = r - i_token * a.group;
+            const bool real = r < it.rows, direct = it.complete && !a.joined;
+            const int limit = real ? keys_seen(a, sq, it.s, i_token) : sq.keys, least = keys_seen(a, sq, it.s, it.row0 / a.group);
+            if (half == 0) {
+                const int64_t token = sq.row0 + i_token;
+                const int head = it.kvh * a.group + i_head;
+                row_q[row] = real ? token * a.qt + head * a.qh : -1;
+                row_out[row] = !real      ? -1
+                               : direct   ? token * a.ot + head * a.oh
+                               : it.complete ? (((it.prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head)
+                                             : ((int64_t)blockIdx.x * 2 + (it.c0 == 0 ? 1 : 0)) * TILE_BLOCK + row;
+            }
+            meet();
+            // ---- queries: LANES lanes bring a row, eight elements each; a warp has 16 rows, some of which are on their way at a time
+            {
+                constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 4;
+                const int d = lane % LANES * 8;
+#pragma unroll 1
+                for (int b = 0; b < 16; b += AT_ONCE * BATCH) {
+                    float v[BATCH][8];
 #pragma unroll
-                        for (int d = 0; d < HD; d += 8) {
-                            const uint4 v = load_shared16_at(v_s + buf * L::KV + (d >> 6) * (TILE_KEYS * 128) + key * 128 + ((((d >> 3) ^ key) & 7) << 4));
-                            const C* const e = reinterpret_cast<const C*>(&v);
+                    for (int i = 0; i < BATCH; i++) {
+                        const int64_t from = row_q[16 * warp + b + i * AT_ONCE + lane / LANES];
+                        load_queries<T>(static_cast<const T*>(a.q) + (from < 0 ? 0 : from) + d, from >= 0, wide, v[i]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < BATCH; i++) {
+                        const int k = 16 * warp + b + i * AT_ONCE + lane / LANES;
+                        if constexpr (QP == 2) {  // a power of two takes the row's largest magnitude to [2^9, 2^10)
+                            float top = 0.0f;
 #pragma unroll
                             for (int j = 0; j < 8; j++) {
-                                acc[d + j] = fmaf(p, to_float(e[j]), acc[d + j]);
+                                top = fmaxf(top, fabsf(v[i][j]));
                             }
+#pragma unroll
+                            for (int o = LANES / 2; o > 0; o >>= 1) {
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            }
+                            uint32_t e = __float_as_uint(top) >> 23;
+                            e = e < 20u ? 20u : (e > 250u ? 250u : e);
+                            const float by = __uint_as_float((263u - e) << 23);
+#pragma unroll
+                            for (int j = 0; j < 8; j++) {
+                                v[i][j] *= by;
+                            }
+                            sums[k] = by;
+                        }
+                        uint32_t w[4][QP];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            split_pair<BF, QP>(v[i][2 * j], v[i][2 * j + 1], w[j]);
+                        }
+#pragma unroll
+                        for (int p = 0; p < QP; p++) {
+                            const uint32_t at = q_s + p * L::Q_PART + (d >> 6) * (TILE_BLOCK * 128) + k * 128 + ((((d >> 3) ^ k) & 7) << 4);
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0][p]), "r"(w[1][p]), "r"(w[2][p]), "r"(w[3][p]) : "memory");
                         }
                     }
                 }
-                tc::fence_before_sync();
-                __syncthreads();  // (the values' buffer is free, and the weights')
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            tc::mbar_arrive(q_full);
+            float up = 1.0f, factor = a.scale * 1.4426950408889634f;
+            if constexpr (QP == 2) {
+                meet();
+                up = sums[row];
+                factor /= up;  // (exact)
+            }
+            float acc[DIMS], m = -INFINITY, l = 0.0f, less = 0.0f;
+#pragma unroll
+            for (int i = 0; i < DIMS; i++) {
+                acc[i] = 0.0f;
+            }
+            auto add_o = [&](int tile) {  // O of a tile to the sums
+                ok = wait(o_full, tile & 1, 17) && ok;
                 tc::fence_after_sync();
+#pragma unroll
+                for (int h = 0; h < DIMS / CH; h++) {
+                    float o[CH];
+                    tile_ld<CH>(o, mine + L::O_AT + half * DIMS + CH * h);
+                    tile_ld_done();
+#pragma unroll
+                    for (int i = 0; i < CH; i++) {
+                        acc[CH * h + i] = fmaf(acc[CH * h + i], less, o[i]);
+                    }
+                }
+            };
+            constexpr float UP = QP == 2 ? 32768.0f : 1.0f;  // (half-precision parts of weights: times 2^15)
+            const float f = factor > 0.0f ? factor : 1.0f;
+            for (int i = 0; i < tiles; i++, n++) {
+                const int key0 = (it.c0 + i) * TILE_KEYS + half * KEYS;  // this thread's first
+                const uint32_t scores = mine + (n % L::BUFS) * TILE_KEYS + half * KEYS;
+                ok = wait(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
+                tc::fence_after_sync();
+                const int gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3] >> (half * (KEYS / 16));
+                const bool edge = key0 - half * KEYS + TILE_KEYS > least || reinterpret_cast<volatile int*>(gone_ring)[n & 3] != 0;
+                auto load = [&](int h, float (&x)[CH]) {  // scores, minus infinity where the row does not see the key
+                    tile_ld<CH>(x, scores + CH * h);
+                    tile_ld_done();
+                    if (!(factor > 0.0f)) {  // (the largest product is not that of the largest score)
+#pragma unroll
+                        for (int j = 0; j < CH; j++) {
+                            x[j] *= factor;
+                        }
+                    }
+                    if (edge) {
+                        const int seen = limit - key0 - CH * h;
+#pragma unroll
+                        for (int j = 0; j < CH; j++) {
+                            x[j] = j < seen && (gone >> (CH / 16 * h + j / 16) & 1) == 0 ? x[j] : -INFINITY;
+                        }
+                    }
+                };
+                float top = -INFINITY, probe = 0.0f;
+                auto largest = [&] {
+#pragma unroll 1  // (a kernel's instructions come from memory too)
+                    for (int h = 0; h < KEYS / CH; h++) {
+                        float x[CH];
+                        load(h, x);
+#pragma unroll
+                        for (int j = 0; j < CH; j++) {
+                            top = fmaxf(top, x[j]);
+                            if constexpr (QP > 1) {
+                                probe = x[j] == -INFINITY ? probe : fmaf(x[j], 0.0f, probe);
+                            }
+                        }
+                    }
+                };
+                largest();
+                if constexpr (QP > 1) {  // in parts an infinity is infinity - infinity too: such scores are worked out again, one product after the other
+                    if (__any_sync(0xffffffffu, probe != probe)) {
+                        const int* const table = it.prefix ? a.b.prefix : a.b.tables + it.s * a.b.table_stride;
+#pragma unroll 1
+                        for (int key = 0; key < KEYS; key++) {
+                            float v = tile_ld1(scores + key);
+                            const int j = key0 + key;
+                            if (v != v && real && j < limit && (gone >> (key / 16) & 1) == 0) {
+                                const C* const k = static_cast<const C*>(a.k_pages) +
+                                                   (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD;
+                                const T* const q = static_cast<const T*>(a.q) + row_q[row];
+                                v = 0.0f;
+#pragma unroll 1
+                                for (int d = 0; d < HD; d++) {
+                                    v = fmaf(to_float(q[d]) * up, to_float(k[d]), v);
+                                }
+                            }
+                            tile_st1(scores + key, v);
+                        }
+                        tile_st_done();
+                        top = -INFINITY;
+                        largest();
+                    }
+                }
+                tops[n & 1][half][row] = top;
+                meet();
+                top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
+                const float from = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(m - from);
+                if (i > 0) {
+                    add_o(n - 1);  // (its product has been made under this tile's scores and maximum; then the weights' columns and O are free)
+                }
+                m = top;
+                less = shrink;
+                float sum0 = 0.0f, sum1 = 0.0f;
+#pragma unroll 1
+                for (int h = 0; h < KEYS / CH; h++) {
+                    float x[CH];
+                    load(h, x);
+                    uint32_t w[QP][CH / 2];
+#pragma unroll
+                    for (int j = 0; j < CH; j++) {
+                        x[j] = exp2_fast(fmaf(x[j], f, -from));
+                    }
+#pragma unroll
+                    for (int j = 0; j < CH / 2; j++) {
+                        sum0 += x[2 * j];
+                        sum1 += x[2 * j + 1];
+                        uint32_t part[QP];
+                        split_pair<BF, QP>(x[2 * j] * UP, x[2 * j + 1] * UP, part);
+#pragma unroll
+                        for (int p = 0; p < QP; p++) {
+                            w[p][j] = part[p];
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < QP; p++) {
+                        const uint32_t to = mine + L::P_AT + p * (TILE_KEYS / 2) + half * L::P_HALF + CH / 2 * h;
+                        if constexpr (CH == 32) {
+                            tile_st16(to, w[p]);
+                        } else {
+                            tile_st8(to, w[p]);
+                        }
+                    }
+                }
+                l = fmaf(l, shrink, sum0 + sum1);
+                tile_st_done();
+                if (edge) {
+                    // two threads look at a key's values
+                    constexpr int PIECES = HD / 16;
+                    const int st = n % VS, key = key0 - half * KEYS + row;
+                    ok = wait(v_full + 8 * st, (n / VS) & 1, 19) && ok;
+                    const uint32_t at = v_s + st * L::KV + row * 128;
+                    bool off = false;
+#pragma unroll 1
+                    for (int j = half * PIECES; j < (half + 1) * PIECES; j++) {
+                        off = off || not_finite<1>(load_shared16_at(at + (j >> 3) * (TILE_KEYS * 128) + (j & 7) * 16), BF);
+                    }
+                    const bool is = key < sq.keys && (reinterpret_cast<volatile int*>(gone_ring)[n & 3] >> (row / 16) & 1) == 0;
+                    const unsigned found = __ballot_sync(0xffffffffu, is && off);
+                    if (lane == 0) {
+                        bad_keys[half][warp & 3] = found;
+                    }
+                    meet();
+                    uint32_t bad[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        bad[j] = bad_keys[0][j] | bad_keys[1][j];
+                    }
+                    const uint32_t here = (row >> 5) == 0 ? bad[0] : ((row >> 5) == 1 ? bad[1] : ((row >> 5) == 2 ? bad[2] : bad[3]));
+                    if (!is || (here >> lane & 1) != 0) {
+#pragma unroll 1
+                        for (int j = half * PIECES; j < (half + 1) * PIECES; j++) {
+                            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(at + (j >> 3) * (TILE_KEYS * 128) + (j & 7) * 16), "r"(0) : "memory");
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    if ((bad[0] | bad[1] | bad[2] | bad[3]) != 0u) {
+                        tc::fence_before_sync();
+                        meet();  // (weights of the other half are read)
+                        tc::fence_after_sync();
+                        const int* const table = it.prefix ? a.b.prefix : a.b.tables + it.s * a.b.table_stride;
+#pragma unroll
+                        for (int j = 0; j < DIMS; j++) {
+                            acc[j] *= less;
+                        }
+                        less = 1.0f;
+#pragma unroll 1
+                        for (int k = 0; k < TILE_KEYS; k++) {
+                            if (((bad_keys[0][k >> 5] | bad_keys[1][k >> 5]) >> (k & 31) & 1) == 0) {
+                                continue;
+                            }
+                            float p = 0.0f;  // the parts of the weight, added up again
+#pragma unroll
+                            for (int j = 0; j < QP; j++) {
+                                const uint32_t pair = __float_as_uint(tile_ld1(mine + L::P_AT + j * (TILE_KEYS / 2) + (k >> 6) * L::P_HALF + ((k & 63) >> 1)));
+                                const uint32_t word = (k & 1) != 0 ? pair >> 16 : pair & 0xffffu;
+                                p += BF ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((unsigned short)word));
+                            }
+                            const int j = key0 - half * KEYS + k;
+                            if (j < limit) {
+                                const C* const v = static_cast<const C*>(a.v_pages) +
+                                                   (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD + half * DIMS;
+#pragma unroll
+                                for (int d = 0; d < DIMS; d++) {
+                                    acc[d] = fmaf(p, to_float(v[d]), acc[d]);
+                                }
+                            }
+                        }
+                    }
+                    meet();  // (the list of keys is free)
+                }
+                tc::fence_before_sync();
+                tc::mbar_arrive(p_full);
             }
-            // the values of the next tile: their buffer's last product has been waited for
-            copy_tile(v_pages, v_s + (buf ^ 1) * L::KV, c + 1);
-        }
-        if (pending && ok) {
-            ok = tc::mbar_wait(o_bar, o_phase, abort_flag, a.status, 11, a.wait_clocks);
-            o_phase ^= 1;
-            tc::fence_after_sync();
-            if (__all_sync(0xffffffffu, ok)) {
-                add_o();
+            add_o(n - 1);
+            tc::fence_before_sync();
+            // ---- what the thread block has of the item. Its warps' rows, some elements at a time, through the queries' memory (their products are done), so that they go out in lines
+            if (half == 1) {
+                sums[row] = l;
             }
-        }
-        tc::fence_before_sync();
-        copies_done<0>();
-        ok = __syncthreads_and(ok);
-        tc::fence_after_sync();
-        if (!ok) {
-            break;
-        }
-        // ---- what the thread block has of the item
-        if (r < rows) {
+            meet();
+            if (half == 0) {
+                l += sums[row];
+            }
             constexpr float DOWN = 1.0f / UP;
-            const bool complete = c0 == 0 && c1 == sq.chunks;
-            const int64_t token = sq.row0 + r / a.group;
-            const int head = kvh * a.group + r % a.group;
-            if (complete && !a.joined) {
-                T* const y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
-#pragma unroll
-                for (int i = 0; i < HD; i++) {
-                    y[i] = from_float<T>(over(acc[i] * DOWN, l));
+            if (half == 0 && real && !direct) {
+                (it.complete ? a.whole_ml : work.part_ml)[row_out[row]] = make_float2(m, l);
+            }
+            if (direct) {
+                if (half == 0) {
+                    tops[0][0][row] = l == 0.0f ? 0.0f : DOWN / l;
                 }
-            } else {
-                const int64_t at = complete ? ((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head : ((int64_t)blockIdx.x * 2 + (c0 == 0 ? 1 : 0)) * TILE_BLOCK + tid;
-                float* const to = (complete ? a.whole : work.part) + at * HD;
-                (complete ? a.whole_ml : work.part_ml)[at] = make_float2(m, l);
+                meet();
+            }
+            const float by = direct ? tops[0][0][row] : DOWN;
+            constexpr int WIDTH = QP * L::Q_PART >= 8 * 32 * 32 * 4 ? 32 : 16, PIECES = WIDTH / 4, AT_ONCE = 32 / PIECES;
+            const uint32_t rows_s = q_s + warp * (32 * WIDTH * 4);
 #pragma unroll
-                for (int i = 0; i < HD; i += 4) {
-                    *reinterpret_cast<float4*>(to + i) = make_float4(acc[i] * DOWN, acc[i + 1] * DOWN, acc[i + 2] * DOWN, acc[i + 3] * DOWN);
+            for (int run = 0; run < DIMS / WIDTH; run++) {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < PIECES; j++) {
+                    const int d = WIDTH * run + 4 * j;
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(rows_s + lane * (WIDTH * 4) + ((j ^ (lane & (PIECES - 1))) << 4)), "f"(acc[d] * by),
+                                 "f"(acc[d + 1] * by), "f"(acc[d + 2] * by), "f"(acc[d + 3] * by)
+                                 : "memory");
+                }
+                __syncwarp();
+#pragma unroll 1
+                for (int i = 0; i < 32 / AT_ONCE; i++) {
+                    const int k = AT_ONCE * i + lane / PIECES, piece = lane % PIECES, d = half * DIMS + WIDTH * run + 4 * piece;
+                    const uint4 w = load_shared16_at(rows_s + k * (WIDTH * 4) + ((piece ^ (k & (PIECES - 1))) << 4));
+                    const int64_t to = row_out[(warp & 3) * 32 + k];
+                    if (to < 0) {
+                        continue;
+                    }
+                    if (direct) {
+                        T* const y = static_cast<T*>(a.out) + to + d;
+                        y[0] = from_float<T>(__uint_as_float(w.x));
+                        y[1] = from_float<T>(__uint_as_float(w.y));
+                        y[2] = from_float<T>(__uint_as_float(w.z));
+                        y[3] = from_float<T>(__uint_as_float(w.w));
+                    } else {
+                        *reinterpret_cast<uint4*>((it.complete ? a.whole : work.part) + to * HD + d) = w;
+                    }
                 }
             }
+            meet();  // (the next item's queries and rows)
         }
-        begin = item0 + c1;
     }
-    copies_done<0>();
+    tc::fence_before_sync();
     __syncthreads();
     if (warp == 0) {
         tc::fence_after_sync();
