@@ -41,7 +41,6 @@ struct Tile {
     static constexpr int P_AT = ALIAS ? 0 : BUFS * TILE_KEYS, O_AT = ALIAS ? TILE_KEYS : P_AT + QP * (TILE_KEYS / 2);
     // where the weights of the second half of the keys begin: in the scores' place, over scores that the same thread has read
     static constexpr int P_HALF = ALIAS ? TILE_KEYS / 2 : TILE_KEYS / 4;
-    static constexpr int CHUNK = RESIDENT == 2 ? 16 : 32;          // scores that a thread holds at a time
     static constexpr int COLS = O_AT + HD <= 256 ? 256 : 512;
     static constexpr uint32_t TYPES = (1u << 4) | (BF ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(TILE_BLOCK >> 4) << 24);
     static constexpr uint32_t IDESC_S = TYPES | ((uint32_t)(TILE_KEYS >> 3) << 17);
@@ -273,94 +272,87 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 t.c = t.it.c0;
             }
         };
-        Cursor kc, vc;
-        start(kc);
-        vc = kc;
-        bring(kc, false);
-        bring(vc, true);
-        if (KS > 1) {
-            bring(kc, false);
-        }
-        if (VS > 1) {
-            bring(vc, true);
-        }
-        int n = 0, ni = 0;
-        auto scores = [&](int k) {  // S of tile k
-            if (lane == 0) {
-                const int st = k % KS;
-                ok = ok && wait(k_full + 8 * st, (k / KS) & 1, 12);
-                tc::fence_after_sync();
-                if (ok) {
-                    const uint32_t kd = tile_desc(k_s + st * L::KV), d = tmem + (k % L::BUFS) * TILE_KEYS;
-                    uint32_t more = 0;
-#pragma unroll
-                    for (int p = QP - 1; p >= 0; p--) {  // smallest parts first
-                        const uint32_t qd = tile_desc(q_s + p * L::Q_PART);
-#pragma unroll
-                        for (int j = 0; j < HD / 16; j++) {
-                            tile_mma(d, qd + (j >> 2) * (TILE_BLOCK * 128 >> 4) + (j & 3) * 2, kd + (j >> 2) * (TILE_KEYS * 128 >> 4) + (j & 3) * 2, L::IDESC_S, more);
-                            more = 1;
-                        }
-                    }
-                    tc::umma_commit(s_full + 8 * (k % L::BUFS));
-                    tc::umma_commit(k_free + 8 * st);
+        Cursor cursors[2];  // of keys, of values
+        start(cursors[0]);
+        cursors[1] = cursors[0];
+        // One place for each action: the instructions of a tile come from memory too when a call is small.
+        int scored = 0, summed = 0, ni = 0, left = 0;  // products issued; tiles of the item whose scores are to come
+        bool more = true;
+        while (ok) {
+            // ---- what there is room for: keys where the scores of KS tiles before have been issued (their end is waited for), values likewise
+#pragma unroll 1
+            for (int values = 0; values < 2; values++) {
+                Cursor& t = cursors[values];
+                while (ok && t.more && t.n < (values ? summed + VS : scored + KS)) {
+                    bring(t, values != 0);
                 }
             }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        };
-        while (ok && items.next(a, it)) {
-            const int tiles = it.c1 - it.c0;
-            if (lane == 0) {
-                ok = wait(q_full, ni & 1, 13);
-            }
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            scores(n);
-            for (int i = 0; i < tiles && ok; i++, n++) {
-                if (L::BUFS == 2 && i + 1 < tiles) {
-                    scores(n + 1);
+            if (left == 0 && scored == summed) {  // the next item
+                more = items.next(a, it);
+                if (!more) {
+                    break;
                 }
-                if (L::BUFS == 1) {
-                    bring(kc, false);  // (where the scores that are being made have their keys)
-                }
+                left = it.c1 - it.c0;
                 if (lane == 0) {
-                    const int st = n % VS;
-                    ok = ok && wait(p_full, n & 1, 14) && wait(v_full + 8 * st, (n / VS) & 1, 15);
+                    ok = ok && wait(q_full, ni & 1, 13);
+                }
+                ni++;
+            }
+            if (left > 0 && scored < summed + L::BUFS) {
+                // ---- S of the next tile
+                if (lane == 0) {
+                    const int st = scored % KS;
+                    if (L::ALIAS && scored > 0) {  // the weights' columns are free
+                        ok = ok && wait(o_full, (scored - 1) & 1, 16);
+                    }
+                    ok = ok && wait(k_full + 8 * st, (scored / KS) & 1, 12);
+                    tc::fence_after_sync();
+                    if (ok) {
+                        const uint32_t kd = tile_desc(k_s + st * L::KV), d = tmem + (scored % L::BUFS) * TILE_KEYS;
+#pragma unroll
+                        for (int p = QP - 1; p >= 0; p--) {  // smallest parts first
+                            const uint32_t qd = tile_desc(q_s + p * L::Q_PART);
+#pragma unroll
+                            for (int j = 0; j < HD / 16; j++) {
+                                tile_mma(d, qd + (j >> 2) * (TILE_BLOCK * 128 >> 4) + (j & 3) * 2, kd + (j >> 2) * (TILE_KEYS * 128 >> 4) + (j & 3) * 2, L::IDESC_S,
+                                         p < QP - 1 || j > 0 ? 1u : 0u);
+                            }
+                        }
+                        tc::umma_commit(s_full + 8 * (scored % L::BUFS));
+                        tc::umma_commit(k_free + 8 * st);
+                    }
+                }
+                scored++;
+                left--;
+            } else {
+                // ---- O of the next
+                if (lane == 0) {
+                    const int st = summed % VS;
+                    ok = ok && wait(p_full, summed & 1, 14) && wait(v_full + 8 * st, (summed / VS) & 1, 15);
                     tc::fence_after_sync();
                     if (ok) {
                         const uint32_t vd = tile_desc_values(v_s + st * L::KV);
-                        uint32_t more = 0;
 #pragma unroll
                         for (int p = QP - 1; p >= 0; p--) {
 #pragma unroll
                             for (int j = 0; j < TILE_KEYS / 16; j++) {
                                 tile_mma_weights(tmem + L::O_AT, tmem + L::P_AT + p * (TILE_KEYS / 2) + (j >> 2) * L::P_HALF + (j & 3) * 8, vd + j * (16 * 128 >> 4), L::IDESC_O,
-                                                 more);
-                                more = 1;
+                                                 p < QP - 1 || j > 0 ? 1u : 0u);
                             }
                         }
                         tc::umma_commit(o_full);
                         tc::umma_commit(v_free + 8 * st);
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                if (L::BUFS == 2) {
-                    bring(kc, false);
-                }
-                bring(vc, true);  // (waits for the product, with which the weights' columns are free as well)
-                if (L::BUFS == 1 && i + 1 < tiles) {
-                    if (L::ALIAS && lane == 0) {
-                        ok = ok && wait(o_full, n & 1, 16);
-                    }
-                    scores(n + 1);
-                }
+                summed++;
             }
-            ni++;
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         }
         // copies that nobody has waited for are waited for here (with a limit): they write to this thread block's memory
         if (!ok && lane == 0) {
             const long long t0 = clock64();
             for (int values = 0; values < 2; values++) {
-                const int stages = values ? VS : KS, upto = values ? vc.n : kc.n;
+                const int stages = values ? VS : KS, upto = cursors[values].n;
                 for (int i = upto > stages ? upto - stages : 0; i < upto; i++) {
                     while (!tc::mbar_try((values ? v_full : k_full) + 8 * (i % stages), (i / stages) & 1) && clock64() - t0 < a.wait_clocks) {
                     }
@@ -371,7 +363,8 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         // ---- rows
         const int half = warp >> 2, row = tid & (TILE_BLOCK - 1);
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // (a warp reaches 32 lanes, from lane 32 (warp % 4) on)
-        constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2, CH = L::CHUNK;  // of a thread
+        constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2;  // of a thread
+        constexpr int CH = 16;  // scores that it holds at a time. (Loops are rolled up: a small call's instructions come from memory, 50 clocks each)
         const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(TILE_ROW_THREADS) : "memory"); };  // all of these warps
         int n = 0;
@@ -393,7 +386,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             meet();
             // ---- queries: LANES lanes bring a row, eight elements each; a warp has 16 rows, some of which are on their way at a time
             {
-                constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 4;
+                constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 2;
                 const int d = lane % LANES * 8;
 #pragma unroll 1
                 for (int b = 0; b < 16; b += AT_ONCE * BATCH) {
@@ -467,13 +460,12 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             };
             constexpr float UP = QP == 2 ? 32768.0f : 1.0f;  // (half-precision parts of weights: times 2^15)
             const float f = factor > 0.0f ? factor : 1.0f;
-            for (int i = 0; i < tiles; i++, n++) {
+            for (int i = 0;; i++, n++) {
                 const int key0 = (it.c0 + i) * TILE_KEYS + half * KEYS;  // this thread's first
                 const uint32_t scores = mine + (n % L::BUFS) * TILE_KEYS + half * KEYS;
-                ok = wait(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
-                tc::fence_after_sync();
-                const int gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3] >> (half * (KEYS / 16));
-                const bool edge = key0 - half * KEYS + TILE_KEYS > least || reinterpret_cast<volatile int*>(gone_ring)[n & 3] != 0;
+                bool edge = false;
+                int gone = 0;
+                float top = -INFINITY;
                 auto load = [&](int h, float (&x)[CH]) {  // scores, minus infinity where the row does not see the key
                     tile_ld<CH>(x, scores + CH * h);
                     tile_ld_done();
@@ -491,24 +483,31 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         }
                     }
                 };
-                float top = -INFINITY, probe = 0.0f;
-                auto largest = [&] {
-#pragma unroll 1  // (a kernel's instructions come from memory too)
-                    for (int h = 0; h < KEYS / CH; h++) {
-                        float x[CH];
-                        load(h, x);
+                if (i < tiles) {
+                    ok = wait(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
+                    tc::fence_after_sync();
+                    gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3];
+                    edge = key0 - half * KEYS + TILE_KEYS > least || gone != 0;
+                    gone >>= half * (KEYS / 16);
+                    for (int turn = 0;; turn++) {
+                        float probe = 0.0f;
+                        top = -INFINITY;
+#pragma unroll 1
+                        for (int h = 0; h < KEYS / CH; h++) {
+                            float x[CH];
+                            load(h, x);
 #pragma unroll
-                        for (int j = 0; j < CH; j++) {
-                            top = fmaxf(top, x[j]);
-                            if constexpr (QP > 1) {
-                                probe = x[j] == -INFINITY ? probe : fmaf(x[j], 0.0f, probe);
+                            for (int j = 0; j < CH; j++) {
+                                top = fmaxf(top, x[j]);
+                                if constexpr (QP > 1) {
+                                    probe = x[j] == -INFINITY ? probe : fmaf(x[j], 0.0f, probe);
+                                }
                             }
                         }
-                    }
-                };
-                largest();
-                if constexpr (QP > 1) {  // in parts an infinity is infinity - infinity too: such scores are worked out again, one product after the other
-                    if (__any_sync(0xffffffffu, probe != probe)) {
+                        // in parts an infinity is infinity - infinity too: such scores are worked out again, one product after the other
+                        if (QP == 1 || turn == 1 || !__any_sync(0xffffffffu, probe != probe)) {
+                            break;
+                        }
                         const int* const table = it.prefix ? a.b.prefix : a.b.tables + it.s * a.b.table_stride;
 #pragma unroll 1
                         for (int key = 0; key < KEYS; key++) {
@@ -527,16 +526,17 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                             tile_st1(scores + key, v);
                         }
                         tile_st_done();
-                        top = -INFINITY;
-                        largest();
                     }
+                    tops[n & 1][half][row] = top;
+                    meet();
+                    top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 }
-                tops[n & 1][half][row] = top;
-                meet();
-                top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 const float from = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(m - from);
                 if (i > 0) {
                     add_o(n - 1);  // (its product has been made under this tile's scores and maximum; then the weights' columns and O are free)
+                }
+                if (i == tiles) {
+                    break;
                 }
                 m = top;
                 less = shrink;
@@ -641,7 +641,6 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 tc::fence_before_sync();
                 tc::mbar_arrive(p_full);
             }
-            add_o(n - 1);
             tc::fence_before_sync();
             // ---- what the thread block has of the item. Its warps' rows, some elements at a time, through the queries' memory (their products are done), so that they go out in lines
             if (half == 1) {
