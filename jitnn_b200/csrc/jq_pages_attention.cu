@@ -299,8 +299,8 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(space + at); };
     auto pairs = [&](int64_t at) { return reinterpret_cast<float2*>(space + at); };
     const int ahead = prefix_length > 0 ? 1 : 0;
-    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 7, plan.tile_workers, 1, floats(plan.tile_part), pairs(plan.tile_part_ml)};
-    const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, 1, floats(plan.part), pairs(plan.part_ml)};
+    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 7, plan.tile_workers, floats(plan.tile_part), pairs(plan.tile_part_ml)};
+    const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, floats(plan.part), pairs(plan.part_ml)};
     a.own = plan.tile_own ? tile : few;
     a.pre = plan.tile_workers > 0 ? tile : few;
     a.wait_clocks = (long long)g_opt_wait_limit_us.load(std::memory_order_relaxed) * 2000;  // about 2 GHz

@@ -15,7 +15,6 @@ struct Work {
     int rows_shift;    // rows of a block, keys of a unit: powers of two
     int keys_shift;
     int workers;       // at most
-    int least;         // units that make another worker worth while
     float* part;       // [slot][rows of a block][head_dim]
     float2* part_ml;   // maxima (of scores times log2 e) and sums
 };
@@ -81,9 +80,14 @@ __device__ __forceinline__ int keys_seen(const AttendArgs& a, const Sequence& q,
     return n < 0 ? 0 : (n < q.keys ? (int)n : q.keys);
 }
 
+// x / d of numbers that are not negative, which nearly always have 32 bits (a division of 64 is a hundred instructions and more).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
+    return ((x | d) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)d) : x / d;
+}
+
 struct Cut {
     int64_t total, per;
-    __device__ __forceinline__ int worker_of(int64_t unit) const { return (int)(unit / per); }
+    __device__ __forceinline__ int worker_of(int64_t unit) const { return (int)quotient(unit, per); }
 };
 
 // By a whole warp: the units of sequences first .. end - 1 of a work, all of them together, and the units of a worker.
@@ -104,9 +108,8 @@ __device__ __forceinline__ int64_t units_before(const AttendArgs& a, const Work&
 __device__ __forceinline__ Cut cut_of(const Work& w, int64_t total) {
     Cut c;
     c.total = total;
-    int64_t used = (total + w.least - 1) / w.least;
-    used = used < w.workers ? used : w.workers;
-    c.per = used > 0 ? (total + used - 1) / used : 1;
+    const int64_t used = total < w.workers ? total : w.workers;
+    c.per = used > 0 ? quotient(total + used - 1, used) : 1;
     return c;
 }
 // The sequence that a unit is in, and the first unit of that sequence; by a whole warp.

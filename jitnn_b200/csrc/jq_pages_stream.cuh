@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
             sq = sequence_at(a, ++s, ROWS_SHIFT, KEYS_SHIFT);
         }
         const bool prefix = s == a.b.sequences;
-        const int64_t item = (begin - base) / sq.chunks, item0 = base + item * sq.chunks;
-        const int kvh = (int)(item / sq.blocks), block = (int)(item % sq.blocks);
+        const int64_t item = quotient(begin - base, sq.chunks), item0 = base + item * sq.chunks;
+        const int kvh = (int)quotient(item, sq.blocks), block = (int)(item - (int64_t)kvh * sq.blocks);
         const int c0 = (int)(begin - item0), c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
         const int rows = sq.rows * a.group, row0 = block * ROWS;  // rows of the group: token * group + head
         const int* const table = prefix ? a.b.prefix : a.b.tables + s * a.b.table_stride;

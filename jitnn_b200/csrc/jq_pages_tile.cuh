@@ -148,11 +148,11 @@ struct Items {
             base += sq.units(a.kv_heads);
             sq = sequence_at(a, ++s, 7, 7);
         }
-        const int64_t item = (begin - base) / sq.chunks, item0 = base + item * sq.chunks;
+        const int64_t item = quotient(begin - base, sq.chunks), item0 = base + item * sq.chunks;
         it.s = s;
         it.prefix = s == a.b.sequences;
-        it.kvh = (int)(item / sq.blocks);
-        it.row0 = (int)(item % sq.blocks) * TILE_BLOCK;
+        it.kvh = (int)quotient(item, sq.blocks);
+        it.row0 = (int)(item - (int64_t)it.kvh * sq.blocks) * TILE_BLOCK;
         it.rows = sq.rows * a.group;
         it.c0 = (int)(begin - item0);
         it.c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     const uint32_t k_full = bar(0), k_free = bar(KS), v_full = bar(2 * KS), v_free = bar(2 * KS + VS);  // one for each stage
     const uint32_t s_full = bar(REST), p_full = bar(REST + 2), o_full = bar(REST + 3), q_full = bar(REST + 4);
     volatile int* const abort_flag = &abort_word;
-    if (tid == 0) {
+    if (warp == 8 && lane == 0) {
         for (int i = 0; i < REST + 5; i++) {
             tc::mbar_init(bar(i), i == REST + 2 || i == REST + 4 ? TILE_ROW_THREADS : 1);
         }
@@ -205,91 +205,119 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&tmem_slot)), "n"(L::COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    const uint32_t tmem = tmem_slot;
     Item it;
     // (a wait that gives up sets the abort flag, on which all others end too: every role goes on to its end without waiting or issuing anything)
     auto wait = [&](uint32_t b, uint32_t parity, int code) { return tc::mbar_wait(b, parity, abort_flag, a.status, code, a.wait_clocks); };
 
+    uint32_t tmem = 0;
+    auto begin_products = [&] {  // everybody: the barriers are made, and the columns allocated
+        tc::fence_before_sync();
+        __syncthreads();
+        tc::fence_after_sync();
+        tmem = tmem_slot;
+    };
     if (warp == 8) {
+        __syncwarp();
         // ---- copies and products. A lane has a box: 64 elements of the keys that a tile has of a page (of 128 of them), at most 16 boxes
         const int box = a.page_size < TILE_KEYS ? a.page_size : TILE_KEYS, boxes = TILE_KEYS / box * L::DB;
         const int my_run = lane % L::DB, my_key = lane / L::DB * box;
         bool ok = true;
-        struct Cursor {  // the next tile whose keys, or values, are to be brought, numbered through the items
+        // The next tile whose keys, or values, are to be brought, numbered through the items; the page of this lane's box is looked up a tile ahead (the values' are the keys')
+        struct Cursor {
             Items items;
             Item it;
-            int c, n;
+            int c;
             bool more;
-        };
-        auto start = [&](Cursor& t) {
-            t.items = items;
-            t.n = 0;
-            t.more = t.items.next(a, t.it);
-            t.c = t.it.c0;
-        };
-        auto bring = [&](Cursor& t, bool values) {
-            if (!ok || !t.more) {
-                return;
+        } next;
+        next.items = items;
+        next.more = next.items.next(a, next.it);
+        next.c = next.it.c0;
+        int page_next = -1;
+        auto look_up = [&] {
+            const int key = next.c * TILE_KEYS + my_key;
+            page_next = -2;
+            if (next.more && lane < boxes && key < next.items.sq.keys) {
+                page_next = (next.it.prefix ? a.b.prefix : a.b.tables + next.it.s * a.b.table_stride)[key >> a.page_shift];
+                page_next = page_next < -1 ? -1 : page_next;
             }
-            const int* const table = t.it.prefix ? a.b.prefix : a.b.tables + t.it.s * a.b.table_stride;
-            const int stages = values ? VS : KS, st = t.n % stages, key = t.c * TILE_KEYS + my_key;
-            const uint32_t full = (values ? v_full : k_full) + 8 * st;
-            int page = -1;
-            const bool mine = lane < boxes && key < t.items.sq.keys;
-            if (mine) {
-                page = table[key >> a.page_shift];
-                page = page >= 0 && page < a.pages ? page : -1;
+        };
+        look_up();
+        // what a tile's values need of its keys' copy: the box's row of pages, -1: none; and its first key in the page. Values are at most KS tiles behind
+        int v_row[2] = {-1, -1}, v_slot[2] = {0, 0};
+        uint32_t v_bytes[2] = {0, 0};
+        int keys_brought = 0, values_brought = 0;
+        auto bring_keys = [&] {
+            const int st = keys_brought % KS, slot = (next.c * TILE_KEYS + my_key) & (a.page_size - 1);
+            const bool real = page_next >= 0 && page_next < a.pages;
+            const unsigned there = __ballot_sync(0xffffffffu, real), missing = __ballot_sync(0xffffffffu, !real && page_next != -2);
+            const int row = real ? page_next * a.kv_heads + next.it.kvh : -1;
+            const uint32_t bytes = (uint32_t)__popc(there) * box * 128;
+            if (++next.c == next.it.c1) {
+                next.more = next.items.next(a, next.it);
+                next.c = next.it.c0;
             }
-            const unsigned there = __ballot_sync(0xffffffffu, page >= 0), missing = __ballot_sync(0xffffffffu, mine && page < 0);
+            look_up();
             if (lane == 0) {
-                ok = wait((values ? v_free : k_free) + 8 * st, ((t.n / stages) & 1) ^ 1, values ? 11 : 10);
-                if (!values) {
-                    int gone = 0;  // which keys are not there: a bit for each of the tile's sixteens
-                    for (int i = 0; i < TILE_KEYS / 16 && missing != 0u; i++) {
-                        gone |= (missing >> (i * 16 / box * L::DB) & 1) << i;
-                    }
-                    gone_ring[t.n & 3] = gone;
-                    if (gone != 0) {
-                        note_status(a.status, STATUS_PAGE);
-                    }
+                ok = ok && wait(k_free + 8 * st, ((keys_brought / KS) & 1) ^ 1, 10);
+                int gone = 0;  // which keys are not there: a bit for each of the tile's sixteens
+                for (int i = 0; i < TILE_KEYS / 16 && missing != 0u; i++) {
+                    gone |= (missing >> (i * 16 / box * L::DB) & 1) << i;
+                }
+                gone_ring[keys_brought & 3] = gone;
+                if (gone != 0) {
+                    note_status(a.status, STATUS_PAGE);
                 }
                 if (ok) {
-                    tc::mbar_expect_tx(full, (uint32_t)__popc(there) * box * 128);
+                    tc::mbar_expect_tx(k_full + 8 * st, bytes);
                 }
             }
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-            if (ok && page >= 0) {
-                copy_box((values ? v_s : k_s) + st * L::KV + my_run * (TILE_KEYS * 128) + my_key * 128, values ? &v_map : &k_map, full, my_run * 64,
-                         key & (a.page_size - 1), page * a.kv_heads + t.it.kvh);
+            if (ok && row >= 0) {
+                copy_box(k_s + st * L::KV + my_run * (TILE_KEYS * 128) + my_key * 128, &k_map, k_full + 8 * st, my_run * 64, slot, row);
             }
-            __syncwarp();
-            t.n++;
-            if (++t.c == t.it.c1) {
-                t.more = t.items.next(a, t.it);
-                t.c = t.it.c0;
+            if (keys_brought == values_brought) {
+                v_row[0] = row; v_slot[0] = slot; v_bytes[0] = bytes;
+            } else {
+                v_row[1] = row; v_slot[1] = slot; v_bytes[1] = bytes;
             }
+            keys_brought++;
         };
-        Cursor cursors[2];  // of keys, of values
-        start(cursors[0]);
-        cursors[1] = cursors[0];
-        // One place for each action: the instructions of a tile come from memory too when a call is small.
-        int scored = 0, summed = 0, ni = 0, left = 0;  // products issued; tiles of the item whose scores are to come
-        bool more = true;
-        while (ok) {
-            // ---- what there is room for: keys where the scores of KS tiles before have been issued (their end is waited for), values likewise
-#pragma unroll 1
-            for (int values = 0; values < 2; values++) {
-                Cursor& t = cursors[values];
-                while (ok && t.more && t.n < (values ? summed + VS : scored + KS)) {
-                    bring(t, values != 0);
+        auto bring_values = [&] {
+            const int st = values_brought % VS;
+            if (lane == 0) {
+                ok = ok && wait(v_free + 8 * st, ((values_brought / VS) & 1) ^ 1, 11);
+                if (ok) {
+                    tc::mbar_expect_tx(v_full + 8 * st, v_bytes[0]);
                 }
             }
+            ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+            if (ok && v_row[0] >= 0) {
+                copy_box(v_s + st * L::KV + my_run * (TILE_KEYS * 128) + my_key * 128, &v_map, v_full + 8 * st, my_run * 64, v_slot[0], v_row[0]);
+            }
+            v_row[0] = v_row[1]; v_slot[0] = v_slot[1]; v_bytes[0] = v_bytes[1];
+            values_brought++;
+        };
+        // One place for each action: the instructions of a tile come from memory too when a call is small.
+        int scored = 0, summed = 0, ni = 0, left = 0;  // products issued; tiles of the item whose scores are to come
+        bool refill = true;
+        while (ok) {
+            // ---- what there is room for: values where the product of VS tiles before has been issued (its end is waited for), keys where the scores have been
+            while (refill && ok) {
+                const bool values = values_brought < keys_brought && values_brought < summed + VS, keys = next.more && keys_brought < scored + KS && keys_brought < values_brought + 2;
+                if (values) {
+                    bring_values();
+                } else if (keys) {
+                    bring_keys();
+                } else {
+                    break;
+                }
+            }
+            refill = false;
+            if (scored == 0) {  // (the first copies are on their way)
+                begin_products();
+            }
             if (left == 0 && scored == summed) {  // the next item
-                more = items.next(a, it);
-                if (!more) {
+                if (!items.next(a, it)) {
                     break;
                 }
                 left = it.c1 - it.c0;
@@ -324,6 +352,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 }
                 scored++;
                 left--;
+                refill = true;
             } else {
                 // ---- O of the next
                 if (lane == 0) {
@@ -352,7 +381,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         if (!ok && lane == 0) {
             const long long t0 = clock64();
             for (int values = 0; values < 2; values++) {
-                const int stages = values ? VS : KS, upto = cursors[values].n;
+                const int stages = values ? VS : KS, upto = values ? values_brought : keys_brought;
                 for (int i = upto > stages ? upto - stages : 0; i < upto; i++) {
                     while (!tc::mbar_try((values ? v_full : k_full) + 8 * (i % stages), (i / stages) & 1) && clock64() - t0 < a.wait_clocks) {
                     }
@@ -361,6 +390,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         }
     } else {
         // ---- rows
+        begin_products();
         const int half = warp >> 2, row = tid & (TILE_BLOCK - 1);
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // (a warp reaches 32 lanes, from lane 32 (warp % 4) on)
         constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2;  // of a thread
@@ -372,7 +402,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         while (items.next(a, it)) {
             const Sequence& sq = items.sq;
             const int r = it.row0 + row, tiles = it.c1 - it.c0, i_token = r / a.group, i_head = r - i_token * a.group;
-            const bool real = r < it.rows, direct = it.complete && !a.joined;
+            const bool real = r < it.rows, direct = it.complete && !a.joined, some = __any_sync(0xffffffffu, real);  // (a warp without rows only keeps the others company)
             const int limit = real ? keys_seen(a, sq, it.s, i_token) : sq.keys, least = keys_seen(a, sq, it.s, it.row0 / a.group);
             if (half == 0) {
                 const int64_t token = sq.row0 + i_token;
@@ -489,7 +519,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3];
                     edge = key0 - half * KEYS + TILE_KEYS > least || gone != 0;
                     gone >>= half * (KEYS / 16);
-                    for (int turn = 0;; turn++) {
+                    for (int turn = 0; some; turn++) {
                         float probe = 0.0f;
                         top = -INFINITY;
 #pragma unroll 1
@@ -532,7 +562,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 }
                 const float from = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(m - from);
-                if (i > 0) {
+                if (i > 0 && some) {
                     add_o(n - 1);  // (its product has been made under this tile's scores and maximum; then the weights' columns and O are free)
                 }
                 if (i == tiles) {
@@ -542,7 +572,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 less = shrink;
                 float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll 1
-                for (int h = 0; h < KEYS / CH; h++) {
+                for (int h = 0; h < KEYS / CH && some; h++) {
                     float x[CH];
                     load(h, x);
                     uint32_t w[QP][CH / 2];
@@ -674,7 +704,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                                  : "memory");
                 }
                 __syncwarp();
-#pragma unroll 1
+#pragma unroll 4
                 for (int i = 0; i < 32 / AT_ONCE; i++) {
                     const int k = AT_ONCE * i + lane / PIECES, piece = lane % PIECES, d = half * DIMS + WIDTH * run + 4 * piece;
                     const uint4 w = load_shared16_at(rows_s + k * (WIDTH * 4) + ((piece ^ (k & (PIECES - 1))) << 4));
