@@ -118,7 +118,7 @@ struct Plan {
     int workers = 0;           // its warps
     int tile_workers = 0;      // the tile kernel's thread blocks; 0: it is not launched
     bool tile_own = false;     // whether it takes own keys too, not the prefix alone
-    int64_t part = 0, part_ml = 0, tile_part = 0, tile_part_ml = 0, whole = 0, whole_ml = 0, bytes = 0;
+    int64_t part = 0, part_ml = 0, tile_part = 0, tile_part_ml = 0, whole = 0, whole_ml = 0, found = 0, bytes = 0;
 };
 
 // How many thread blocks of the stream kernel an SM holds (by its registers).
@@ -161,6 +161,7 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
         plan.whole = take(2 * tokens * heads * hd * 4);
         plan.whole_ml = take(2 * tokens * heads * 8);
     }
+    plan.found = take(2 * tokens * heads * (int64_t)sizeof(int2));
     plan.bytes = at;
     return plan;
 }
@@ -307,6 +308,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     a.whole = reinterpret_cast<float*>(space + plan.whole);
     a.whole_ml = reinterpret_cast<float2*>(space + plan.whole_ml);
     a.joined = prefix_length > 0 ? 1 : 0;
+    a.found = reinterpret_cast<int2*>(space + plan.found);
     a.scale = scale;
     a.fill = fill != 0;
     const DeviceGuard guard(p->device);

@@ -34,6 +34,8 @@ struct AttendArgs {
     float* whole;      // of complete items, where own keys and a prefix are to be joined: over own keys and over the prefix, [2][token][head][head_dim]
     float2* whole_ml;
     int joined;        // whether they are
+    int2* found;       // for every row and head, of its own keys and of the prefix: the first worker that has some of them, and how many have (256 times that, and the row's
+                       // place in its block); the worker of the item's first unit says it. [2][token][head]
     long long wait_clocks;
 };
 
@@ -68,6 +70,7 @@ __device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int s, int 
     }
     q.blocks = (int)(((int64_t)q.rows * a.group + (1 << rows_shift) - 1) >> rows_shift);
     q.chunks = (int)(((int64_t)q.keys + (1 << keys_shift) - 1) >> keys_shift);
+    q.chunks = q.rows > 0 && q.chunks == 0 ? 1 : q.chunks;  // (rows without keys: an item that finds none)
     return q;
 }
 
@@ -87,6 +90,11 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
 
 struct Cut {
     int64_t total, per;
+    // What `found` says of a row of the item from unit item0 on.
+    __device__ __forceinline__ int2 found(int64_t item0, int chunks, int in_block) const {
+        const int first = worker_of(item0);
+        return make_int2(first, (worker_of(item0 + chunks - 1) - first + 1) << 8 | in_block);
+    }
     __device__ __forceinline__ int worker_of(int64_t unit) const { return (int)quotient(unit, per); }
 };
 

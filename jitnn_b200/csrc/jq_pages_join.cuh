@@ -1,5 +1,5 @@
-// Joins what the workers have of a row: a thread block has one head of one token. Which workers those are it works out anew from the lengths, while the kernels in front
-// still run. Its warps take the partial results in turn, eight each at once, a lane each the maximum and sum of 32.
+// Joins what the workers have of a row: a thread block has one head of one token. Its warps take the partial results in turn, eight each at once, a lane each the maximum and
+// sum of 32. Which workers those are the one with the row's first keys has written down. (Worked out here from all lengths, it was most of this kernel: 15 us for 1536 rows.)
 #pragma once
 
 #include "jq_pages_attention.cuh"
@@ -16,74 +16,54 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
     __shared__ float meet[JOIN_WARPS][HD];
     __shared__ float2 meet_ml[JOIN_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x, h = blockIdx.y;
-    // the token's sequence: the last that has it
-    int s = -1;
-    for (int s0 = 0; s0 < a.b.sequences; s0 += 32) {
-        const int i = s0 + lane;
-        const bool mine = i < a.b.sequences && token >= a.b.starts[i] && token < a.b.starts[i + 1];
-        const unsigned hit = __ballot_sync(0xffffffffu, mine);
-        s = hit != 0u ? s0 + 31 - __clz(hit) : s;
-    }
     T* const out = static_cast<T*>(a.out) + (int64_t)token * a.ot + h * a.oh;
-    if (s < 0) {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            if (a.fill && warp == 0) {
-                out[lane * V + j] = from_float<T>(0.0f);
-            }
+    const bool real = token >= a.b.starts[0] && token < a.b.starts[a.b.sequences];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!real) {
+        for (int d = threadIdx.x; d < HD && a.fill; d += JOIN_THREADS) {
+            out[d] = from_float<T>(0.0f);
         }
         return;
     }
-    // where the results over own keys and over the prefix are: `count` of them in slots of workers first, first + 1 ..; or one complete
-    int count[2], first[2], in_block[2];
     const bool one = a.joined == 0;
-    const int kvh = h / a.group;
-#pragma unroll
-    for (int part = 0; part < 2; part++) {
-        const Work& w = part == 0 ? a.own : a.pre;
-        count[part] = first[part] = in_block[part] = 0;
-        if (part == 1 && one) {
-            continue;
-        }
-        const int seq = part == 0 ? s : a.b.sequences;
-        const Sequence q = sequence_at(a, seq, w.rows_shift, w.keys_shift);
-        const int64_t base = units_before(a, w, seq, lane);
-        const Cut cut = cut_of(w, w.last - w.first == 1 ? q.units(a.kv_heads) : units_before(a, w, w.last, lane));
-        if (q.chunks > 0) {
-            const int row = (token - q.row0) * a.group + h % a.group;
-            const int64_t item0 = base + ((int64_t)kvh * q.blocks + (row >> w.rows_shift)) * q.chunks;
-            first[part] = cut.worker_of(item0);
-            count[part] = cut.worker_of(item0 + q.chunks - 1) - first[part] + 1;
-            in_block[part] = row & ((1 << w.rows_shift) - 1);
-        }
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (one && count[0] == 1) {
+    // (where the starts are in no order nobody may have said anything: whatever stands there stays in range)
+    auto in_range = [](int2 f, const Work& w, int& first, int& count, int& in_block) {
+        first = f.x < 0 || f.x >= w.workers ? 0 : f.x;
+        count = f.y >> 8;
+        count = count < 1 ? 1 : (count > w.workers - first ? w.workers - first : count);
+        in_block = f.y & ((1 << w.rows_shift) - 1);
+    };
+    const int64_t mine_at = (int64_t)token * a.heads + h;
+    int first0, count0, block0, first1 = 0, count1 = 0, block1 = 0;
+    in_range(a.found[mine_at], a.own, first0, count0, block0);
+    if (one && count0 == 1) {
         return;  // it is there already
+    }
+    if (!one) {
+        in_range(a.found[(int64_t)a.b.tokens * a.heads + mine_at], a.pre, first1, count1, block1);
     }
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
         acc[j] = 0.0f;
     }
-    const int all = count[0] + count[1], each = (all + JOIN_WARPS - 1) / JOIN_WARPS;
+    const int all = count0 + count1, each = (all + JOIN_WARPS - 1) / JOIN_WARPS;
     const int mine = each * warp < all ? each * warp : all, upto = mine + each < all ? mine + each : all;
     for (int n0 = mine; n0 < upto; n0 += 32) {
         const int n = n0 + lane;
         const float* from = nullptr;
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (n < upto) {
-            const int part = n < count[0] ? 0 : 1, i = part == 0 ? n : n - count[0];
-            const Work& w = part == 0 ? a.own : a.pre;
-            if (count[part] == 1) {
-                const int64_t at = ((part == 1 ? (int64_t)a.b.tokens : 0) + token) * a.heads + h;
+            const bool own = n < count0;
+            const int i = own ? n : n - count0;
+            if ((own ? count0 : count1) == 1) {
+                const int64_t at = (own ? 0 : (int64_t)a.b.tokens * a.heads) + mine_at;
                 from = a.whole + at * HD;
                 ml = a.whole_ml[at];
             } else {
-                const int64_t slot = (((int64_t)(first[part] + i) * 2 + (i == 0 ? 1 : 0)) << w.rows_shift) + in_block[part];
-                from = w.part + slot * HD;
-                ml = w.part_ml[slot];
+                const int64_t slot = (((int64_t)((own ? first0 : first1) + i) * 2 + (i == 0 ? 1 : 0)) << (own ? a.own.rows_shift : a.pre.rows_shift)) + (own ? block0 : block1);
+                from = (own ? a.own.part : a.pre.part) + slot * HD;
+                ml = (own ? a.own.part_ml : a.pre.part_ml)[slot];
             }
         }
         float top = ml.x;

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
             }
             const int64_t at_now = at;
-            if (at_now < 0) {
+            if (at_now < 0 && left > 0) {
                 note_status(a.status, STATUS_PAGE);
             }
             page = page_next;
@@ -459,6 +459,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
                 const int64_t token = sq.row0 + (row0 + r) / a.group;
                 const int head = kvh * a.group + (row0 + r) % a.group;
+                if (c0 == 0 && g == 0) {
+                    a.found[((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(item0, sq.chunks, r);
+                }
                 if (complete && !a.joined) {
                     T* const y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
 #pragma unroll

@@ -21,6 +21,8 @@
 #include "jq_pages_mma.cuh"
 #include "jq_tc.cuh"
 
+#include <cstring>
+
 namespace jq {
 namespace pages {
 
@@ -38,6 +40,8 @@ struct Tile {
     static constexpr int SMEM = 1024 + QP * Q_PART + (KS + VS) * KV;
     static constexpr int BUFS = QP == 2 ? 2 : 1;                   // of scores
     static constexpr bool ALIAS = QP == 1;                         // weights in the scores' columns
+    // where the sums over values are held: FP32 results need them added up with rounding, tile by tile; for 16-bit results the instruction does it
+    static constexpr bool IN_REGISTERS = QP > 1;
     static constexpr int P_AT = ALIAS ? 0 : BUFS * TILE_KEYS, O_AT = ALIAS ? TILE_KEYS : P_AT + QP * (TILE_KEYS / 2);
     // where the weights of the second half of the keys begin: in the scores' place, over scores that the same thread has read
     static constexpr int P_HALF = ALIAS ? TILE_KEYS / 2 : TILE_KEYS / 4;
@@ -134,6 +138,7 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, ui
 // What all of a thread block's roles go through alike: its items, each a run of tiles.
 struct Item {
     int s, kvh, row0, rows, c0, c1;
+    int64_t item0;
     bool prefix, complete;
 };
 struct Items {
@@ -150,6 +155,7 @@ struct Items {
         }
         const int64_t item = quotient(begin - base, sq.chunks), item0 = base + item * sq.chunks;
         it.s = s;
+        it.item0 = item0;
         it.prefix = s == a.b.sequences;
         it.kvh = (int)quotient(item, sq.blocks);
         it.row0 = (int)(item - (int64_t)it.kvh * sq.blocks) * TILE_BLOCK;
@@ -171,7 +177,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     extern __shared__ uint8_t raw_smem[];
     __shared__ __align__(8) uint64_t bars[2 * (KS + VS) + 5];
     __shared__ uint32_t tmem_slot;
-    __shared__ int abort_word, gone_ring[4];
+    __shared__ int abort_word, gone_ring[4], o_begun;  // o_begun: an item's sums have been begun by the rows
     __shared__ uint32_t bad_keys[2][4];
     __shared__ float tops[2][2][TILE_BLOCK], sums[TILE_BLOCK];  // of either half
     __shared__ int64_t row_q[TILE_BLOCK], row_out[TILE_BLOCK];  // where a row's queries are, and its results go; -1: there is no such row
@@ -199,6 +205,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             tc::mbar_init(bar(i), i == REST + 2 || i == REST + 4 ? TILE_ROW_THREADS : 1);
         }
         abort_word = 0;
+        o_begun = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             values_brought++;
         };
         // One place for each action: the instructions of a tile come from memory too when a call is small.
-        int scored = 0, summed = 0, ni = 0, left = 0;  // products issued; tiles of the item whose scores are to come
+        int scored = 0, summed = 0, ni = 0, left = 0, item_first = 0;  // products issued; items; tiles of the item whose scores are to come
         bool refill = true;
         while (ok) {
             // ---- what there is room for: values where the product of VS tiles before has been issued (its end is waited for), keys where the scores have been
@@ -321,6 +328,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     break;
                 }
                 left = it.c1 - it.c0;
+                item_first = summed;
                 if (lane == 0) {
                     ok = ok && wait(q_full, ni & 1, 13);
                 }
@@ -361,12 +369,17 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     tc::fence_after_sync();
                     if (ok) {
                         const uint32_t vd = tile_desc_values(v_s + st * L::KV);
+                        bool add = false;  // to what the item's tiles in front have left
+                        if constexpr (!L::IN_REGISTERS) {
+                            add = summed > item_first || reinterpret_cast<volatile int&>(o_begun) != 0;
+                            o_begun = 0;
+                        }
 #pragma unroll
                         for (int p = QP - 1; p >= 0; p--) {
 #pragma unroll
                             for (int j = 0; j < TILE_KEYS / 16; j++) {
                                 tile_mma_weights(tmem + L::O_AT, tmem + L::P_AT + p * (TILE_KEYS / 2) + (j >> 2) * L::P_HALF + (j & 3) * 8, vd + j * (16 * 128 >> 4), L::IDESC_O,
-                                                 p < QP - 1 || j > 0 ? 1u : 0u);
+                                                 p < QP - 1 || j > 0 || add ? 1u : 0u);
                             }
                         }
                         tc::umma_commit(o_full);
@@ -394,6 +407,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         const int half = warp >> 2, row = tid & (TILE_BLOCK - 1);
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // (a warp reaches 32 lanes, from lane 32 (warp % 4) on)
         constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2;  // of a thread
+        constexpr bool IN_REGISTERS = L::IN_REGISTERS;
         constexpr int CH = 16;  // scores that it holds at a time. (Loops are rolled up: a small call's instructions come from memory, 50 clocks each)
         const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(TILE_ROW_THREADS) : "memory"); };  // all of these warps
@@ -407,6 +421,9 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             if (half == 0) {
                 const int64_t token = sq.row0 + i_token;
                 const int head = it.kvh * a.group + i_head;
+                if (real && it.c0 == 0) {
+                    a.found[((it.prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(it.item0, sq.chunks, row);
+                }
                 row_q[row] = real ? token * a.qt + head * a.qh : -1;
                 row_out[row] = !real      ? -1
                                : direct   ? token * a.ot + head * a.oh
@@ -414,44 +431,65 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                                              : ((int64_t)blockIdx.x * 2 + (it.c0 == 0 ? 1 : 0)) * TILE_BLOCK + row;
             }
             meet();
-            // ---- queries: LANES lanes bring a row, eight elements each; a warp has 16 rows, some of which are on their way at a time
+            // ---- queries: LANES lanes bring a row, eight elements each; a warp has 16 rows, as many of which as registers take are on their way at a time
             {
-                constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 2;
-                const int d = lane % LANES * 8;
+                constexpr int LANES = HD / 8, AT_ONCE = 32 / LANES, BATCH = 16 / AT_ONCE < 4 || QP == 1 ? 16 / AT_ONCE : 4, WORDS = sizeof(T) / 2;
+                const int d = lane % LANES * 8, k0 = 16 * warp + lane / LANES;
 #pragma unroll 1
                 for (int b = 0; b < 16; b += AT_ONCE * BATCH) {
-                    float v[BATCH][8];
+                    uint4 raw[BATCH][WORDS];
 #pragma unroll
                     for (int i = 0; i < BATCH; i++) {
-                        const int64_t from = row_q[16 * warp + b + i * AT_ONCE + lane / LANES];
-                        load_queries<T>(static_cast<const T*>(a.q) + (from < 0 ? 0 : from) + d, from >= 0, wide, v[i]);
+                        const int64_t from = row_q[k0 + b + i * AT_ONCE];
+                        const T* const x = static_cast<const T*>(a.q) + (from < 0 ? 0 : from) + d;
+#pragma unroll
+                        for (int w = 0; w < WORDS; w++) {
+                            raw[i][w] = make_uint4(0, 0, 0, 0);
+                            if (from >= 0 && wide) {
+                                raw[i][w] = *reinterpret_cast<const uint4*>(x + 4 * w);
+                            } else if (from >= 0) {  // at any address
+                                T e[16 / sizeof(T)];
+#pragma unroll 1
+                                for (int j = 0; j < (int)(16 / sizeof(T)); j++) {
+                                    e[j] = x[w * (16 / sizeof(T)) + j];
+                                }
+                                memcpy(&raw[i][w], e, 16);
+                            }
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < BATCH; i++) {
-                        const int k = 16 * warp + b + i * AT_ONCE + lane / LANES;
-                        if constexpr (QP == 2) {  // a power of two takes the row's largest magnitude to [2^9, 2^10)
-                            float top = 0.0f;
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                top = fmaxf(top, fabsf(v[i][j]));
-                            }
-#pragma unroll
-                            for (int o = LANES / 2; o > 0; o >>= 1) {
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                            }
-                            uint32_t e = __float_as_uint(top) >> 23;
-                            e = e < 20u ? 20u : (e > 250u ? 250u : e);
-                            const float by = __uint_as_float((263u - e) << 23);
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                v[i][j] *= by;
-                            }
-                            sums[k] = by;
-                        }
+                        const int k = k0 + b + i * AT_ONCE;
                         uint32_t w[4][QP];
+                        if constexpr (QP == 1) {
+                            w[0][0] = raw[i][0].x; w[1][0] = raw[i][0].y; w[2][0] = raw[i][0].z; w[3][0] = raw[i][0].w;
+                        } else {
+                            float v[8] = {__uint_as_float(raw[i][0].x), __uint_as_float(raw[i][0].y), __uint_as_float(raw[i][0].z), __uint_as_float(raw[i][0].w),
+                                          __uint_as_float(raw[i][WORDS - 1].x), __uint_as_float(raw[i][WORDS - 1].y), __uint_as_float(raw[i][WORDS - 1].z),
+                                          __uint_as_float(raw[i][WORDS - 1].w)};
+                            if constexpr (QP == 2) {  // a power of two takes the row's largest magnitude to [2^9, 2^10)
+                                float top = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            split_pair<BF, QP>(v[i][2 * j], v[i][2 * j + 1], w[j]);
+                                for (int j = 0; j < 8; j++) {
+                                    top = fmaxf(top, fabsf(v[j]));
+                                }
+#pragma unroll
+                                for (int o = LANES / 2; o > 0; o >>= 1) {
+                                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                                }
+                                uint32_t e = __float_as_uint(top) >> 23;
+                                e = e < 20u ? 20u : (e > 250u ? 250u : e);
+                                const float by = __uint_as_float((263u - e) << 23);
+#pragma unroll
+                                for (int j = 0; j < 8; j++) {
+                                    v[j] *= by;
+                                }
+                                sums[k] = by;
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                split_pair<BF, QP>(v[2 * j], v[2 * j + 1], w[j]);
+                            }
                         }
 #pragma unroll
                         for (int p = 0; p < QP; p++) {
@@ -469,12 +507,16 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 up = sums[row];
                 factor /= up;  // (exact)
             }
-            float acc[DIMS], m = -INFINITY, l = 0.0f, less = 0.0f;
+            float m = -INFINITY, l = 0.0f, less = 0.0f;
+            float acc[IN_REGISTERS ? DIMS : 1];
+            if constexpr (IN_REGISTERS) {
 #pragma unroll
-            for (int i = 0; i < DIMS; i++) {
-                acc[i] = 0.0f;
+                for (int i = 0; i < DIMS; i++) {
+                    acc[i] = 0.0f;
+                }
             }
             auto add_o = [&](int tile) {  // O of a tile to the sums
+                if constexpr (IN_REGISTERS) {
                 ok = wait(o_full, tile & 1, 17) && ok;
                 tc::fence_after_sync();
 #pragma unroll
@@ -486,6 +528,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     for (int i = 0; i < CH; i++) {
                         acc[CH * h + i] = fmaf(acc[CH * h + i], less, o[i]);
                     }
+                }
                 }
             };
             constexpr float UP = QP == 2 ? 32768.0f : 1.0f;  // (half-precision parts of weights: times 2^15)
@@ -561,15 +604,44 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     meet();
                     top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 }
-                const float from = top == -INFINITY ? 0.0f : top, shrink = exp2_fast(m - from);
-                if (i > 0 && some) {
-                    add_o(n - 1);  // (its product has been made under this tile's scores and maximum; then the weights' columns and O are free)
+                if constexpr (!IN_REGISTERS) {
+                    if (i == tiles) {
+                        ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                        tc::fence_after_sync();
+                        break;
+                    }
+                    // The sums stay as they are, and weights may be up to 2^8, until a maximum is more than that above the one they go by (or is the first)
+                    const bool far = top > m + 8.0f;
+                    const float shrink = far ? exp2_fast(m - top) : 1.0f;
+                    if (i > 0 && __any_sync(0xffffffffu, far)) {
+                        ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                        tc::fence_after_sync();
+#pragma unroll 1
+                        for (int h = 0; h < DIMS / CH; h++) {
+                            float o[CH];
+                            tile_ld<CH>(o, mine + L::O_AT + half * DIMS + CH * h);
+                            tile_ld_done();
+                            uint32_t w[CH];
+#pragma unroll
+                            for (int j = 0; j < CH; j++) {
+                                w[j] = __float_as_uint(o[j] * shrink);
+                            }
+                            tile_st16(mine + L::O_AT + half * DIMS + CH * h, w);
+                        }
+                    }
+                    m = far ? top : m;
+                    less = shrink;
+                } else {
+                    if (i > 0 && some) {
+                        add_o(n - 1);  // (its product has been made under this tile's scores and maximum; then the weights' columns and O are free)
+                    }
+                    if (i == tiles) {
+                        break;
+                    }
+                    less = exp2_fast(m - (top == -INFINITY ? 0.0f : top));
+                    m = top;
                 }
-                if (i == tiles) {
-                    break;
-                }
-                m = top;
-                less = shrink;
+                const float from = m == -INFINITY ? 0.0f : m;
                 float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll 1
                 for (int h = 0; h < KEYS / CH && some; h++) {
@@ -601,7 +673,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         }
                     }
                 }
-                l = fmaf(l, shrink, sum0 + sum1);
+                l = fmaf(l, less, sum0 + sum1);
                 tile_st_done();
                 if (edge) {
                     // two threads look at a key's values
@@ -638,11 +710,26 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         meet();  // (weights of the other half are read)
                         tc::fence_after_sync();
                         const int* const table = it.prefix ? a.b.prefix : a.b.tables + it.s * a.b.table_stride;
+                        if constexpr (IN_REGISTERS) {
 #pragma unroll
-                        for (int j = 0; j < DIMS; j++) {
-                            acc[j] *= less;
+                            for (int j = 0; j < DIMS; j++) {
+                                acc[j] *= less;
+                            }
+                            less = 1.0f;
+                        } else {
+                            if (i > 0) {
+                                ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                                tc::fence_after_sync();
+                            } else {  // the sums begin here
+                                const uint32_t none[16] = {};
+#pragma unroll 1
+                                for (int h = 0; h < DIMS / 16; h++) {
+                                    tile_st16(mine + L::O_AT + half * DIMS + 16 * h, none);
+                                }
+                                tile_st_done();
+                                o_begun = 1;
+                            }
                         }
-                        less = 1.0f;
 #pragma unroll 1
                         for (int k = 0; k < TILE_KEYS; k++) {
                             if (((bad_keys[0][k >> 5] | bad_keys[1][k >> 5]) >> (k & 31) & 1) == 0) {
@@ -656,13 +743,22 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                                 p += BF ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((unsigned short)word));
                             }
                             const int j = key0 - half * KEYS + k;
-                            if (j < limit) {
-                                const C* const v = static_cast<const C*>(a.v_pages) +
-                                                   (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD + half * DIMS;
+                            const C* const v = static_cast<const C*>(a.v_pages) +
+                                               (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD + half * DIMS;
+                            if constexpr (IN_REGISTERS) {
+                                if (j < limit) {
 #pragma unroll
-                                for (int d = 0; d < DIMS; d++) {
-                                    acc[d] = fmaf(p, to_float(v[d]), acc[d]);
+                                    for (int d = 0; d < DIMS; d++) {
+                                        acc[d] = fmaf(p, to_float(v[d]), acc[d]);
+                                    }
                                 }
+                            } else {
+#pragma unroll 1
+                                for (int d = 0; d < DIMS; d++) {
+                                    const float o = tile_ld1(mine + L::O_AT + half * DIMS + d);
+                                    tile_st1(mine + L::O_AT + half * DIMS + d, j < limit ? fmaf(p, to_float(v[d]), o) : o);
+                                }
+                                tile_st_done();
                             }
                         }
                     }
@@ -693,14 +789,20 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             const float by = direct ? tops[0][0][row] : DOWN;
             constexpr int WIDTH = QP * L::Q_PART >= 8 * 32 * 32 * 4 ? 32 : 16, PIECES = WIDTH / 4, AT_ONCE = 32 / PIECES;
             const uint32_t rows_s = q_s + warp * (32 * WIDTH * 4);
+            float out_o[IN_REGISTERS ? 1 : WIDTH];
 #pragma unroll
             for (int run = 0; run < DIMS / WIDTH; run++) {
                 __syncwarp();
+                if constexpr (!IN_REGISTERS) {
+                    tile_ld<WIDTH>(out_o, mine + L::O_AT + half * DIMS + WIDTH * run);
+                    tile_ld_done();
+                }
+                const float* const o = IN_REGISTERS ? acc : out_o;
 #pragma unroll
                 for (int j = 0; j < PIECES; j++) {
-                    const int d = WIDTH * run + 4 * j;
-                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(rows_s + lane * (WIDTH * 4) + ((j ^ (lane & (PIECES - 1))) << 4)), "f"(acc[d] * by),
-                                 "f"(acc[d + 1] * by), "f"(acc[d + 2] * by), "f"(acc[d + 3] * by)
+                    const int d = IN_REGISTERS ? WIDTH * run + 4 * j : 4 * j;
+                    asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(rows_s + lane * (WIDTH * 4) + ((j ^ (lane & (PIECES - 1))) << 4)), "f"(o[d] * by),
+                                 "f"(o[d + 1] * by), "f"(o[d + 2] * by), "f"(o[d + 3] * by)
                                  : "memory");
                 }
                 __syncwarp();
