@@ -134,6 +134,9 @@ def load_front(weight_class):
     L = ctypes.CDLL(LIB_PATH)  # (the one that load() has)
     names = ("jq_linear_f32", "jq_linear_bf16", "jq_linear_backward_f32", "jq_dequantize", "jq_quantize_q8_0")
     front.bind(weight_class, check, *(ctypes.cast(getattr(L, name), vp).value for name in names))
+    from .paged import PagedBatch, PagedCache, Rope
+    names = ("jq_rope_apply", "jq_pages_append", "jq_pages_attention_bytes", "jq_pages_attention", "jq_verify_bytes", "jq_verify_drafts")
+    front.bind_paged(Rope, PagedCache, PagedBatch, *(ctypes.cast(getattr(L, name), vp).value for name in names))
     return front
 
 

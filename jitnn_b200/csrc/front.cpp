@@ -243,6 +243,338 @@ PyObject* quantize(PyObject*, PyObject* const* args, Py_ssize_t count) {
     });
 }
 
+// ---- the operators of paged decoding: the same for their plain calls, with outputs of their own (a rotation of queries and keys from Python 21 us a call, from here 5) ----
+using RopeApply = int (*)(const void* r, int elem, int count, const void* const* x, void* const* y, const int* heads, int head_dim, const int64_t* strides, int64_t batch,
+                          int64_t seq, const void* positions, int position_bytes, int64_t position_batch_stride, int64_t position_stride, int64_t offset, int inverse, void* stream);
+using Append = int (*)(const void* p, const void* rope, int elem, int heads, const void* q, const void* k, const void* v, void* q_out, const int64_t* strides, int64_t tokens,
+                       const int32_t* tables, int64_t table_stride, int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, int64_t prefix_length,
+                       int fill, void* stream);
+using AttentionBytes = int (*)(const void* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length, int64_t* nbytes);
+using Attention = int (*)(const void* p, int elem, int heads, const void* q, void* out, const int64_t* strides, int64_t tokens, const int32_t* tables, int64_t table_stride,
+                          int64_t table_width, const int32_t* starts, const int32_t* lengths, int sequences, const int32_t* prefix, int64_t prefix_width, int64_t prefix_length,
+                          float scale, int fill, void* workspace, int64_t workspace_bytes, void* stream);
+using VerifyBytes = int (*)(int64_t sequences, int64_t drafts, int64_t vocab, int logits, int64_t* nbytes);
+using Verify = int (*)(int device, int elem, const void* target, int64_t target_stride, int64_t target_row_stride, const int32_t* drafts, const float* draft_probs,
+                       int64_t draft_stride, int64_t draft_row_stride, const float* uniforms, const int32_t* counts, int64_t sequences, int64_t drafts_most, int64_t vocab,
+                       int logits, double temperature, int32_t* accepted, int32_t* tokens, void* workspace, int64_t workspace_bytes, void* stream);
+RopeApply g_rope_apply = nullptr;
+Append g_append = nullptr;
+AttentionBytes g_attention_bytes = nullptr;
+Attention g_attention = nullptr;
+VerifyBytes g_verify_bytes = nullptr;
+Verify g_verify = nullptr;
+PyObject *g_rope = nullptr, *g_pages = nullptr, *g_batch = nullptr;  // the classes
+PyObject *s_plain_device = nullptr, *s_kv_heads = nullptr, *s_head_dim = nullptr, *s_code = nullptr, *s_rows = nullptr, *s_ahead = nullptr;
+
+// The tensor behind a plain CUDA tensor on `device` (-1: any) whose last axis is in one piece, or null.
+const at::Tensor* plain_strided(PyObject* obj, int64_t dims, int64_t device) {
+    using c10::DispatchKey;
+    if (!THPVariable_CheckExact(obj)) {
+        return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(obj);
+    constexpr c10::DispatchKeySet special({DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper, DispatchKey::Functionalize, DispatchKey::Batched,
+                                           DispatchKey::Conjugate, DispatchKey::Negative, DispatchKey::ZeroTensor});
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.dim() != dims || t.key_set().has_any(special) || (device >= 0 && t.get_device() != device) ||
+        t.numel() == 0 || t.stride(-1) != 1) {
+        return nullptr;
+    }
+    return &t;
+}
+
+// The library's element type, -1 for others.
+int elem_of(const at::Tensor& t) {
+    const at::ScalarType s = t.scalar_type();
+    return s == at::kFloat ? 0 : (s == at::kHalf ? 1 : (s == at::kBFloat16 ? 2 : -1));
+}
+
+at::Tensor like(const at::Tensor& x) { return at::cuda::empty(x.sizes(), x.options()); }
+
+// An int32 tensor of that shape in one piece, or null.
+const at::Tensor* whole(PyObject* obj, at::IntArrayRef shape, int64_t device) {
+    const at::Tensor* const t = plain(obj, at::kInt);
+    return t != nullptr && t->get_device() == device && t->sizes() == shape ? t : nullptr;
+}
+
+PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t count) {  // rope, tensor or pair, positions, inverse
+    return guarded([&]() -> PyObject* {
+        int64_t addr = 0, device = 0;
+        if (count != 4 || (PyObject*)Py_TYPE(args[0]) != g_rope || !attribute(args[0], s_addr, addr) || addr == 0 || !attribute(args[0], s_plain_device, device) || !undisturbed()) {
+            return not_plain();
+        }
+        const bool pair = PyTuple_Check(args[1]);
+        const Py_ssize_t n = pair ? PyTuple_GET_SIZE(args[1]) : 1;
+        if (n < 1 || n > 2) {
+            return not_plain();
+        }
+        const at::Tensor* x[2] = {nullptr, nullptr};
+        int heads[2] = {0, 0};
+        int64_t dims = 0;
+        for (Py_ssize_t i = 0; i < n; i++) {
+            PyObject* const obj = pair ? PyTuple_GET_ITEM(args[1], i) : args[1];
+            x[i] = plain_strided(obj, 3, device);
+            if (x[i] == nullptr) {
+                x[i] = plain_strided(obj, 4, device);
+            }
+            if (x[i] == nullptr || elem_of(*x[i]) < 0 || x[i]->scalar_type() != x[0]->scalar_type() || x[i]->dim() != x[0]->dim()) {
+                return not_plain();
+            }
+            dims = x[i]->dim();
+            for (int64_t d = 0; d < dims; d++) {
+                if (d != dims - 2 && x[i]->size(d) != x[0]->size(d)) {
+                    return not_plain();
+                }
+            }
+            heads[i] = (int)x[i]->size(dims - 2);
+        }
+        const int64_t batch = dims == 4 ? x[0]->size(0) : 1, seq = x[0]->size(dims - 3);
+        const void* at = nullptr;
+        int bytes = 0;
+        int64_t pb = 0, pt = 0, offset = 0;
+        if (PyLong_CheckExact(args[2])) {
+            offset = PyLong_AsLongLong(args[2]);
+            if (PyErr_Occurred() != nullptr) {
+                PyErr_Clear();
+                return not_plain();
+            }
+        } else {
+            const at::Tensor* p = plain(args[2], at::kInt);
+            bytes = 4;
+            if (p == nullptr) {
+                p = plain(args[2], at::kLong);
+                bytes = 8;
+            }
+            if (p == nullptr || p->get_device() != device || p->size(-1) != seq || !(p->dim() == 1 || (dims == 4 && p->dim() == 2 && p->size(0) == batch))) {
+                return not_plain();
+            }
+            at = p->const_data_ptr();
+            pt = 1;
+            pb = p->dim() == 2 ? seq : 0;
+        }
+        const int inverse = PyObject_IsTrue(args[3]);
+        at::Tensor y[2];
+        const void* xp[2];
+        void* yp[2];
+        int64_t strides[12];
+        for (Py_ssize_t i = 0; i < n; i++) {
+            y[i] = like(*x[i]);
+            xp[i] = x[i]->const_data_ptr();
+            yp[i] = y[i].mutable_data_ptr();
+            const at::Tensor* const of[2] = {x[i], &y[i]};
+            for (int j = 0; j < 2; j++) {
+                int64_t* const s = strides + 6 * i + 3 * j;
+                s[0] = dims == 4 ? of[j]->stride(0) : 0;
+                s[1] = of[j]->stride(dims - 3);
+                s[2] = of[j]->stride(dims - 2);
+            }
+        }
+        const int elem = elem_of(*x[0]), hd = (int)x[0]->size(-1);
+        void* const stream = stream_of((int)device);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = g_rope_apply((const void*)addr, elem, (int)n, xp, yp, heads, hd, strides, batch, seq, at, bytes, pb, pt, offset, inverse, stream);
+        Py_END_ALLOW_THREADS;
+        if (rc != 0) {
+            return finish(rc, nullptr);
+        }
+        PyObject* first = THPVariable_Wrap(std::move(y[0]));
+        if (!pair) {
+            return first;
+        }
+        return n == 2 ? Py_BuildValue("(NN)", first, THPVariable_Wrap(std::move(y[1]))) : Py_BuildValue("(N)", first);
+    });
+}
+
+struct Pages {
+    const void* handle;
+    int64_t device, kv_heads, head_dim, code;
+};
+bool pages_of(PyObject* obj, Pages& p) {
+    int64_t addr = 0;
+    if ((PyObject*)Py_TYPE(obj) != g_pages || !attribute(obj, s_addr, addr) || addr == 0 || !attribute(obj, s_plain_device, p.device) || !attribute(obj, s_kv_heads, p.kv_heads) ||
+        !attribute(obj, s_head_dim, p.head_dim) || !attribute(obj, s_code, p.code)) {
+        return false;
+    }
+    p.handle = (const void*)addr;
+    return true;
+}
+// The numbers that a PagedBatch keeps: tables, their stride and width, starts, lengths, sequences; prefix, its pages, its keys.
+bool batch_of(PyObject* obj, int64_t device, int64_t (&v)[9]) {
+    int64_t on = 0;
+    if ((PyObject*)Py_TYPE(obj) != g_batch || !attribute(obj, s_plain_device, on) || on != device) {
+        return false;
+    }
+    PyObject* const lists[2] = {PyObject_GetAttr(obj, s_rows), PyObject_GetAttr(obj, s_ahead)};
+    bool ok = true;
+    int at = 0;
+    for (int i = 0; i < 2; i++) {
+        const int want = i == 0 ? 6 : 3;
+        ok = ok && lists[i] != nullptr && PyTuple_Check(lists[i]) && PyTuple_GET_SIZE(lists[i]) == want;
+        for (int j = 0; j < want && ok; j++) {
+            PyObject* const n = PyTuple_GET_ITEM(lists[i], j);
+            v[at++] = n == Py_None ? 0 : PyLong_AsLongLong(n);
+        }
+        Py_XDECREF(lists[i]);
+    }
+    if (PyErr_Occurred() != nullptr) {
+        PyErr_Clear();
+        return false;
+    }
+    return ok;
+}
+
+PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t count) {  // pages, q, k, v, batch, rope or None
+    return guarded([&]() -> PyObject* {
+        Pages p;
+        int64_t b[9], rope_addr = 0, rope_device = 0;
+        if (count != 6 || !pages_of(args[0], p) || !batch_of(args[4], p.device, b) || !undisturbed()) {
+            return not_plain();
+        }
+        if (args[5] != Py_None && ((PyObject*)Py_TYPE(args[5]) != g_rope || !attribute(args[5], s_addr, rope_addr) || rope_addr == 0 ||
+                                   !attribute(args[5], s_plain_device, rope_device) || rope_device != p.device)) {
+            return not_plain();
+        }
+        const at::Tensor *const q = plain_strided(args[1], 3, p.device), *const k = plain_strided(args[2], 3, p.device), *const v = plain_strided(args[3], 3, p.device);
+        if (q == nullptr || k == nullptr || v == nullptr) {
+            return not_plain();
+        }
+        const int elem = elem_of(*k);
+        if (elem < 0 || (elem != 0 && elem != p.code) || elem_of(*q) != elem || elem_of(*v) != elem || k->size(1) != p.kv_heads || k->size(2) != p.head_dim ||
+            v->sizes() != k->sizes() || q->size(0) != k->size(0) || q->size(2) != p.head_dim) {
+            return not_plain();
+        }
+        at::Tensor y = like(*q);
+        const int64_t strides[8] = {q->stride(0), q->stride(1), k->stride(0), k->stride(1), v->stride(0), v->stride(1), y.stride(0), y.stride(1)};
+        const void *const qp = q->const_data_ptr(), *const kp = k->const_data_ptr(), *const vp = v->const_data_ptr();
+        void *const yp = y.mutable_data_ptr(), *const stream = stream_of((int)p.device);
+        const int heads = (int)q->size(1);
+        const int64_t tokens = q->size(0);
+        int rc;
+        Py_BEGIN_ALLOW_THREADS;
+        rc = g_append(p.handle, (const void*)rope_addr, elem, heads, qp, kp, vp, yp, strides, tokens, (const int32_t*)b[0], b[1], b[2], (const int32_t*)b[3], (const int32_t*)b[4],
+                      (int)b[5], b[8], 1, stream);
+        Py_END_ALLOW_THREADS;
+        return finish(rc, rc == 0 ? THPVariable_Wrap(std::move(y)) : nullptr);
+    });
+}
+
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t count) {  // pages, q, batch, scale
+    return guarded([&]() -> PyObject* {
+        Pages p;
+        int64_t b[9];
+        if (count != 4 || !pages_of(args[0], p) || !PyFloat_CheckExact(args[3]) || !batch_of(args[2], p.device, b) || !undisturbed()) {
+            return not_plain();
+        }
+        const at::Tensor* const q = plain_strided(args[1], 3, p.device);
+        if (q == nullptr) {
+            return not_plain();
+        }
+        const int elem = elem_of(*q), heads = (int)q->size(1);
+        const int64_t tokens = q->size(0);
+        if (elem < 0 || (elem != 0 && elem != p.code) || q->size(2) != p.head_dim || heads % p.kv_heads != 0) {
+            return not_plain();
+        }
+        int64_t need = 0;
+        int rc = g_attention_bytes(p.handle, elem, heads, tokens, b[5], b[8], &need);
+        if (rc != 0) {
+            return finish(rc, nullptr);
+        }
+        at::Tensor y = like(*q), space;
+        if (need > 0) {
+            space = at::cuda::empty({need}, q->options().dtype(at::kByte));
+        }
+        const int64_t strides[4] = {q->stride(0), q->stride(1), y.stride(0), y.stride(1)};
+        const void* const qp = q->const_data_ptr();
+        void *const yp = y.mutable_data_ptr(), *const sp = need > 0 ? space.mutable_data_ptr() : nullptr, *const stream = stream_of((int)p.device);
+        const float scale = (float)PyFloat_AS_DOUBLE(args[3]);
+        Py_BEGIN_ALLOW_THREADS;
+        rc = g_attention(p.handle, elem, heads, qp, yp, strides, tokens, (const int32_t*)b[0], b[1], b[2], (const int32_t*)b[3], (const int32_t*)b[4], (int)b[5],
+                         (const int32_t*)b[6], b[7], b[8], scale, 1, sp, need, stream);
+        Py_END_ALLOW_THREADS;
+        return finish(rc, rc == 0 ? THPVariable_Wrap(std::move(y)) : nullptr);
+    });
+}
+
+PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t count) {  // target, drafts, uniforms, draft_probs, counts, temperature
+    return guarded([&]() -> PyObject* {
+        if (count != 6 || !undisturbed()) {
+            return not_plain();
+        }
+        const at::Tensor* const x = plain_strided(args[0], 3, -1);
+        if (x == nullptr || elem_of(*x) < 0 || x->size(1) < 2) {
+            return not_plain();
+        }
+        const int64_t device = x->get_device(), n = x->size(0), rows = x->size(1), vocab = x->size(2);
+        const bool logits = args[5] != Py_None;
+        if (logits && !PyFloat_CheckExact(args[5])) {
+            return not_plain();
+        }
+        const double temperature = logits ? PyFloat_AS_DOUBLE(args[5]) : 0.0;
+        const at::Tensor* const drafts = whole(args[1], {n, rows - 1}, device);
+        const at::Tensor* const u = plain(args[2], at::kFloat);
+        const at::Tensor* q = nullptr;
+        const at::Tensor* counts = nullptr;
+        if (drafts == nullptr || u == nullptr || u->get_device() != device || u->sizes() != at::IntArrayRef({n, rows})) {
+            return not_plain();
+        }
+        if (args[3] != Py_None) {
+            q = plain_strided(args[3], 3, device);
+            if (q == nullptr || q->scalar_type() != at::kFloat || q->sizes() != at::IntArrayRef({n, rows - 1, vocab})) {
+                return not_plain();
+            }
+        }
+        if (args[4] != Py_None) {
+            counts = whole(args[4], {n}, device);
+            if (counts == nullptr) {
+                return not_plain();
+            }
+        }
+        int64_t need = 0;
+        int rc = g_verify_bytes(n, rows - 1, vocab, logits, &need);
+        if (rc != 0) {
+            return finish(rc, nullptr);
+        }
+        const at::TensorOptions options = x->options().dtype(at::kInt);
+        at::Tensor accepted = at::cuda::empty({n}, options), tokens = at::cuda::empty({n, rows}, options), space;
+        if (need > 0) {
+            space = at::cuda::empty({need}, options.dtype(at::kByte));
+        }
+        const void* const xp = x->const_data_ptr();
+        const int64_t xb = x->stride(0), xr = x->stride(1), qb = q != nullptr ? q->stride(0) : 0, qr = q != nullptr ? q->stride(1) : 0;
+        const int32_t *const dp = (const int32_t*)drafts->const_data_ptr(), *const cp = counts != nullptr ? (const int32_t*)counts->const_data_ptr() : nullptr;
+        const float *const up = (const float*)u->const_data_ptr(), *const qp = q != nullptr ? (const float*)q->const_data_ptr() : nullptr;
+        int32_t *const ap = (int32_t*)accepted.mutable_data_ptr(), *const tp = (int32_t*)tokens.mutable_data_ptr();
+        void *const sp = need > 0 ? space.mutable_data_ptr() : nullptr, *const stream = stream_of((int)device);
+        const int elem = elem_of(*x);
+        Py_BEGIN_ALLOW_THREADS;
+        rc = g_verify((int)device, elem, xp, xb, xr, dp, qp, qb, qr, up, cp, n, rows - 1, vocab, logits, temperature, ap, tp, sp, need, stream);
+        Py_END_ALLOW_THREADS;
+        if (rc != 0) {
+            return finish(rc, nullptr);
+        }
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(accepted)), THPVariable_Wrap(std::move(tokens)));
+    });
+}
+
+// bind_paged(Rope, PagedCache, PagedBatch, addresses of jq_rope_apply, jq_pages_append, jq_pages_attention_bytes, jq_pages_attention, jq_verify_bytes, jq_verify_drafts)
+PyObject* bind_paged(PyObject*, PyObject* args) {
+    PyObject *r, *p, *b;
+    unsigned long long f[6];
+    if (!PyArg_ParseTuple(args, "OOOKKKKKK", &r, &p, &b, &f[0], &f[1], &f[2], &f[3], &f[4], &f[5])) {
+        return nullptr;
+    }
+    Py_XSETREF(g_rope, Py_NewRef(r));
+    Py_XSETREF(g_pages, Py_NewRef(p));
+    Py_XSETREF(g_batch, Py_NewRef(b));
+    g_rope_apply = (RopeApply)f[0];
+    g_append = (Append)f[1];
+    g_attention_bytes = (AttentionBytes)f[2];
+    g_attention = (Attention)f[3];
+    g_verify_bytes = (VerifyBytes)f[4];
+    g_verify = (Verify)f[5];
+    Py_RETURN_NONE;
+}
+
 // bind(weight class, check, addresses of jq_linear_f32, jq_linear_bf16, jq_linear_backward_f32, jq_dequantize, jq_quantize_q8_0)
 PyObject* bind(PyObject*, PyObject* args) {
     PyObject *weight, *check;
@@ -267,6 +599,11 @@ PyMethodDef METHODS[] = {
     {"backward", (PyCFunction)(void (*)(void))backward, METH_FASTCALL, nullptr},
     {"dequantize", (PyCFunction)(void (*)(void))dequantize, METH_FASTCALL, nullptr},
     {"quantize", (PyCFunction)(void (*)(void))quantize, METH_FASTCALL, nullptr},
+    {"bind_paged", bind_paged, METH_VARARGS, nullptr},
+    {"rope", (PyCFunction)(void (*)(void))rope, METH_FASTCALL, nullptr},
+    {"append", (PyCFunction)(void (*)(void))append, METH_FASTCALL, nullptr},
+    {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, nullptr},
+    {"verify", (PyCFunction)(void (*)(void))verify, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_front", nullptr, -1, METHODS, nullptr, nullptr, nullptr, nullptr};
@@ -277,5 +614,16 @@ PyMODINIT_FUNC PyInit__front(void) {
     s_addr = PyUnicode_InternFromString("_addr");
     s_dims = PyUnicode_InternFromString("_dims");
     s_device = PyUnicode_InternFromString("_device");
-    return s_addr != nullptr && s_dims != nullptr && s_device != nullptr ? PyModule_Create(&MODULE) : nullptr;
+    s_plain_device = PyUnicode_InternFromString("device");
+    s_kv_heads = PyUnicode_InternFromString("kv_heads");
+    s_head_dim = PyUnicode_InternFromString("head_dim");
+    s_code = PyUnicode_InternFromString("_code");
+    s_rows = PyUnicode_InternFromString("_rows");
+    s_ahead = PyUnicode_InternFromString("_ahead");
+    for (PyObject* name : {s_addr, s_dims, s_device, s_plain_device, s_kv_heads, s_head_dim, s_code, s_rows, s_ahead}) {
+        if (name == nullptr) {
+            return nullptr;
+        }
+    }
+    return PyModule_Create(&MODULE);
 }

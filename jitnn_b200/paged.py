@@ -8,9 +8,11 @@ beside their arguments is allocated by torch for that call.
 import ctypes
 import math
 
-from . import _lib
+from . import _lib, ops
 from ._lib import check
 from .ops import _raw_stream, _t
+
+# The plain calls, with outputs of their own, are methods of the native front (csrc/front.cpp) where there is one; it hands back None for everything else, which goes on here.
 
 _ELEM = {"F32": 0, "F16": 1, "BF16": 2}
 
@@ -110,6 +112,7 @@ class Rope:
         h = ctypes.c_void_p()
         check(_lib.load().jq_rope_create(device, positions, dim, (ctypes.c_double * len(freqs))(*freqs), magnitude, int(interleaved), ctypes.byref(h)))
         self._h, self.positions, self.dim, self.device = h, positions, dim, device
+        self._addr = h.value
 
     def _handle(self):
         if self._h is None:
@@ -119,10 +122,18 @@ class Rope:
     def rotate(self, x, positions, out=None):
         """x [tokens, heads, head size] or [batch, tokens, heads, head size], or a pair of such (queries, keys), rotated. ``positions``: an int32 or int64 CUDA tensor
         [tokens] or [batch, tokens], or the int position of the first token. ``out`` may be x."""
+        if ops._front is not None and out is None:
+            y = ops._front.rope(self, x, positions, 0)
+            if y is not None:
+                return y
         return self._turn(x, positions, out, 0, "rotation")
 
     def backward(self, g, positions, out=None):
         """The gradient of x from the gradient of ``rotate(x, positions)``."""
+        if ops._front is not None and out is None:
+            y = ops._front.rope(self, g, positions, 1)
+            if y is not None:
+                return y
         return self._turn(g, positions, out, 1, "rotation backward")
 
     def _turn(self, x, positions, out, inverse, what):
@@ -163,7 +174,7 @@ class Rope:
 
     def release(self):
         if self._h is not None:
-            h, self._h = self._h, None
+            h, self._h, self._addr = self._h, None, 0
             check(_lib.load().jq_rope_free(h))
 
     def __del__(self):
@@ -221,6 +232,7 @@ class PagedCache:
         check(_lib.load().jq_pages_create(device, code, pages, page_size, kv_heads, head_dim, k.data_ptr(), v.data_ptr(), ctypes.byref(h)))
         self._h, self.k, self.v, self.device, self.dtype = h, k, v, device, t
         self.pages, self.page_size, self.kv_heads, self.head_dim = pages, page_size, kv_heads, head_dim
+        self._addr, self._code, self._scale = h.value, code, 1.0 / math.sqrt(head_dim)
 
     def _handle(self):
         if self._h is None:
@@ -240,6 +252,10 @@ class PagedCache:
     def append(self, q, k, v, batch, rope=None, out=None):
         """Stores the rows k and v [tokens, kv_heads, head_dim] on their sequences' pages, k rotated by ``rope`` at each row's position, and returns q [tokens, heads,
         head_dim] rotated likewise (``out``, which may be q; None where q is None). Rows of no sequence become zero in a new tensor, and stay as they are in ``out``."""
+        if ops._front is not None and out is None:
+            y = ops._front.append(self, q, k, v, batch, rope)
+            if y is not None:
+                return y
         torch = _t()
         h = self._handle()
         self._on_pages(batch)
@@ -267,6 +283,11 @@ class PagedCache:
     def attention(self, q, batch, scale=None, out=None):
         """softmax(scale q . k) v [tokens, heads, head_dim] of each row over the prefix and its sequence's keys up to its own; ``scale`` is 1 / sqrt(head_dim) where it
         is None. Neighbouring heads share a key/value head. A row that sees no key, or only keys with scores of negative infinity, gives zeros; rows of no sequence become zero in a new tensor, and stay as they are in ``out``."""
+        scale = self._scale if scale is None else float(scale)
+        if ops._front is not None and out is None:
+            y = ops._front.attention(self, q, batch, scale)
+            if y is not None:
+                return y
         torch = _t()
         h = self._handle()
         self._on_pages(batch)
@@ -283,13 +304,13 @@ class PagedCache:
             space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
             strides = (ctypes.c_int64 * 4)(q.stride(0), q.stride(1), y.stride(0), y.stride(1))
             check(L.jq_pages_attention(h, code, q.shape[1], q.data_ptr(), y.data_ptr(), strides, q.shape[0], *batch._rows, *batch._ahead,
-                                       1.0 / math.sqrt(self.head_dim) if scale is None else scale, int(out is None), None if space is None else space.data_ptr(), need.value,
+                                       scale, int(out is None), None if space is None else space.data_ptr(), need.value,
                                        _raw_stream(torch, self.device)))
         return y
 
     def release(self):
         if self._h is not None:
-            h, self._h = self._h, None
+            h, self._h, self._addr = self._h, None, 0
             check(_lib.load().jq_pages_free(h))
 
     def __del__(self):
@@ -310,6 +331,11 @@ class Speculative:
 
         Draft i is kept while uniforms[i] q_i(x_i) < p_i(x_i), then one token is drawn at uniforms[drafts], from max(p - q, 0) behind the first refused draft and from p
         behind the last. ``tokens``: the drafts kept, that token, -1 in the rest. Temperature 0 takes the likeliest token instead and needs no uniforms. All in double."""
+        temperature = None if temperature is None else float(temperature)
+        if ops._front is not None:
+            y = ops._front.verify(target, drafts, uniforms, draft_probs, counts, temperature)
+            if y is not None:
+                return y
         torch = _t()
         if not isinstance(target, torch.Tensor) or target.dim() != 3 or not target.is_cuda:
             raise ValueError("verify: a CUDA tensor [sequences, drafts + 1, vocab] of logits or probabilities is needed")
@@ -344,6 +370,6 @@ class Speculative:
         space = torch.empty(need.value, dtype=torch.uint8, device=target.device) if need.value else None
         check(L.jq_verify_drafts(device, code, target.data_ptr(), target.stride(0), target.stride(1), drafts.data_ptr(), None if draft_probs is None else draft_probs.data_ptr(),
                                  qb, qr, None if uniforms is None else uniforms.data_ptr(), None if counts is None else counts.data_ptr(), n, rows - 1, vocab, int(logits),
-                                 float(temperature) if logits else 0.0, accepted.data_ptr(), tokens.data_ptr(), None if space is None else space.data_ptr(), need.value,
+                                 temperature if logits else 0.0, accepted.data_ptr(), tokens.data_ptr(), None if space is None else space.data_ptr(), need.value,
                                  _raw_stream(torch, device)))
         return accepted, tokens
