@@ -7,8 +7,10 @@
 // The results are whole numbers that may not depend on how the work is cut, so everything is computed in double: the products u q of two floats are exact, sums of a
 // vocabulary's probabilities are good to 1e-14, and a cut in another place moves a token with a chance of about 1e-10.
 //
-// Logits: stats_kernel takes the maximum and the sum of exponentials of chunks of all rows that count, bound by reading them. choose_kernel is one cluster per sequence:
-// it joins the chunks, finds the row, adds up the row's weights (its second reading, from L2) and looks the token up.
+// Logits: stats_kernel takes the maximum and the sum of exponentials of chunks of all rows that count. choose_kernel is one cluster per sequence: it joins the chunks, finds the
+// row, adds up the row's weights (its second reading, from L2) and looks the token up. The exponential is table-driven (Tang 1989): 2^(t / 32) = 2^n 2^(j / 32) 2^(r / 32) with
+// the 32 values of the middle factor in a warp's lanes and a polynomial of the fifth degree, |r| <= 1/2, 13 double instructions where exp() takes about 48.
+// Bound: 64 of those a clock and SM, 11 us for the 16.8 million logits of 16 sequences with 8 rows of 131072, beside 10 us for reading them.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -20,14 +22,16 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int STATS_THREADS = 256, HELD = 32, CHUNK_MOST = STATS_THREADS * HELD;  // a thread's values of a chunk stay in registers
-constexpr int CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32, CLUSTER = 8;
+constexpr int STATS_THREADS = 256, CHUNK_MOST = 8192;  // (a chunk stays in the first-level cache between its two readings)
+constexpr int CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32, CLUSTER = 8;  // (the largest)
 
 struct Stat {
     double sum;  // of exp((x - top) / temperature)
     float top;
     int at;      // where top is first
 };
+
+enum { GREEDY, LOGITS, PROBABILITIES };  // what the target is taken as
 
 struct VerifyArgs {
     const void* target;
@@ -39,44 +43,49 @@ struct VerifyArgs {
     const int* counts;
     int sequences, drafts_most, vocab;
     double inverse;     // of the temperature
-    int form;           // GREEDY, LOGITS, PROBABILITIES
     int *accepted, *tokens;
     Stat* stats;        // [row][chunks]
     int chunk, chunks;
+    int cluster;        // thread blocks of a sequence's choice
     int* status;
 };
-enum { GREEDY, LOGITS, PROBABILITIES };
 
 __device__ __forceinline__ int count_of(const VerifyArgs& a, int b) {
     const int n = a.counts != nullptr ? a.counts[b] : a.drafts_most;
     return n < 0 ? 0 : (n > a.drafts_most ? a.drafts_most : n);
 }
 
+// exp((x - top) inverse) of a warp's 32 numbers; every lane has 2^(lane / 32) in `entry`. Off by less than 4e-15 of it: the polynomial's remainder is (ln 2 / 64)^6 / 720 = 2.2e-15,
+// the roundings of t (whose integer part is at most 2^15 here) and of the products the rest.
+struct Exponential {
+    double to_32nds, entry;  // 32 / ln 2 times inverse
+    float far;               // x - top below this: less than e^-690, taken as zero (minus infinity too)
+    __device__ __forceinline__ Exponential(double inverse, int lane) : to_32nds(inverse * 46.166241308446828384), entry(exp2(lane / 32.0)), far((float)(-690.0 / inverse)) {}
+    // Of x far below, zero (ZERO), or something no larger than e^-690 (a NaN too).
+    template <bool ZERO>
+    __device__ __forceinline__ double of(float x, float top) const {
+        if (!ZERO) {
+            x = fmaxf(x, top + far);
+        }
+        const double t = ((double)x - (double)top) * to_32nds;
+        const double shifted = t + 6755399441055744.0;  // 2^52 + 2^51: the nearest integer in the low bits
+        const int k = __double2loint(shifted);
+        const double r = t - (shifted - 6755399441055744.0);
+        // (2^(r / 32) - 1) = sum (r ln 2 / 32)^i / i!
+        constexpr double A = 0.021660849392498290, A2 = A * A / 2, A3 = A * A * A / 6, A4 = A * A * A * A / 24, A5 = A * A * A * A * A / 120;
+        const double p = r * fma(r, fma(r, fma(r, fma(r, A5, A4), A3), A2), A);
+        const double e = __shfl_sync(0xffffffffu, entry, k & 31);
+        const double v = fma(e, p, e);
+        const double scaled = __hiloint2double(__double2hiint(v) + ((k & ~31) << 15), __double2loint(v));  // (times 2^(k / 32))
+        return ZERO && x - top < far ? 0.0 : scaled;
+    }
+};
+
 __device__ __forceinline__ bool before(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
 
-template <typename T>
-__global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
-    __shared__ double sums[STATS_THREADS / 32];
-    __shared__ float tops[STATS_THREADS / 32];
-    __shared__ int ats[STATS_THREADS / 32];
-    const int row = blockIdx.y, b = row / (a.drafts_most + 1), i = row % (a.drafts_most + 1), tid = threadIdx.x;
-    if (i > count_of(a, b)) {
-        return;
-    }
-    const T* x = static_cast<const T*>(a.target) + b * a.tb + i * a.tr;
-    const int c0 = blockIdx.x * a.chunk, c1 = c0 + a.chunk < a.vocab ? c0 + a.chunk : a.vocab;
-    float v[HELD];
-    float top = -INFINITY;
-    int at = 0x7fffffff;
+// The largest of a warp's numbers and where it is first.
+__device__ __forceinline__ void warp_top(float& top, int& at) {
 #pragma unroll
-    for (int n = 0; n < HELD; n++) {
-        const int j = c0 + n * STATS_THREADS + tid;
-        v[n] = j < c1 ? to_float(x[j]) : -INFINITY;
-        if (j < c1 && before(v[n], j, top, at)) {
-            top = v[n];
-            at = j;
-        }
-    }
     for (int o = 16; o > 0; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, top, o);
         const int j = __shfl_xor_sync(0xffffffffu, at, o);
@@ -85,6 +94,68 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
             at = j;
         }
     }
+}
+__device__ __forceinline__ double warp_total(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    }
+    return v;
+}
+__device__ __forceinline__ double warp_scan(double v, int lane) {  // sums up to and with each lane
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double n = __shfl_up_sync(0xffffffffu, v, o);
+        v += lane >= o ? n : 0.0;
+    }
+    return v;
+}
+
+// A chunk of a row: its maximum, then (a second reading) the sum. Eight values a thread are on their way at a time.
+template <typename T, bool SUMS>
+__global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
+    constexpr int TAKE = 8, STEP = TAKE * STATS_THREADS;
+    __shared__ double sums[STATS_THREADS / 32];
+    __shared__ float tops[STATS_THREADS / 32];
+    __shared__ int ats[STATS_THREADS / 32];
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int row = blockIdx.y, b = row / (a.drafts_most + 1), i = row % (a.drafts_most + 1), tid = threadIdx.x;
+    if (i > count_of(a, b)) {
+        return;
+    }
+    const T* x = static_cast<const T*>(a.target) + b * a.tb + i * a.tr;
+    const int c0 = blockIdx.x * a.chunk, c1 = c0 + a.chunk < a.vocab ? c0 + a.chunk : a.vocab;
+    float top = -INFINITY;
+    int at = 0x7fffffff;
+    auto values = [&](int j0, float (&v)[TAKE]) {  // j0, j0 + STATS_THREADS ..., minus infinity behind the end
+        if (j0 + (TAKE - 1) * STATS_THREADS < c1) {
+#pragma unroll
+            for (int n = 0; n < TAKE; n++) {
+                v[n] = to_float(x[j0 + n * STATS_THREADS]);
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < TAKE; n++) {
+                v[n] = j0 + n * STATS_THREADS < c1 ? to_float(x[j0 + n * STATS_THREADS]) : -INFINITY;
+            }
+        }
+    };
+#pragma unroll 1
+    for (int j0 = c0 + tid; j0 < c1; j0 += STEP) {
+        float v[TAKE];
+        values(j0, v);
+#pragma unroll
+        for (int n = 0; n < TAKE; n++) {
+            if constexpr (SUMS) {
+                top = fmaxf(top, v[n]);
+            } else {  // (in rising order: the first of equal ones stays)
+                const bool larger = v[n] > top || (at == 0x7fffffff && v[n] == top && j0 + n * STATS_THREADS < c1);
+                at = larger ? j0 + n * STATS_THREADS : at;
+                top = larger ? v[n] : top;
+            }
+        }
+    }
+    warp_top(top, at);
     if ((tid & 31) == 0) {
         tops[tid >> 5] = top;
         ats[tid >> 5] = at;
@@ -99,16 +170,20 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
         }
     }
     double sum = 0.0;
-    if (a.form == LOGITS) {
+    if (SUMS && top != -INFINITY) {
+        const Exponential exponential(a.inverse, tid & 31);
+#pragma unroll 1
+        for (int j0 = c0 + (tid & ~31); j0 < c1; j0 += STEP) {
+            float v[TAKE];
+            values(j0 + (tid & 31), v);
+            double part = 0.0;
 #pragma unroll
-        for (int n = 0; n < HELD; n++) {
-            if (c0 + n * STATS_THREADS + tid < c1 && v[n] != -INFINITY) {
-                sum += exp(((double)v[n] - (double)top) * a.inverse);
+            for (int n = 0; n < TAKE; n++) {
+                part += exponential.of<false>(v[n], top);
             }
+            sum += part;
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
+        sum = warp_total(sum);
         if ((tid & 31) == 0) {
             sums[tid >> 5] = sum;
         }
@@ -123,171 +198,160 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
     }
 }
 
-// One cluster per sequence; thread block r of it has a run of the vocabulary, each warp a run of that.
-template <typename T>
-__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
-    __shared__ double of_warp[CHOOSE_WARPS], upto[CLUSTER * CHOOSE_WARPS + 1];  // a warp's weight; the weight in front of each warp of the cluster
-    __shared__ int last_some, likeliest;  // the last warp that has any weight; the first of the largest
-    __shared__ double row_top, row_scale;  // of the row that is drawn from: p = exp((x - top) / temperature) scale
-    __shared__ int refused;
-    cg::cluster_group cluster = cg::this_cluster();
-    const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
-    const int b = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int count = count_of(a, b), rows = a.drafts_most + 1;
-    const T* const target = static_cast<const T*>(a.target) + b * a.tb;
-    if (tid == 0) {
-        refused = count;
+// A row's chunks joined, by a warp.
+template <int FORM>
+__device__ __forceinline__ void join_chunks(const VerifyArgs& a, int64_t row, int lane, float& top, int& at, double& sum) {
+    const Stat* const st = a.stats + row * a.chunks;
+    top = -INFINITY;
+    at = 0x7fffffff;
+    sum = 0.0;
+    for (int c = lane; c < a.chunks; c += 32) {
+        if (before(st[c].top, st[c].at, top, at)) {
+            top = st[c].top;
+            at = st[c].at;
+        }
     }
-    __syncthreads();
-    // every thread block finds the row by itself; a warp has a row
-    for (int i = warp; i <= count; i += CHOOSE_WARPS) {
-        float top = -INFINITY;
-        int at = 0x7fffffff;
-        double sum = 0.0;
-        if (a.form != PROBABILITIES) {
-            const Stat* st = a.stats + ((int64_t)b * rows + i) * a.chunks;
-            for (int c = lane; c < a.chunks; c += 32) {
-                if (before(st[c].top, st[c].at, top, at)) {
-                    top = st[c].top;
-                    at = st[c].at;
-                }
-            }
-            for (int o = 16; o > 0; o >>= 1) {
-                const float w = __shfl_xor_sync(0xffffffffu, top, o);
-                const int j = __shfl_xor_sync(0xffffffffu, at, o);
-                if (before(w, j, top, at)) {
-                    top = w;
-                    at = j;
-                }
-            }
-            if (a.form == LOGITS) {
-                for (int c = lane; c < a.chunks; c += 32) {
-                    if (st[c].top != -INFINITY) {
-                        sum += st[c].sum * exp(((double)st[c].top - (double)top) * a.inverse);
-                    }
-                }
-                for (int o = 16; o > 0; o >>= 1) {
-                    sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                }
+    warp_top(top, at);
+    if constexpr (FORM == LOGITS) {
+        for (int c = lane; c < a.chunks; c += 32) {
+            if (st[c].top != -INFINITY) {
+                sum += st[c].sum * exp(((double)st[c].top - (double)top) * a.inverse);
             }
         }
-        if (lane == 0 && i < count) {
-            const int x = a.drafts[b * a.drafts_most + i];
-            bool good = x >= 0 && x < a.vocab;
-            if (!good) {
-                note_status(a.status, STATUS_TOKEN);
-            } else if (a.form == GREEDY) {
-                good = x == at;
-            } else {
-                const double t = to_float(target[i * a.tr + x]);
-                const double p = a.form == LOGITS ? exp((t - (double)top) * a.inverse) / sum : t;
-                const double q = a.q != nullptr ? (double)a.q[b * a.qb + i * a.qr + x] : 1.0;
-                good = (double)a.u[(int64_t)b * rows + i] * q < p;
+        sum = warp_total(sum);
+    }
+}
+
+// One cluster per sequence (one thread block at temperature 0); thread block r of it has a run of the vocabulary, each warp a run of that.
+template <typename T, int FORM>
+__global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
+    __shared__ double of_warp[CHOOSE_WARPS], of_part[CHOOSE_WARPS], upto[CLUSTER * CHOOSE_WARPS + 1];  // a warp's weight, or a part's; the weight in front of each warp of the cluster
+    __shared__ int last_some;    // the last warp that has any weight
+    __shared__ double row_sum[CHOOSE_WARPS];  // of the last row that each warp has looked at, which one of them goes on with: p = exp((x - top) / temperature) / sum
+    __shared__ float row_top[CHOOSE_WARPS];
+    __shared__ int row_at[CHOOSE_WARPS], refused;
+    const int blocks = FORM == GREEDY ? 1 : a.cluster, rank = blockIdx.x % blocks, b = blockIdx.x / blocks;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rows = a.drafts_most + 1;
+    if (tid == 0) {
+        refused = 0x7fffffff;
+    }
+    const Exponential exponential(FORM == LOGITS ? a.inverse : 1.0, lane);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int count = count_of(a, b);
+    const T* const target = static_cast<const T*>(a.target) + b * a.tb;
+    __syncthreads();
+    // ---- the first refused draft: every thread block finds it by itself, a warp a draft
+    for (int i = warp; i <= count; i += CHOOSE_WARPS) {
+        const int x = i < count ? a.drafts[b * a.drafts_most + i] : 0;
+        bool good = x >= 0 && x < a.vocab;
+        float top = 0.0f;
+        int at = 0;
+        double sum = 0.0;
+        if constexpr (FORM != PROBABILITIES) {
+            join_chunks<FORM>(a, (int64_t)b * rows + i, lane, top, at, sum);
+            if (lane == 0) {
+                row_top[warp] = top;
+                row_at[warp] = at;
+                row_sum[warp] = sum;
             }
-            if (!good) {
+        }
+        if (i == count) {
+            break;
+        }
+        if (!good) {
+            note_status(a.status, STATUS_TOKEN);
+        } else if constexpr (FORM == GREEDY) {
+            good = x == at;
+        } else {
+            const double t = to_float(target[i * a.tr + x]);
+            const double p = FORM == LOGITS ? exp((t - (double)top) * a.inverse) / sum : t;
+            const double q = a.q != nullptr ? (double)a.q[b * a.qb + i * a.qr + x] : 1.0;
+            good = (double)a.u[(int64_t)b * rows + i] * q < p;
+        }
+        if (!good) {
+            if (lane == 0) {
                 atomicMin(&refused, i);
             }
+            break;  // (this warp's later drafts are behind it)
         }
     }
     __syncthreads();
-    const int j = refused;
-    // the row's maximum and sum once more, for whoever needs them
-    if (warp == 0 && a.form != PROBABILITIES) {
-        const Stat* st = a.stats + ((int64_t)b * rows + j) * a.chunks;
-        float top = -INFINITY;
-        int at = 0x7fffffff;
-        for (int c = lane; c < a.chunks; c += 32) {
-            if (before(st[c].top, st[c].at, top, at)) {
-                top = st[c].top;
-                at = st[c].at;
-            }
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            const float w = __shfl_xor_sync(0xffffffffu, top, o);
-            const int n = __shfl_xor_sync(0xffffffffu, at, o);
-            if (before(w, n, top, at)) {
-                top = w;
-                at = n;
-            }
-        }
-        double sum = 0.0;
-        if (a.form == LOGITS) {
-            for (int c = lane; c < a.chunks; c += 32) {
-                if (st[c].top != -INFINITY) {
-                    sum += st[c].sum * exp(((double)st[c].top - (double)top) * a.inverse);
-                }
-            }
-            for (int o = 16; o > 0; o >>= 1) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
-        }
-        if (lane == 0) {
-            row_top = top;
-            row_scale = 1.0 / sum;
-            if (a.form == GREEDY) {
-                likeliest = at < a.vocab ? at : 0;
-            }
-        }
-    }
-    __syncthreads();
-    if (a.form != GREEDY) {
+    const int j = refused < count ? refused : count;
+    if constexpr (FORM != GREEDY) {
+        cg::cluster_group cluster = cg::this_cluster();
         const T* const x = target + j * a.tr;
-        const double top = row_top, scale = row_scale;
+        const float top = row_top[j % CHOOSE_WARPS];
+        const double scale = 1.0 / row_sum[j % CHOOSE_WARPS];
         const int draft = j < count ? a.drafts[b * a.drafts_most + j] : -1;
         const float* const q = j < count && a.q != nullptr ? a.q + b * a.qb + j * a.qr : nullptr;
-        // a warp's run of the vocabulary, in steps of 32
-        const int per = (a.vocab + blocks * CHOOSE_WARPS * 32 - 1) / (blocks * CHOOSE_WARPS * 32) * 32;
-        const int from = (rank * CHOOSE_WARPS + warp) * per;
-        const int to = from + per < a.vocab ? from + per : a.vocab;
         bool less = j < count;  // whether the drafter's share is taken off
-        auto weight = [&](int v) {
-            const double t = to_float(x[v]);
-            double p = a.form == LOGITS ? (t == -INFINITY ? 0.0 : exp((t - top) * a.inverse) * scale) : t;
-            if (less) {
-                p = q != nullptr ? p - (double)q[v] : (v == draft ? 0.0 : p);
+        // the weights of N times 32 values from `at` on (none from `end` on), by a warp: a lane has the values lane, lane + 32 ...
+        auto weigh = [&](int at, int end, auto& w) {
+            constexpr int N = sizeof(w) / sizeof(w[0]);
+            float t[N], share[N];
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const int v = at + 32 * i + lane;
+                t[i] = v < end ? to_float(x[v]) : (FORM == LOGITS ? -INFINITY : 0.0f);
+                share[i] = v < end && less && q != nullptr ? q[v] : 0.0f;
             }
-            return p > 0.0 ? p : 0.0;  // (a NaN counts as nothing)
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                double p;
+                if constexpr (FORM == LOGITS) {
+                    p = exponential.of<true>(t[i], top) * scale;
+                } else {
+                    p = (double)t[i];
+                }
+                const double rest = less && q == nullptr && at + 32 * i + lane == draft ? 0.0 : p - (double)share[i];
+                w[i] = rest > 0.0 ? rest : 0.0;  // (a NaN counts as nothing)
+            }
         };
-        double total = 0.0;
-        for (int round = 0; round < 2; round++) {
+        auto total_of = [&](int from, int to) {  // the weight of a run, by a warp
             double sum = 0.0;
-            for (int v = from + lane; v < to; v += 32) {
-                sum += weight(v);
+#pragma unroll 1
+            for (int at = from; at < to; at += 8 * 32) {
+                double w[8];
+                weigh(at, to, w);
+                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
             }
-            for (int o = 16; o > 0; o >>= 1) {
-                sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            }
+            return warp_total(sum);
+        };
+        // a warp's run of the vocabulary, and a sixteenth of it
+        const int part = (int)(((int64_t)a.vocab + blocks * CHOOSE_WARPS * CHOOSE_WARPS * 32 - 1) / (blocks * CHOOSE_WARPS * CHOOSE_WARPS * 32)) * 32, per = part * CHOOSE_WARPS;
+        auto begin_of = [&](int w) { return (int)((int64_t)w * per < a.vocab ? w * per : a.vocab); };
+        const int me = rank * CHOOSE_WARPS + warp;
+        double total = 0.0;
+#pragma unroll 1
+        for (int round = 0; round < 2; round++) {
+            const double sum = total_of(begin_of(me), begin_of(me + 1));
             if (lane == 0) {
                 of_warp[warp] = sum;
             }
             cluster.sync();
             // every thread block makes the same sums up to each warp of the cluster, whose intervals leave no gap
             if (warp == 0) {
-                double each[CLUSTER * CHOOSE_WARPS / 32], run = 0.0;
+                constexpr int N = CLUSTER * CHOOSE_WARPS / 32;  // (of smaller clusters the last have nothing)
+                double each[N], run = 0.0;
                 int last = -1;
 #pragma unroll
-                for (int n = 0; n < CLUSTER * CHOOSE_WARPS / 32; n++) {
-                    const int w = lane * (CLUSTER * CHOOSE_WARPS / 32) + n;
-                    each[n] = *cluster.map_shared_rank(&of_warp[w % CHOOSE_WARPS], w / CHOOSE_WARPS);
+                for (int n = 0; n < N; n++) {
+                    const int w = lane * N + n;
+                    each[n] = w < blocks * CHOOSE_WARPS ? *cluster.map_shared_rank(&of_warp[w % CHOOSE_WARPS], w / CHOOSE_WARPS) : 0.0;
                     run += each[n];
                     last = each[n] > 0.0 ? w : last;
                 }
-                double scan = run;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double n = __shfl_up_sync(0xffffffffu, scan, o);
-                    scan += lane >= o ? n : 0.0;
-                }
-                double upto_here = __shfl_up_sync(0xffffffffu, scan, 1);
-                upto_here = lane == 0 ? 0.0 : upto_here;
+                const double scan = warp_scan(run, lane);
+                double here = __shfl_up_sync(0xffffffffu, scan, 1);
+                here = lane == 0 ? 0.0 : here;
 #pragma unroll
-                for (int n = 0; n < CLUSTER * CHOOSE_WARPS / 32; n++) {
-                    upto[lane * (CLUSTER * CHOOSE_WARPS / 32) + n] = upto_here;
-                    upto_here += each[n];
+                for (int n = 0; n < N; n++) {
+                    upto[lane * N + n] = here;
+                    here += each[n];
                 }
-                upto_here = __shfl_sync(0xffffffffu, upto_here, 31);
                 last = __reduce_max_sync(0xffffffffu, last);
-                if (lane == 0) {
-                    upto[CLUSTER * CHOOSE_WARPS] = upto_here;
+                if (lane == 31) {
+                    upto[CLUSTER * CHOOSE_WARPS] = here;
                     last_some = last;
                 }
             }
@@ -300,26 +364,38 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
             less = false;  // p nowhere above q: they are the same
         }
         const double aim = (double)a.u[(int64_t)b * rows + a.drafts_most] * total;
-        const int me = rank * CHOOSE_WARPS + warp;
-        // the warp whose run the aim falls into; with a uniform number of 1 or more, or none at all, the last that has any weight
-        if (aim < total ? upto[me] <= aim && aim < upto[me + 1] : me == last_some) {
-            double run = upto[me];
-            int found = -1, positive = -1;
-            for (int v0 = from; v0 < to && found < 0; v0 += 32) {
-                const int v = v0 + lane;
-                const double w = v < to ? weight(v) : 0.0;
-                double scan = w;
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double n = __shfl_up_sync(0xffffffffu, scan, o);
-                    scan += lane >= o ? n : 0.0;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, w > 0.0 && run + scan > aim), some = __ballot_sync(0xffffffffu, w > 0.0);
-                positive = some != 0u ? v0 + 31 - __clz(some) : positive;
-                found = hit != 0u ? v0 + __ffs(hit) - 1 : -1;
-                run += __shfl_sync(0xffffffffu, scan, 31);
+        // the warp of this thread block whose run the aim falls into; with a uniform number of 1 or more, or none at all, the last that has any weight
+        const int w = rank * CHOOSE_WARPS + (lane & (CHOOSE_WARPS - 1));
+        const unsigned hit = __ballot_sync(0xffffffffu, aim < total ? upto[w] <= aim && aim < upto[w + 1] : w == last_some);
+        if (hit != 0u) {
+            // all warps look at its run, a sixteenth each; then the one whose sixteenth it is looks it up
+            const int run = rank * CHOOSE_WARPS + __ffs(hit) - 1, end = begin_of(run + 1);
+            auto part_of = [&](int n) { return begin_of(run) + n * part < end ? begin_of(run) + n * part : end; };
+            const double sum = total_of(part_of(warp), part_of(warp + 1));
+            if (lane == 0) {
+                of_part[warp] = sum;
             }
-            if (lane == 0) {  // (not found by a rounding of the sums: the last with any weight)
-                a.tokens[(int64_t)b * rows + j] = found >= 0 ? found : (positive >= 0 ? positive : a.vocab - 1);
+            __syncthreads();
+            const double mine = lane < CHOOSE_WARPS ? of_part[lane] : 0.0, scan = warp_scan(mine, lane) + upto[run];
+            const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && scan > aim), some = __ballot_sync(0xffffffffu, mine > 0.0);
+            const int chosen = over != 0u ? __ffs(over) - 1 : (some != 0u ? 31 - __clz(some) : 0);  // (not found by a rounding of the sums: the last with any weight)
+            const double ahead = __shfl_sync(0xffffffffu, scan - mine, chosen);
+            if (warp == chosen) {
+                double before_it = ahead;
+                int found = -1, positive = -1;
+#pragma unroll 1
+                for (int at = part_of(chosen); at < part_of(chosen + 1) && found < 0; at += 32) {
+                    double v[1];
+                    weigh(at, part_of(chosen + 1), v);
+                    const double upto_here = warp_scan(v[0], lane);
+                    const unsigned is = __ballot_sync(0xffffffffu, v[0] > 0.0 && before_it + upto_here > aim), any = __ballot_sync(0xffffffffu, v[0] > 0.0);
+                    positive = any != 0u ? at + 31 - __clz(any) : positive;
+                    found = is != 0u ? at + __ffs(is) - 1 : -1;
+                    before_it += __shfl_sync(0xffffffffu, upto_here, 31);
+                }
+                if (lane == 0) {
+                    a.tokens[(int64_t)b * rows + j] = found >= 0 ? found : (positive >= 0 ? positive : a.vocab - 1);
+                }
             }
         }
         if (rank == 0 && tid == 0 && last_some < 0) {
@@ -328,8 +404,8 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     }
     if (rank == 0) {
         for (int i = tid; i < rows; i += CHOOSE_THREADS) {
-            if (i != j || a.form == GREEDY) {
-                a.tokens[(int64_t)b * rows + i] = i < j ? a.drafts[b * a.drafts_most + i] : (i == j ? likeliest : -1);
+            if (i != j || FORM == GREEDY) {
+                a.tokens[(int64_t)b * rows + i] = i < j ? a.drafts[b * a.drafts_most + i] : (i == j ? (row_at[j % CHOOSE_WARPS] < a.vocab ? row_at[j % CHOOSE_WARPS] : 0) : -1);
             }
         }
         if (tid == 0) {
@@ -347,32 +423,39 @@ int chunk_of(int64_t rows, int vocab) {
     return chunk;
 }
 
-template <typename T>
+template <typename T, int FORM>
 int launch_verify(const VerifyArgs& a, cudaStream_t s) {
     const int64_t rows = (int64_t)a.sequences * (a.drafts_most + 1);
-    if (a.form != PROBABILITIES) {
-        stats_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)rows), STATS_THREADS, 0, s>>>(a);
+    if constexpr (FORM != PROBABILITIES) {
+        stats_kernel<T, FORM == LOGITS><<<dim3((unsigned)a.chunks, (unsigned)rows), STATS_THREADS, 0, s>>>(a);
         count_launch();
         const int rc = check_launch("stats_kernel");
         if (rc != JQ_OK) {
             return rc;
         }
     }
-    const int blocks = a.form == GREEDY ? 1 : CLUSTER;
+    const int blocks = FORM == GREEDY ? 1 : a.cluster;
     cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)blocks;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = FORM == PROBABILITIES ? 1 : 2;  // behind the statistics programmatically
     cfg.gridDim = dim3((unsigned)(a.sequences * blocks));
     cfg.blockDim = dim3(CHOOSE_THREADS);
     cfg.stream = s;
-    JQ_CUDA(cudaLaunchKernelEx(&cfg, choose_kernel<T>, a));
+    JQ_CUDA(cudaLaunchKernelEx(&cfg, choose_kernel<T, FORM>, a));
     count_launch();
     return JQ_OK;
+}
+
+template <typename T>
+int launch_verify_form(const VerifyArgs& a, int form, cudaStream_t s) {
+    return form == GREEDY ? launch_verify<T, GREEDY>(a, s) : (form == LOGITS ? launch_verify<T, LOGITS>(a, s) : launch_verify<T, PROBABILITIES>(a, s));
 }
 
 }  // namespace
@@ -431,17 +514,21 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     a.drafts = drafts; a.u = uniforms; a.counts = counts;
     a.sequences = (int)sequences; a.drafts_most = (int)drafts_most; a.vocab = (int)vocab;
     a.inverse = form == LOGITS ? 1.0 / temperature : 1.0;
-    a.form = form;
     a.accepted = accepted; a.tokens = tokens;
     a.stats = static_cast<Stat*>(workspace);
     a.chunk = chunk_of(sequences * (drafts_most + 1), a.vocab);
     a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
+    // eight thread blocks a sequence while all of them fit the GPU at once (two to an SM), and not more than leave a warp 256 values
+    a.cluster = CLUSTER;
+    while (a.cluster > 1 && (sequences * a.cluster > 2 * 148 || (int64_t)a.cluster * CHOOSE_WARPS * 256 > 2 * vocab)) {
+        a.cluster /= 2;
+    }
     rc = status_word(&a.status);
     if (rc != JQ_OK) {
         return rc;
     }
     const cudaStream_t s = (cudaStream_t)stream;
-    return elem == JQ_ELEM_F32 ? launch_verify<float>(a, s) : (elem == JQ_ELEM_F16 ? launch_verify<__half>(a, s) : launch_verify<__nv_bfloat16>(a, s));
+    return elem == JQ_ELEM_F32 ? launch_verify_form<float>(a, form, s) : (elem == JQ_ELEM_F16 ? launch_verify_form<__half>(a, form, s) : launch_verify_form<__nv_bfloat16>(a, form, s));
 }
 
 }  // extern "C"
