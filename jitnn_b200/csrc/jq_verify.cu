@@ -22,13 +22,13 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int STATS_THREADS = 256, CHUNK_MOST = 8192;  // (a chunk stays in the first-level cache between its two readings)
+constexpr int STATS_THREADS = 256, CHUNK_MOST = 8192;
 constexpr int CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32, CLUSTER = 8;  // (the largest)
 
 struct Stat {
     double sum;  // of exp((x - top) / temperature)
-    float top;
-    int at;      // where top is first
+    float top;   // one of the chunk's larger numbers, at temperature 0 the largest; minus infinity where there is no other
+    int at;      // where that is first
 };
 
 enum { GREEDY, LOGITS, PROBABILITIES };  // what the target is taken as
@@ -111,7 +111,8 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {  // sums up to
     return v;
 }
 
-// A chunk of a row: its maximum, then (a second reading) the sum. Eight values a thread are on their way at a time.
+// A chunk of a row in one reading, eight values a thread on their way at a time. SUMS: every thread adds exponentials up relative to the largest of its first eight numbers, which
+// in double need not be the largest of all: only a number e^600 times as large moves it. Else the largest and where it is first.
 template <typename T, bool SUMS>
 __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
     constexpr int TAKE = 8, STEP = TAKE * STATS_THREADS;
@@ -119,44 +120,62 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
     __shared__ float tops[STATS_THREADS / 32];
     __shared__ int ats[STATS_THREADS / 32];
     asm volatile("griddepcontrol.launch_dependents;");
-    const int row = blockIdx.y, b = row / (a.drafts_most + 1), i = row % (a.drafts_most + 1), tid = threadIdx.x;
+    const int row = blockIdx.y, b = row / (a.drafts_most + 1), i = row % (a.drafts_most + 1), tid = threadIdx.x, lane = tid & 31;
     if (i > count_of(a, b)) {
         return;
     }
     const T* x = static_cast<const T*>(a.target) + b * a.tb + i * a.tr;
     const int c0 = blockIdx.x * a.chunk, c1 = c0 + a.chunk < a.vocab ? c0 + a.chunk : a.vocab;
+    const Exponential exponential(SUMS ? a.inverse : 1.0, lane);
+    const float reach = SUMS ? (float)(600.0 / a.inverse) : 0.0f;
     float top = -INFINITY;
     int at = 0x7fffffff;
-    auto values = [&](int j0, float (&v)[TAKE]) {  // j0, j0 + STATS_THREADS ..., minus infinity behind the end
-        if (j0 + (TAKE - 1) * STATS_THREADS < c1) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int j0 = c0 + (tid & ~31); j0 < c1; j0 += STEP) {  // (a warp's lanes stay together)
+        float v[TAKE];
+        if (j0 + 31 + (TAKE - 1) * STATS_THREADS < c1) {
 #pragma unroll
             for (int n = 0; n < TAKE; n++) {
-                v[n] = to_float(x[j0 + n * STATS_THREADS]);
+                v[n] = to_float(x[j0 + lane + n * STATS_THREADS]);
             }
         } else {
 #pragma unroll
             for (int n = 0; n < TAKE; n++) {
-                v[n] = j0 + n * STATS_THREADS < c1 ? to_float(x[j0 + n * STATS_THREADS]) : -INFINITY;
+                v[n] = j0 + lane + n * STATS_THREADS < c1 ? to_float(x[j0 + lane + n * STATS_THREADS]) : -INFINITY;
             }
         }
-    };
-#pragma unroll 1
-    for (int j0 = c0 + tid; j0 < c1; j0 += STEP) {
-        float v[TAKE];
-        values(j0, v);
+        if constexpr (SUMS) {
+            float here = v[0];
 #pragma unroll
-        for (int n = 0; n < TAKE; n++) {
-            if constexpr (SUMS) {
-                top = fmaxf(top, v[n]);
-            } else {  // (in rising order: the first of equal ones stays)
-                const bool larger = v[n] > top || (at == 0x7fffffff && v[n] == top && j0 + n * STATS_THREADS < c1);
-                at = larger ? j0 + n * STATS_THREADS : at;
+            for (int n = 1; n < TAKE; n++) {
+                here = fmaxf(here, v[n]);
+            }
+            const bool far = here > top + reach;  // (top is minus infinity at first, and as long as nothing else has come)
+            if (__any_sync(0xffffffffu, far)) {
+                const double shrink = exponential.of<true>(top, far ? here : 0.0f);
+                sum = far && sum != 0.0 ? sum * shrink : sum;
+                top = far ? here : top;
+            }
+            double part = 0.0;
+#pragma unroll
+            for (int n = 0; n < TAKE; n++) {
+                part += exponential.of<false>(v[n], top);
+            }
+            sum += top == -INFINITY ? 0.0 : part;
+        } else {
+#pragma unroll
+            for (int n = 0; n < TAKE; n++) {  // (in rising order: the first of equal ones stays)
+                const int j = j0 + lane + n * STATS_THREADS;
+                const bool larger = v[n] > top || (at == 0x7fffffff && v[n] == top && j < c1);
+                at = larger ? j : at;
                 top = larger ? v[n] : top;
             }
         }
     }
+    const float mine = top;
     warp_top(top, at);
-    if ((tid & 31) == 0) {
+    if (lane == 0) {
         tops[tid >> 5] = top;
         ats[tid >> 5] = at;
     }
@@ -169,22 +188,10 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
             at = ats[w];
         }
     }
-    double sum = 0.0;
-    if (SUMS && top != -INFINITY) {
-        const Exponential exponential(a.inverse, tid & 31);
-#pragma unroll 1
-        for (int j0 = c0 + (tid & ~31); j0 < c1; j0 += STEP) {
-            float v[TAKE];
-            values(j0 + (tid & 31), v);
-            double part = 0.0;
-#pragma unroll
-            for (int n = 0; n < TAKE; n++) {
-                part += exponential.of<false>(v[n], top);
-            }
-            sum += part;
-        }
-        sum = warp_total(sum);
-        if ((tid & 31) == 0) {
+    if constexpr (SUMS) {
+        const double shrink = exponential.of<true>(mine, top);
+        sum = warp_total(sum != 0.0 ? sum * shrink : 0.0);
+        if (lane == 0) {
             sums[tid >> 5] = sum;
         }
         __syncthreads();
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
 
 // A row's chunks joined, by a warp.
 template <int FORM>
-__device__ __forceinline__ void join_chunks(const VerifyArgs& a, int64_t row, int lane, float& top, int& at, double& sum) {
+__device__ __forceinline__ void join_chunks(const VerifyArgs& a, const Exponential& exponential, int64_t row, int lane, float& top, int& at, double& sum) {
     const Stat* const st = a.stats + row * a.chunks;
     top = -INFINITY;
     at = 0x7fffffff;
@@ -213,10 +220,11 @@ __device__ __forceinline__ void join_chunks(const VerifyArgs& a, int64_t row, in
     }
     warp_top(top, at);
     if constexpr (FORM == LOGITS) {
-        for (int c = lane; c < a.chunks; c += 32) {
-            if (st[c].top != -INFINITY) {
-                sum += st[c].sum * exp(((double)st[c].top - (double)top) * a.inverse);
-            }
+        for (int c0 = 0; c0 < a.chunks; c0 += 32) {
+            const int c = c0 + lane;
+            const float t = c < a.chunks ? st[c].top : -INFINITY;
+            const double e = exponential.of<true>(t, top);
+            sum += t != -INFINITY ? st[c].sum * e : 0.0;
         }
         sum = warp_total(sum);
     }
@@ -225,7 +233,7 @@ __device__ __forceinline__ void join_chunks(const VerifyArgs& a, int64_t row, in
 // One cluster per sequence (one thread block at temperature 0); thread block r of it has a run of the vocabulary, each warp a run of that.
 template <typename T, int FORM>
 __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
-    __shared__ double of_warp[CHOOSE_WARPS], of_part[CHOOSE_WARPS], upto[CLUSTER * CHOOSE_WARPS + 1];  // a warp's weight, or a part's; the weight in front of each warp of the cluster
+    __shared__ double of_warp[2][CHOOSE_WARPS], upto[CLUSTER * CHOOSE_WARPS + 1];  // a warp's weight; the weight in front of each warp of the cluster
     __shared__ int last_some;    // the last warp that has any weight
     __shared__ double row_sum[CHOOSE_WARPS];  // of the last row that each warp has looked at, which one of them goes on with: p = exp((x - top) / temperature) / sum
     __shared__ float row_top[CHOOSE_WARPS];
@@ -248,7 +256,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
         int at = 0;
         double sum = 0.0;
         if constexpr (FORM != PROBABILITIES) {
-            join_chunks<FORM>(a, (int64_t)b * rows + i, lane, top, at, sum);
+            join_chunks<FORM>(a, exponential, (int64_t)b * rows + i, lane, top, at, sum);
             if (lane == 0) {
                 row_top[warp] = top;
                 row_at[warp] = at;
@@ -263,8 +271,11 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
         } else if constexpr (FORM == GREEDY) {
             good = x == at;
         } else {
-            const double t = to_float(target[i * a.tr + x]);
-            const double p = FORM == LOGITS ? exp((t - (double)top) * a.inverse) / sum : t;
+            const float t = to_float(target[i * a.tr + x]);
+            double p = (double)t;
+            if constexpr (FORM == LOGITS) {
+                p = exponential.of<true>(t, top) / sum;
+            }
             const double q = a.q != nullptr ? (double)a.q[b * a.qb + i * a.qr + x] : 1.0;
             good = (double)a.u[(int64_t)b * rows + i] * q < p;
         }
@@ -285,61 +296,84 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
         const int draft = j < count ? a.drafts[b * a.drafts_most + j] : -1;
         const float* const q = j < count && a.q != nullptr ? a.q + b * a.qb + j * a.qr : nullptr;
         bool less = j < count;  // whether the drafter's share is taken off
-        // the weights of N times 32 values from `at` on (none from `end` on), by a warp: a lane has the values lane, lane + 32 ...
-        auto weigh = [&](int at, int end, auto& w) {
-            constexpr int N = sizeof(w) / sizeof(w[0]);
-            float t[N], share[N];
-#pragma unroll
-            for (int i = 0; i < N; i++) {
-                const int v = at + 32 * i + lane;
-                t[i] = v < end ? to_float(x[v]) : (FORM == LOGITS ? -INFINITY : 0.0f);
-                share[i] = v < end && less && q != nullptr ? q[v] : 0.0f;
+        // the weight of one value a lane (at or behind `end`: none); by a whole warp
+        auto weight = [&](float t, float share, int v, int end) {
+            double p = (double)t;
+            if constexpr (FORM == LOGITS) {
+                p = exponential.of<true>(t, top) * scale;
             }
+            const double rest = less && q == nullptr && v == draft ? 0.0 : p - (double)share;
+            return v < end && rest > 0.0 ? rest : 0.0;  // (a NaN counts as nothing)
+        };
+        // A warp has a run of the vocabulary, a lane `each` neighbouring values of it, four of which are on their way ahead: the lane's sum is a place of the search too
+        const int each = (int)(((int64_t)a.vocab + blocks * CHOOSE_THREADS * 4 - 1) / (blocks * CHOOSE_THREADS * 4)) * 4;
+        auto begin_of = [&](int lane_of_all) { return (int)((int64_t)lane_of_all * each < a.vocab ? lane_of_all * each : a.vocab); };
+        const int me = rank * CHOOSE_WARPS + warp, from = begin_of(me * 32 + lane), to = begin_of(me * 32 + lane + 1);
+        const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0;
+        auto four = [&](int v, float (&t)[4], float (&share)[4]) {
 #pragma unroll
-            for (int i = 0; i < N; i++) {
-                double p;
-                if constexpr (FORM == LOGITS) {
-                    p = exponential.of<true>(t[i], top) * scale;
+            for (int n = 0; n < 4; n++) {
+                t[n] = share[n] = 0.0f;
+            }
+            if (wide && v + 4 <= to) {
+                if constexpr (sizeof(T) == 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(x + v);
+                    t[0] = f.x; t[1] = f.y; t[2] = f.z; t[3] = f.w;
                 } else {
-                    p = (double)t[i];
+                    const uint2 f = *reinterpret_cast<const uint2*>(x + v);
+                    const T* const e = reinterpret_cast<const T*>(&f);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        t[n] = to_float(e[n]);
+                    }
                 }
-                const double rest = less && q == nullptr && at + 32 * i + lane == draft ? 0.0 : p - (double)share[i];
-                w[i] = rest > 0.0 ? rest : 0.0;  // (a NaN counts as nothing)
+                if (less && q != nullptr) {
+                    const float4 f = *reinterpret_cast<const float4*>(q + v);
+                    share[0] = f.x; share[1] = f.y; share[2] = f.z; share[3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    if (v + n < to) {
+                        t[n] = to_float(x[v + n]);
+                        share[n] = less && q != nullptr ? q[v + n] : 0.0f;
+                    }
+                }
             }
         };
-        auto total_of = [&](int from, int to) {  // the weight of a run, by a warp
-            double sum = 0.0;
-#pragma unroll 1
-            for (int at = from; at < to; at += 8 * 32) {
-                double w[8];
-                weigh(at, to, w);
-                sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            }
-            return warp_total(sum);
-        };
-        // a warp's run of the vocabulary, and a sixteenth of it
-        const int part = (int)(((int64_t)a.vocab + blocks * CHOOSE_WARPS * CHOOSE_WARPS * 32 - 1) / (blocks * CHOOSE_WARPS * CHOOSE_WARPS * 32)) * 32, per = part * CHOOSE_WARPS;
-        auto begin_of = [&](int w) { return (int)((int64_t)w * per < a.vocab ? w * per : a.vocab); };
-        const int me = rank * CHOOSE_WARPS + warp;
-        double total = 0.0;
+        double total = 0.0, mine = 0.0;
 #pragma unroll 1
         for (int round = 0; round < 2; round++) {
-            const double sum = total_of(begin_of(me), begin_of(me + 1));
+            float t[4], share[4];
+            four(from, t, share);
+            mine = 0.0;
+#pragma unroll 1
+            for (int v = 0; v < each; v += 4) {
+                float t_next[4], share_next[4];
+                four(from + v + 4, t_next, share_next);
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    mine += weight(t[n], share[n], from + v + n, to);
+                    t[n] = t_next[n];
+                    share[n] = share_next[n];
+                }
+            }
+            const double sum = warp_total(mine);
             if (lane == 0) {
-                of_warp[warp] = sum;
+                of_warp[round][warp] = sum;
             }
             cluster.sync();
             // every thread block makes the same sums up to each warp of the cluster, whose intervals leave no gap
             if (warp == 0) {
                 constexpr int N = CLUSTER * CHOOSE_WARPS / 32;  // (of smaller clusters the last have nothing)
-                double each[N], run = 0.0;
+                double part[N], run = 0.0;
                 int last = -1;
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     const int w = lane * N + n;
-                    each[n] = w < blocks * CHOOSE_WARPS ? *cluster.map_shared_rank(&of_warp[w % CHOOSE_WARPS], w / CHOOSE_WARPS) : 0.0;
-                    run += each[n];
-                    last = each[n] > 0.0 ? w : last;
+                    part[n] = w < blocks * CHOOSE_WARPS ? *cluster.map_shared_rank(&of_warp[round][w % CHOOSE_WARPS], w / CHOOSE_WARPS) : 0.0;
+                    run += part[n];
+                    last = part[n] > 0.0 ? w : last;
                 }
                 const double scan = warp_scan(run, lane);
                 double here = __shfl_up_sync(0xffffffffu, scan, 1);
@@ -347,7 +381,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     upto[lane * N + n] = here;
-                    here += each[n];
+                    here += part[n];
                 }
                 last = __reduce_max_sync(0xffffffffu, last);
                 if (lane == 31) {
@@ -356,51 +390,42 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
                 }
             }
             __syncthreads();
-            cluster.sync();  // nobody's sums go away while others read them
             total = upto[CLUSTER * CHOOSE_WARPS];
             if (total != 0.0 || !less) {
                 break;
             }
+            __syncthreads();
             less = false;  // p nowhere above q: they are the same
         }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nobody's sums go away while others read them
+        // the warp whose run the aim falls into; with a uniform number of 1 or more, or none at all, the last that has any weight
         const double aim = (double)a.u[(int64_t)b * rows + a.drafts_most] * total;
-        // the warp of this thread block whose run the aim falls into; with a uniform number of 1 or more, or none at all, the last that has any weight
-        const int w = rank * CHOOSE_WARPS + (lane & (CHOOSE_WARPS - 1));
-        const unsigned hit = __ballot_sync(0xffffffffu, aim < total ? upto[w] <= aim && aim < upto[w + 1] : w == last_some);
-        if (hit != 0u) {
-            // all warps look at its run, a sixteenth each; then the one whose sixteenth it is looks it up
-            const int run = rank * CHOOSE_WARPS + __ffs(hit) - 1, end = begin_of(run + 1);
-            auto part_of = [&](int n) { return begin_of(run) + n * part < end ? begin_of(run) + n * part : end; };
-            const double sum = total_of(part_of(warp), part_of(warp + 1));
-            if (lane == 0) {
-                of_part[warp] = sum;
-            }
-            __syncthreads();
-            const double mine = lane < CHOOSE_WARPS ? of_part[lane] : 0.0, scan = warp_scan(mine, lane) + upto[run];
+        if (aim < total ? upto[me] <= aim && aim < upto[me + 1] : me == last_some) {
+            const double scan = warp_scan(mine, lane) + upto[me];
             const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && scan > aim), some = __ballot_sync(0xffffffffu, mine > 0.0);
-            const int chosen = over != 0u ? __ffs(over) - 1 : (some != 0u ? 31 - __clz(some) : 0);  // (not found by a rounding of the sums: the last with any weight)
-            const double ahead = __shfl_sync(0xffffffffu, scan - mine, chosen);
-            if (warp == chosen) {
-                double before_it = ahead;
-                int found = -1, positive = -1;
+            const int chosen = over != 0u ? __ffs(over) - 1 : 31 - __clz(some);  // (not found by a rounding of the sums: the last with any weight)
+            double before_it = __shfl_sync(0xffffffffu, scan - mine, chosen);
+            const int first = begin_of(me * 32 + chosen), end = begin_of(me * 32 + chosen + 1);
+            int found = -1, positive = -1;
 #pragma unroll 1
-                for (int at = part_of(chosen); at < part_of(chosen + 1) && found < 0; at += 32) {
-                    double v[1];
-                    weigh(at, part_of(chosen + 1), v);
-                    const double upto_here = warp_scan(v[0], lane);
-                    const unsigned is = __ballot_sync(0xffffffffu, v[0] > 0.0 && before_it + upto_here > aim), any = __ballot_sync(0xffffffffu, v[0] > 0.0);
-                    positive = any != 0u ? at + 31 - __clz(any) : positive;
-                    found = is != 0u ? at + __ffs(is) - 1 : -1;
-                    before_it += __shfl_sync(0xffffffffu, upto_here, 31);
-                }
-                if (lane == 0) {
-                    a.tokens[(int64_t)b * rows + j] = found >= 0 ? found : (positive >= 0 ? positive : a.vocab - 1);
-                }
+            for (int at = first; at < end && found < 0; at += 32) {
+                const int v = at + lane;
+                const double w = weight(v < end ? to_float(x[v]) : 0.0f, v < end && less && q != nullptr ? q[v] : 0.0f, v, end);
+                const double upto_here = warp_scan(w, lane);
+                const unsigned is = __ballot_sync(0xffffffffu, w > 0.0 && before_it + upto_here > aim), any = __ballot_sync(0xffffffffu, w > 0.0);
+                positive = any != 0u ? at + 31 - __clz(any) : positive;
+                found = is != 0u ? at + __ffs(is) - 1 : -1;
+                before_it += __shfl_sync(0xffffffffu, upto_here, 31);
+            }
+            if (lane == 0) {
+                a.tokens[(int64_t)b * rows + j] = found >= 0 ? found : (positive >= 0 ? positive : a.vocab - 1);
             }
         }
         if (rank == 0 && tid == 0 && last_some < 0) {
             a.tokens[(int64_t)b * rows + j] = a.vocab - 1;  // no weight anywhere
         }
+        __syncwarp();
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
     if (rank == 0) {
         for (int i = tid; i < rows; i += CHOOSE_THREADS) {
