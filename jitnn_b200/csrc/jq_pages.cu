@@ -2,7 +2,7 @@
 // in one launch. [page][key/value head][slot][element]: what the attention of one key/value head reads of a page is one contiguous run.
 #include <new>
 
-#include "jq_pages.cuh"
+#include "jq_rope.cuh"
 #include "jq_tc.cuh"
 
 namespace jq {
@@ -15,7 +15,7 @@ struct AppendArgs {
     int heads;
     void *k_pages, *v_pages;
     int64_t pages;
-    int page_size, kv_heads, head_dim;
+    int page_shift, kv_heads, head_dim;
     const float2* table;  // of the rotations, or null
     int half;
     int64_t positions;    // of that table
@@ -24,62 +24,54 @@ struct AppendArgs {
     int* status;
 };
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T e[V];
-};
-
+// A run rounded to the pages' type and stored.
 template <typename Out, typename In, int V>
-__device__ __forceinline__ void store_run(Out* to, const Vec<In, V>& from) {
-    Vec<Out, V> r;
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        if constexpr (sizeof(Out) == sizeof(In)) {
-            r.e[j] = from.e[j];
-        } else {
-            r.e[j] = from_float<Out>(to_float(from.e[j]));
+__device__ __forceinline__ void store_run(Out* to, const Run<In, V>& from) {
+    if constexpr (sizeof(Out) == sizeof(In)) {
+        from.store(reinterpret_cast<In*>(to));
+    } else {
+        float v[V];
+        from.numbers(v);
+        if constexpr (V == 1) {
+            *to = from_float<Out>(v[0]);
+        } else {  // four FP32 numbers, eight bytes
+            *reinterpret_cast<uint2*>(to) = make_uint2(Run<Out, 8>::packed(v[0], v[1]), Run<Out, 8>::packed(v[2], v[3]));
         }
     }
-    *reinterpret_cast<Vec<Out, V>*>(to) = r;
 }
 
 // As the rotation's kernel: a thread has up to ITEMS units of 2 V elements of the same place in different heads of a row (query heads, key heads, value heads). The values
-// are on their way while the row's sequence is looked for: thread i of the block asks whether the row is sequence i's, all at once, so that the chain of dependent loads
-// is sequence, page, store. Bound by memory: everything is read once and written once; with few rows by that chain.
+// are on their way while the row's sequence is looked for: every thread of the block asks whether the row is some sequence's, all at once, so that the chain of dependent
+// loads is sequence, page, store. Bound by memory: everything is read once and written once; with few rows by that chain.
 template <typename T, typename C, int V, bool INTERLEAVED, int ITEMS>
-__global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
+__global__ void __launch_bounds__(256, V == 1 ? 1 : 4) append_kernel(AppendArgs a) {
     __shared__ int found[2];  // sequence and own position
-    const int row = blockIdx.x;
-    if (threadIdx.x == 0) {
+    const int row = blockIdx.x, u = threadIdx.x, lanes = blockDim.y, tid = threadIdx.y * blockDim.x + u, threads = blockDim.x * lanes;
+    if (tid == 0) {
         found[0] = -1;
     }
-    const int units = a.head_dim / (2 * V), pair_units = a.table != nullptr ? a.half / V : 0;
-    const int u = threadIdx.x % units, lanes = blockDim.x / units, lane = threadIdx.x / units;
-    const int all = a.heads + 2 * a.kv_heads, h0 = blockIdx.y * lanes * ITEMS + lane;
-    int first, second, plain_first = 2 * V * u;  // a value head's unit is one run of 2 V elements
-    if (u < pair_units) {
-        first = INTERLEAVED ? 2 * V * u : V * u;
-        second = INTERLEAVED ? first + V : first + a.half;
-    } else {
-        first = plain_first;
-        second = first + V;
+    const int pair_units = a.table != nullptr ? a.half / V : 0;
+    const int all = a.heads + 2 * a.kv_heads, h0 = blockIdx.y * lanes * ITEMS + threadIdx.y;
+    const int plain = 2 * V * u;  // a value head's unit is one run of 2 V elements
+    int first = plain, second = plain + V;
+    if (u < pair_units && !INTERLEAVED) {
+        first = V * u;
+        second = first + a.half;
     }
-    using Run = Vec<T, V>;
-    Run p[ITEMS], r[ITEMS];
+    Run<T, V> p[ITEMS], r[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
         const int h = h0 + i * lanes;
         if (h < all) {
-            const T* x = h < a.heads ? static_cast<const T*>(a.q) + row * a.qt + h * a.qh
-                                     : (h < a.heads + a.kv_heads ? static_cast<const T*>(a.k) + row * a.kt + (h - a.heads) * a.kh
-                                                                 : static_cast<const T*>(a.v) + row * a.vt + (h - a.heads - a.kv_heads) * a.vh);
-            const bool value = h >= a.heads + a.kv_heads;
-            p[i] = *reinterpret_cast<const Run*>(x + (value ? plain_first : first));
-            r[i] = *reinterpret_cast<const Run*>(x + (value ? plain_first + V : second));
+            const bool value = h >= a.heads + a.kv_heads, query = h < a.heads;
+            const T* const x = static_cast<const T*>(query ? a.q : (value ? a.v : a.k)) + row * (query ? a.qt : (value ? a.vt : a.kt)) +
+                               (query ? h : h - a.heads - (value ? a.kv_heads : 0)) * (query ? a.qh : (value ? a.vh : a.kh));
+            p[i].load(x + (value ? plain : first));
+            r[i].load(x + (value ? plain + V : second));
         }
     }
     __syncthreads();
-    for (int s = threadIdx.x; s < a.b.sequences; s += blockDim.x) {
+    for (int s = tid; s < a.b.sequences; s += threads) {
         const int from = a.b.starts[s], to = a.b.starts[s + 1], length = a.b.lengths[s];
         if (row >= from && row < to) {
             found[0] = s;
@@ -89,75 +81,56 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
     __syncthreads();
     const int seq = found[0], at = found[1];
     const bool real = seq >= 0 && at >= 0;  // (a negative position: more rows than keys, for the padding of a sequence that is not there)
-    int64_t slot0 = -1;  // where the row's keys of head 0 go
     const int64_t pos = (int64_t)a.b.prefix_length + at;
-    if (real) {
-        const int64_t where = (int64_t)at / a.page_size;
+    const bool turned = u < pair_units && real;
+    Turns<V> turns;
+    bool placed = real;
+    if (turned) {
+        if (pos < a.positions) {
+            turns.load(a.table, pos, a.half, u * V, 1.0f);
+        } else {
+            turns.none();
+            note_status(a.status, STATUS_POSITION);
+        }
+    }
+    placed = placed && (a.table == nullptr || pos < a.positions);
+    int64_t slot0 = -1;  // where the row's keys of head 0 go
+    if (placed) {
+        const int where = at >> a.page_shift;
         const int64_t page = where < a.b.table_width ? a.b.tables[seq * a.b.table_stride + where] : -1;
         if (page < 0 || page >= a.pages) {
             note_status(a.status, STATUS_PAGE);
         } else {
-            slot0 = page * a.kv_heads * a.page_size + at % a.page_size;
-        }
-    }
-    if (u < pair_units && real) {
-        float2 cs[V];
-        if (pos < a.positions) {
-            const float2* f = a.table + pos * a.half + u * V;
-            if constexpr (V % 2 == 0) {
-#pragma unroll
-                for (int j = 0; j < V; j += 2) {
-                    const float4 w = *reinterpret_cast<const float4*>(f + j);
-                    cs[j] = make_float2(w.x, w.y);
-                    cs[j + 1] = make_float2(w.z, w.w);
-                }
-            } else {
-                cs[0] = f[0];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                cs[j] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-            }
-            slot0 = -1;
-            note_status(a.status, STATUS_POSITION);
-        }
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int h = h0 + i * lanes;
-            if (h < a.heads + a.kv_heads) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    T& ea = !INTERLEAVED || V == 1 ? p[i].e[j] : (j < V / 2 ? p[i].e[(2 * j) % V] : r[i].e[(2 * j) % V]);
-                    T& eb = !INTERLEAVED || V == 1 ? r[i].e[j] : (j < V / 2 ? p[i].e[(2 * j + 1) % V] : r[i].e[(2 * j + 1) % V]);
-                    const float f = to_float(ea), g = to_float(eb);
-                    ea = from_float<T>(f * cs[j].x - g * cs[j].y);
-                    eb = from_float<T>(f * cs[j].y + g * cs[j].x);
-                }
-            }
+            slot0 = ((page * a.kv_heads) << a.page_shift) + (at & ((1 << a.page_shift) - 1));
         }
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
         const int h = h0 + i * lanes;
+        if (h >= all) {
+            continue;
+        }
+        const bool value = h >= a.heads + a.kv_heads;
+        if (turned && !value) {
+            turns.template turn<INTERLEAVED>(p[i], r[i]);
+        }
         if (h < a.heads) {
             if (real || a.fill) {
-                T* y = static_cast<T*>(a.q_out) + row * a.ot + h * a.oh;
+                T* const y = static_cast<T*>(a.q_out) + row * a.ot + h * a.oh;
                 if (!real) {
 #pragma unroll
-                    for (int j = 0; j < V; j++) {
-                        p[i].e[j] = r[i].e[j] = from_float<T>(0.0f);
+                    for (int j = 0; j < Run<T, V>::WORDS; j++) {
+                        p[i].w[j] = r[i].w[j] = 0;
                     }
                 }
-                store_run<T, T, V>(y + first, p[i]);
-                store_run<T, T, V>(y + second, r[i]);
+                p[i].store(y + first);
+                r[i].store(y + second);
             }
-        } else if (h < all && slot0 >= 0) {
-            const bool value = h >= a.heads + a.kv_heads;
+        } else if (slot0 >= 0) {
             const int head = h - a.heads - (value ? a.kv_heads : 0);
-            C* y = static_cast<C*>(value ? a.v_pages : a.k_pages) + (slot0 + (int64_t)head * a.page_size) * a.head_dim;
-            store_run<C, T, V>(y + (value ? plain_first : first), p[i]);
-            store_run<C, T, V>(y + (value ? plain_first + V : second), r[i]);
+            C* const y = static_cast<C*>(value ? a.v_pages : a.k_pages) + (slot0 + ((int64_t)head << a.page_shift)) * a.head_dim;
+            store_run<C, T, V>(y + (value ? plain : first), p[i]);
+            store_run<C, T, V>(y + (value ? plain + V : second), r[i]);
         }
     }
 }
@@ -165,9 +138,8 @@ __global__ void __launch_bounds__(256) append_kernel(AppendArgs a) {
 template <typename T, typename C, int V, bool INTERLEAVED>
 void launch_append(const AppendArgs& a, cudaStream_t s) {
     constexpr int ITEMS = 4;
-    const int units = a.head_dim / (2 * V), heads = a.heads + 2 * a.kv_heads;
-    const int most = 256 / units * ITEMS, blocks = (heads + most - 1) / most, lanes = (heads + blocks * ITEMS - 1) / (blocks * ITEMS);
-    append_kernel<T, C, V, INTERLEAVED, ITEMS><<<dim3((unsigned)a.b.tokens, (unsigned)blocks), lanes * units, 0, s>>>(a);
+    const HeadGrid g(a.head_dim, V, a.heads + 2 * a.kv_heads, ITEMS);
+    append_kernel<T, C, V, INTERLEAVED, ITEMS><<<dim3((unsigned)a.b.tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), 0, s>>>(a);
 }
 
 template <typename T, typename C>
@@ -304,7 +276,7 @@ JQ_API int jq_pages_append(const jq_pages* p, const jq_rope* rope, int elem, int
     a.heads = heads;
     a.k_pages = p->k; a.v_pages = p->v;
     a.pages = p->pages;
-    a.page_size = p->page_size; a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
+    a.page_shift = 31 - __builtin_clz((unsigned)p->page_size); a.kv_heads = p->kv_heads; a.head_dim = p->head_dim;
     a.fill = fill != 0;
     const int width = 16 / elem_bytes(elem);
     bool wide = p->head_dim % (2 * width) == 0;

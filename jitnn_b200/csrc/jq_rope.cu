@@ -7,7 +7,7 @@
 #include <cmath>
 #include <new>
 
-#include "jq_pages.cuh"
+#include "jq_rope.cuh"
 
 namespace jq {
 namespace {
@@ -40,20 +40,14 @@ struct RopeArgs {
     int* status;
 };
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-    T e[V];
-};
-
 // A thread has up to ITEMS units of 2 V elements, of the same place in different heads of one token: their loads are on their way together, and one read of the table
 // serves them. Units of a head: the pairs (2 V elements each), then what is only copied. Bound by memory: x read once, y written once.
 template <typename T, int V, bool INTERLEAVED, int ITEMS>
-__global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
-    const int units = a.head_dim / (2 * V), pair_units = a.half / V;
-    const int u = threadIdx.x % units, lanes = blockDim.x / units, lane = threadIdx.x / units;
-    const int64_t token = blockIdx.x, b = token / a.seq, t = token % a.seq;
+__global__ void __launch_bounds__(256, V == 1 ? 1 : 4) rope_kernel(RopeArgs a) {
+    const int pair_units = a.half / V, u = threadIdx.x, lanes = blockDim.y;
+    const uint32_t token = blockIdx.x, b = token / (uint32_t)a.seq, t = token - b * (uint32_t)a.seq;
     const int heads = a.t[0].heads + a.t[1].heads;
-    const int h0 = blockIdx.y * lanes * ITEMS + lane;
+    const int h0 = blockIdx.y * lanes * ITEMS + threadIdx.y;
     int first, second;  // where the unit's two runs of V elements start
     if (u < pair_units) {
         first = INTERLEAVED ? 2 * V * u : V * u;
@@ -62,8 +56,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
         first = 2 * V * u;
         second = first + V;
     }
-    using Run = Vec<T, V>;
-    Run p[ITEMS], q[ITEMS];
+    Run<T, V> p[ITEMS], q[ITEMS];
     T* y[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
@@ -71,15 +64,15 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
         y[i] = nullptr;
         if (h < heads) {
             const RopeTensor& w = h < a.t[0].heads ? a.t[0] : a.t[1];
-            const int64_t head = h < a.t[0].heads ? h : h - a.t[0].heads;
-            const T* x = static_cast<const T*>(w.x) + b * w.xb + t * w.xt + head * w.xh;
+            const int head = h < a.t[0].heads ? h : h - a.t[0].heads;
+            const T* const x = static_cast<const T*>(w.x) + b * w.xb + t * w.xt + head * w.xh;
             T* const to = static_cast<T*>(w.y) + b * w.yb + t * w.yt + head * w.yh;
             if (u >= pair_units && to == x) {
                 continue;  // in place
             }
             y[i] = to;
-            p[i] = *reinterpret_cast<const Run*>(x + first);
-            q[i] = *reinterpret_cast<const Run*>(x + second);
+            p[i].load(x + first);
+            q[i].load(x + second);
         }
     }
     if (u < pair_units) {
@@ -89,46 +82,25 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
         } else if (a.pos_bytes == 8) {
             pos = static_cast<const int64_t*>(a.pos)[b * a.pos_b + t * a.pos_t];
         }
-        float2 cs[V];
+        Turns<V> turns;
         if (pos >= 0 && pos < a.positions) {
-            const float2* row = a.table + pos * a.half + u * V;
-            if constexpr (V % 2 == 0) {
-#pragma unroll
-                for (int j = 0; j < V; j += 2) {
-                    const float4 f = *reinterpret_cast<const float4*>(row + j);
-                    cs[j] = make_float2(f.x, f.y * a.sign);
-                    cs[j + 1] = make_float2(f.z, f.w * a.sign);
-                }
-            } else {
-                cs[0] = make_float2(row[0].x, row[0].y * a.sign);
-            }
+            turns.load(a.table, pos, a.half, u * V, a.sign);
         } else {  // no such position: NaN, so that it does not pass for a result
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                cs[j] = make_float2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
-            }
+            turns.none();
             note_status(a.status, STATUS_POSITION);
         }
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             if (y[i] != nullptr) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    // pair j: (p[j], q[j]); interleaved, the pairs stand one after the other in p, then in q
-                    T& ea = !INTERLEAVED || V == 1 ? p[i].e[j] : (j < V / 2 ? p[i].e[(2 * j) % V] : q[i].e[(2 * j) % V]);
-                    T& eb = !INTERLEAVED || V == 1 ? q[i].e[j] : (j < V / 2 ? p[i].e[(2 * j + 1) % V] : q[i].e[(2 * j + 1) % V]);
-                    const float f = to_float(ea), g = to_float(eb);
-                    ea = from_float<T>(f * cs[j].x - g * cs[j].y);
-                    eb = from_float<T>(f * cs[j].y + g * cs[j].x);
-                }
+                turns.template turn<INTERLEAVED>(p[i], q[i]);
             }
         }
     }
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
         if (y[i] != nullptr) {
-            *reinterpret_cast<Run*>(y[i] + first) = p[i];
-            *reinterpret_cast<Run*>(y[i] + second) = q[i];
+            p[i].store(y[i] + first);
+            q[i].store(y[i] + second);
         }
     }
 }
@@ -136,10 +108,8 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
 template <typename T, int V, bool INTERLEAVED>
 void launch_rope(const RopeArgs& a, int64_t tokens, cudaStream_t s) {
     constexpr int ITEMS = 4;
-    const int units = a.head_dim / (2 * V), heads = a.t[0].heads + a.t[1].heads;
-    const int most = 256 / units * ITEMS, blocks = (heads + most - 1) / most;             // heads of a thread block, thread blocks of a token
-    const int lanes = (heads + blocks * ITEMS - 1) / (blocks * ITEMS);                    // heads that a thread block has beside one another
-    rope_kernel<T, V, INTERLEAVED, ITEMS><<<dim3((unsigned)tokens, (unsigned)blocks), lanes * units, 0, s>>>(a);
+    const HeadGrid g(a.head_dim, V, a.t[0].heads + a.t[1].heads, ITEMS);
+    rope_kernel<T, V, INTERLEAVED, ITEMS><<<dim3((unsigned)tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), 0, s>>>(a);
 }
 
 template <typename T>
