@@ -317,6 +317,29 @@ JQ_API int jq_decoder_prompt(jq_decoder* d, int seq, const int32_t* tokens_host,
                              void* stream);
 
 /*
+ * The decoder on paged caches: the operators of paged decoding below, in its layers. Not for the row-sharded decoder (JQ_ERR_UNSUPPORTED).
+ *
+ * jq_decoder_set_rope       the rotation by freqs[head_dim / 2] radians per position, times `magnitude` (jq_rope_frequencies), in place of rope_base's, on all of the decoder's
+ *                           paths. Cached keys were rotated by the old ones.
+ * jq_decoder_set_pages      `pages` pages of page_size keys for every layer, keys and values of type `elem` (JQ_ELEM_*); what they held is lost, 0 pages releases them.
+ * jq_decoder_forward_pages  counts[s] new tokens of each of n_seqs sequences (up to 16 in all, tokens_host one sequence after the other) in one pass over the weights. Sequence s has
+ *                           lengths[s] keys of its own once they are appended, key i on page tables[s * table_width + i / page_size] of every layer; in front of
+ *                           them all sequences see the prefix_length keys on the pages prefix[0 ..]. A token's position is prefix_length plus its place among its
+ *                           sequence's keys, below max_seq. logits_host [tokens, vocab] and next_host [tokens] as for jq_decoder_forward.
+ * jq_decoder_verify_pages   speculative decoding: every sequence's tokens are its last one and then `drafts` drafted ones (tokens_host [n_seqs, drafts + 1], appended as by
+ *                           jq_decoder_forward_pages), which jq_verify_drafts verifies against the logits at `temperature`; the logits stay on the GPU. draft_probs
+ *                           [n_seqs, drafts, vocab] (or NULL) and uniforms [n_seqs, drafts + 1] are host arrays. accepted_host [n_seqs], next_host [n_seqs, drafts + 1]:
+ *                           the drafts kept, the token behind them, -1 in the rest. Keys of refused drafts are behind the sequence's end: the next call's lengths say so.
+ */
+JQ_API int jq_decoder_set_rope(jq_decoder* d, const double* freqs, double magnitude);
+JQ_API int jq_decoder_set_pages(jq_decoder* d, int elem, int pages, int page_size);
+JQ_API int jq_decoder_forward_pages(jq_decoder* d, const int32_t* tokens_host, const int32_t* counts, int n_seqs, const int32_t* tables, int table_width, const int32_t* lengths,
+                                    const int32_t* prefix, int prefix_pages, int prefix_length, float* logits_host, int32_t* next_host, void* stream);
+JQ_API int jq_decoder_verify_pages(jq_decoder* d, const int32_t* tokens_host, int n_seqs, int drafts, const int32_t* tables, int table_width, const int32_t* lengths,
+                                   const int32_t* prefix, int prefix_pages, int prefix_length, const float* draft_probs, const float* uniforms, double temperature,
+                                   int32_t* accepted_host, int32_t* next_host, void* stream);
+
+/*
  * GGUF file -> device weights (the reference's jitnn-gguf/.../GgufFile.java:100-175,329-418, whose GgufFile.tensor(name)
  * hands a tensor's block bytes to Tensor.persistent): the file is mapped read-only, header, metadata and tensor table are
  * parsed with every access bounds-checked, and a tensor's blocks go to the GPU straight from the mapping. GGUF versions 2

@@ -71,6 +71,10 @@ SIGNATURES = {
     "jq_gguf_meta_number": (c_int, [vp, ctypes.c_char_p, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(c_i64)]),
     "jq_gguf_meta_string": (c_int, [vp, ctypes.c_char_p, ctypes.POINTER(vp), ctypes.POINTER(c_i64)]),
     "jq_gguf_upload": (c_int, [vp, c_i64, c_int, c_i64, c_i64, ctypes.POINTER(vp)]),
+    "jq_decoder_set_rope": (c_int, [vp, vp, c_double]),
+    "jq_decoder_set_pages": (c_int, [vp, c_int, c_int, c_int]),
+    "jq_decoder_forward_pages": (c_int, [vp, vp, vp, c_int, vp, c_int, vp, vp, c_int, c_int, vp, vp, vp]),
+    "jq_decoder_verify_pages": (c_int, [vp, vp, c_int, c_int, vp, c_int, vp, vp, c_int, c_int, vp, vp, c_double, vp, vp, vp]),
     "jq_rope_frequencies": (c_int, [c_int, c_double, c_int, vp, vp, ctypes.POINTER(c_double)]),
     "jq_rope_create": (c_int, [c_int, c_i64, c_int, vp, c_double, c_int, ctypes.POINTER(vp)]),
     "jq_rope_free": (c_int, [vp]),

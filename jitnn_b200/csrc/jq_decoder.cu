@@ -1188,6 +1188,7 @@ int decoder_peer_status(int* status) {
 
 #define JQ_DECODER_MAGIC 0x4a514443u
 constexpr int GRAPHS = 6;  // 256 << 5 = 8192 positions
+constexpr int VERIFY_SLOT = 96;  // of the stream's scratch buffers: the verification's
 
 struct jq_decoder {
     uint32_t magic;
@@ -1231,6 +1232,17 @@ struct jq_decoder {
     uint16_t* prompt_bf16;
     int* prompt_tokens;
     int prompt_rows;
+    // Paged caches (jq_decoder_set_pages): each layer's pages, the rotations' table, and where a call's tables of pages lie on the device.
+    std::vector<jq_pages*> paged;
+    void *paged_k, *paged_v;
+    jq_rope* rope;
+    std::vector<double> rope_freqs;
+    double rope_magnitude;
+    int page_size, page_count;
+    int* paged_meta;      // starts [MAX_TOKENS + 1], lengths [MAX_TOKENS], tables [MAX_TOKENS][width], prefix [width]
+    uint8_t* paged_space; // the attention's workspace
+    int64_t paged_space_bytes;
+    int paged_sequences, paged_width, paged_prefix_pages, paged_prefix;  // of the call being enqueued; sequences 0: none of this kind
 };
 
 using namespace jq;
@@ -1249,6 +1261,40 @@ static int check_decoder(const jq_decoder* d, const char* who) {
         return fail(JQ_ERR_INVALID, "%s: not a live decoder handle", who);
     }
     return JQ_OK;
+}
+
+static void free_pages(jq_decoder* d) {
+    for (jq_pages* p : d->paged) {
+        jq_pages_free(p);
+    }
+    d->paged.clear();
+    jq_rope_free(d->rope);
+    cudaFree(d->paged_k);
+    cudaFree(d->paged_v);
+    cudaFree(d->paged_meta);
+    cudaFree(d->paged_space);
+    d->rope = nullptr;
+    d->paged_k = d->paged_v = nullptr;
+    d->paged_meta = nullptr;
+    d->paged_space = nullptr;
+    d->paged_space_bytes = 0;
+    d->page_count = 0;
+}
+
+// cos / sin tables in double, stored as float (ops/Rope.java:84-101)
+static cudaError_t fill_rope_tables(jq_decoder* d) {
+    const int half = d->head_dim / 2;
+    std::vector<float> c((size_t)d->max_seq * half), s((size_t)d->max_seq * half);
+    for (int t = 0; t < d->max_seq; t++) {
+        for (int i = 0; i < half; i++) {
+            const double angle = t * d->rope_freqs[i];
+            c[(size_t)t * half + i] = (float)(std::cos(angle) * d->rope_magnitude);
+            s[(size_t)t * half + i] = (float)(std::sin(angle) * d->rope_magnitude);
+        }
+    }
+    cudaError_t e = cudaMemcpy(d->cos_t, c.data(), c.size() * sizeof(float), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaMemcpy(d->sin_t, s.data(), s.size() * sizeof(float), cudaMemcpyHostToDevice);
+    return e;
 }
 
 extern "C" {
@@ -1285,6 +1331,7 @@ JQ_API int jq_decoder_destroy(jq_decoder* d) {
     drop_graphs(d);
     if (d->own_stream != nullptr) {
         cudaStreamSynchronize(d->own_stream);
+        free_pages(d);
         scratch_release(d->own_stream);
         cudaStreamDestroy(d->own_stream);
     }
@@ -1342,6 +1389,13 @@ JQ_API int jq_decoder_create(int device, int layers, int dim, int heads, int kv_
     d->prompt_bf16 = nullptr;
     d->prompt_tokens = nullptr;
     d->prompt_rows = 0;
+    d->paged_k = d->paged_v = nullptr;
+    d->rope = nullptr;
+    d->page_size = d->page_count = 0;
+    d->paged_meta = nullptr;
+    d->paged_space = nullptr;
+    d->paged_space_bytes = 0;
+    d->paged_sequences = 0;
     d->world = 1;
     d->rank = 0;
     for (int r = 0; r < 8; r++) {
@@ -1407,18 +1461,11 @@ JQ_API int jq_decoder_create(int device, int layers, int dim, int heads, int kv_
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&d->own_stream, cudaStreamNonBlocking);
     if (e == cudaSuccess && take_status_word(&d->status) != JQ_OK) e = cudaErrorMemoryAllocation;
     if (e == cudaSuccess) {
-        // cos / sin tables in double, stored as float (ops/Rope.java:84-101)
-        const int half = head_dim / 2;
-        std::vector<float> c((size_t)max_seq * half), s((size_t)max_seq * half);
-        for (int t = 0; t < max_seq; t++) {
-            for (int i = 0; i < half; i++) {
-                const double freq = std::pow((double)rope_base, -2.0 * i / head_dim);
-                c[(size_t)t * half + i] = (float)std::cos(t * freq);
-                s[(size_t)t * half + i] = (float)std::sin(t * freq);
-            }
+        for (int i = 0; i < head_dim / 2; i++) {
+            d->rope_freqs.push_back(std::pow((double)rope_base, -2.0 * i / head_dim));
         }
-        e = cudaMemcpy(d->cos_t, c.data(), c.size() * sizeof(float), cudaMemcpyHostToDevice);
-        if (e == cudaSuccess) e = cudaMemcpy(d->sin_t, s.data(), s.size() * sizeof(float), cudaMemcpyHostToDevice);
+        d->rope_magnitude = 1.0;
+        e = fill_rope_tables(d);
     }
     if (prev >= 0) {
         cudaSetDevice(prev);
@@ -1774,7 +1821,7 @@ static int enqueue_forward(jq_decoder* d, int T, int max_keys, const TokenArgs* 
     if (d->world > 1) {
         return enqueue_forward_sharded(d, T, max_keys, ta, s);
     }
-    if (T == 1 && fused_step_possible(d)) {
+    if (T == 1 && d->paged_sequences == 0 && fused_step_possible(d)) {
         return enqueue_forward_fused(d, max_keys, ta, s);
     }
     const int dim = d->dim, hd = d->head_dim;
@@ -1860,10 +1907,21 @@ static int enqueue_forward(jq_decoder* d, int T, int max_keys, const TokenArgs* 
         float* const qkv[3] = {d->q, d->k, d->v};
         NORMED(l == 0 ? nullptr : d->proj, d->norms + (size_t)(2 * l) * dim, L, 3, qkv);
         if (rc != JQ_OK) break;
+        if (d->paged_sequences > 0) {
+            const int64_t rows[8] = {dim, hd, kv_dim, hd, kv_dim, hd, dim, hd}, back[4] = {dim, hd, dim, hd};
+            const int *starts = d->paged_meta, *lengths = starts + MAX_TOKENS + 1, *tables = lengths + MAX_TOKENS, *prefix = tables + (size_t)d->paged_sequences * d->paged_width;
+            rc = jq_pages_append(d->paged[l], d->rope, JQ_ELEM_F32, d->heads, d->q, d->k, d->v, d->q, rows, T, tables, d->paged_width, d->paged_width, starts, lengths,
+                                 d->paged_sequences, d->paged_prefix, 0, s);
+            if (rc == JQ_OK) {
+                rc = jq_pages_attention(d->paged[l], JQ_ELEM_F32, d->heads, d->q, d->att, back, T, tables, d->paged_width, d->paged_width, starts, lengths, d->paged_sequences, prefix,
+                                        d->paged_prefix_pages, d->paged_prefix, scale, 0, d->paged_space, d->paged_space_bytes, s);
+            }
+            LIN(L[3], d->att, d->proj);
+        }
         // only the key chunks that can hold a position of this call are launched (all of them inside the captured graph)
         const int splits_now = (max_keys + ATT_CHUNK - 1) / ATT_CHUNK;
-        CKL(launch_attention(d, d->heads, d->kv_heads, T, splits_now, kc, vc, scale, pos_step, tok_stride, true, s), "attention_group_kernel");
-        {
+        if (d->paged_sequences == 0) {
+            CKL(launch_attention(d, d->heads, d->kv_heads, T, splits_now, kc, vc, scale, pos_step, tok_stride, true, s), "attention_group_kernel");
             uint8_t* image = nullptr;
             float* scales = nullptr;
             if (rc == JQ_OK && dim % 256 == 0 && hd >= 32 && 256 % hd == 0 && linears_take_rows(L + 3, 1, T)) {
@@ -2484,6 +2542,278 @@ JQ_API int jq_decoder_set_sequences(jq_decoder* d, int sequences) {
     d->sequences = sequences;
     if (prev >= 0) cudaSetDevice(prev);
     return JQ_OK;
+}
+
+// Other frequencies of the rotation than the base's, in both kinds of caches; what those hold was rotated by the old ones.
+JQ_API int jq_decoder_set_rope(jq_decoder* d, const double* freqs, double magnitude) {
+    int rc = check_decoder(d, "jq_decoder_set_rope");
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (freqs == nullptr || !std::isfinite(magnitude)) {
+        return fail(JQ_ERR_INVALID, "jq_decoder_set_rope: null frequencies, or magnitude %g", magnitude);
+    }
+    const DeviceGuard guard(d->device);
+    if (!guard.ok) {
+        return fail(JQ_ERR_CUDA, "jq_decoder_set_rope: device %d", d->device);
+    }
+    JQ_CUDA(cudaDeviceSynchronize());  // (steps that read the tables)
+    jq_rope* rope = nullptr;
+    if (d->rope != nullptr) {
+        rc = jq_rope_create(d->device, d->max_seq, d->head_dim, freqs, magnitude, 0, &rope);
+        if (rc != JQ_OK) {
+            return rc;
+        }
+        jq_rope_free(d->rope);
+        d->rope = rope;
+    }
+    d->rope_freqs.assign(freqs, freqs + d->head_dim / 2);
+    d->rope_magnitude = magnitude;
+    const cudaError_t e = fill_rope_tables(d);
+    return e == cudaSuccess ? JQ_OK : cuda_fail(e, "jq_decoder_set_rope");
+}
+
+JQ_API int jq_decoder_set_pages(jq_decoder* d, int elem, int pages, int page_size) {
+    int rc = check_decoder(d, "jq_decoder_set_pages");
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (d->world > 1) {
+        return fail(JQ_ERR_UNSUPPORTED, "jq_decoder_set_pages: not for the row-sharded decoder");
+    }
+    if (elem < JQ_ELEM_F32 || elem > JQ_ELEM_BF16 || pages < 0 || (pages > 0 && (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0))) {
+        return fail(JQ_ERR_INVALID, "jq_decoder_set_pages: %d pages of %d keys (a power of two from 16 to 1024), element type %d", pages, page_size, elem);
+    }
+    const DeviceGuard guard(d->device);
+    if (!guard.ok) {
+        return fail(JQ_ERR_CUDA, "jq_decoder_set_pages: device %d", d->device);
+    }
+    JQ_CUDA(cudaDeviceSynchronize());
+    free_pages(d);
+    if (pages == 0) {
+        return JQ_OK;
+    }
+    const size_t layer_bytes = (size_t)pages * page_size * d->kv_heads * d->head_dim * (elem == JQ_ELEM_F32 ? 4 : 2);
+    const int width = (d->max_seq + page_size - 1) / page_size;
+    cudaError_t e = cudaMalloc(&d->paged_k, layer_bytes * d->layers);
+    if (e == cudaSuccess) e = cudaMalloc(&d->paged_v, layer_bytes * d->layers);
+    if (e == cudaSuccess) e = cudaMalloc(&d->paged_meta, ((size_t)2 * MAX_TOKENS + 1 + (size_t)(MAX_TOKENS + 1) * width) * sizeof(int));
+    if (e != cudaSuccess) {
+        free_pages(d);
+        return cuda_fail(e, "jq_decoder_set_pages");
+    }
+    try {
+        d->paged.reserve(d->layers);
+    } catch (const std::bad_alloc&) {
+        free_pages(d);
+        return fail(JQ_ERR_OOM, "jq_decoder_set_pages: out of host memory");
+    }
+    rc = jq_rope_create(d->device, d->max_seq, d->head_dim, d->rope_freqs.data(), d->rope_magnitude, 0, &d->rope);
+    for (int l = 0; l < d->layers && rc == JQ_OK; l++) {
+        jq_pages* p = nullptr;
+        rc = jq_pages_create(d->device, elem, pages, page_size, d->kv_heads, d->head_dim, (uint8_t*)d->paged_k + l * layer_bytes, (uint8_t*)d->paged_v + l * layer_bytes, &p);
+        if (rc == JQ_OK) {
+            d->paged.push_back(p);
+        }
+    }
+    // the attention's workspace: for every number of rows and sequences that a call may have
+    for (int n = 1; n <= MAX_TOKENS && rc == JQ_OK; n++) {
+        for (int tokens = n; tokens <= MAX_TOKENS && rc == JQ_OK; tokens++) {
+            int64_t need = 0;
+            rc = jq_pages_attention_bytes(d->paged[0], JQ_ELEM_F32, d->heads, tokens, n, d->max_seq, &need);
+            d->paged_space_bytes = need > d->paged_space_bytes ? need : d->paged_space_bytes;
+        }
+    }
+    if (rc == JQ_OK && d->paged_space_bytes > 0) {
+        e = cudaMalloc(&d->paged_space, d->paged_space_bytes);
+        rc = e == cudaSuccess ? JQ_OK : cuda_fail(e, "jq_decoder_set_pages");
+    }
+    if (rc != JQ_OK) {
+        free_pages(d);
+        return rc;
+    }
+    d->page_size = page_size;
+    d->page_count = pages;
+    return JQ_OK;
+}
+
+static int forward_pages(jq_decoder* d, const char* who, const int32_t* tokens_host, const int32_t* counts, int n_seqs, const int32_t* tables, int table_width,
+                         const int32_t* lengths, const int32_t* prefix, int prefix_pages, int prefix_length, cudaStream_t s, int* n_tokens) {
+    int rc = check_decoder(d, who);
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (d->paged.empty()) {
+        return fail(JQ_ERR_INVALID, "%s: the decoder has no pages (jq_decoder_set_pages)", who);
+    }
+    if (tokens_host == nullptr || counts == nullptr || tables == nullptr || lengths == nullptr || n_seqs < 1 || n_seqs > MAX_TOKENS || table_width < 1) {
+        return fail(JQ_ERR_INVALID, "%s: %d sequences (1 to %d), tables of %d pages", who, n_seqs, MAX_TOKENS, table_width);
+    }
+    const int width_most = (d->max_seq + d->page_size - 1) / d->page_size;
+    const int ahead = prefix_length <= 0 ? 0 : (int)(((int64_t)prefix_length + d->page_size - 1) / d->page_size);
+    if (prefix_length < 0 || prefix_length > d->max_seq || ahead > prefix_pages || (ahead > 0 && prefix == nullptr)) {
+        return fail(JQ_ERR_INVALID, "%s: a prefix of %d keys on %d pages of %d (%d positions)", who, prefix_length, prefix_pages, d->page_size, d->max_seq);
+    }
+    int total = 0, width = 1;
+    for (int i = 0; i < n_seqs; i++) {
+        if (counts[i] < 0 || counts[i] > MAX_TOKENS || lengths[i] < counts[i] || lengths[i] > d->max_seq - prefix_length) {
+            return fail(JQ_ERR_INVALID, "%s: sequence %d: %d new tokens, %d keys behind a prefix of %d (%d positions)", who, i, counts[i], lengths[i], prefix_length, d->max_seq);
+        }
+        const int need = (lengths[i] + d->page_size - 1) / d->page_size;
+        if (need > table_width) {
+            return fail(JQ_ERR_INVALID, "%s: sequence %d: %d keys on %d pages of %d", who, i, lengths[i], table_width, d->page_size);
+        }
+        total += counts[i];
+        width = need > width ? need : width;
+    }
+    if (total < 1 || total > MAX_TOKENS) {
+        return fail(JQ_ERR_INVALID, "%s: %d tokens (1 to %d)", who, total, MAX_TOKENS);
+    }
+    width = width < width_most ? width : width_most;
+    std::vector<int32_t> meta;
+    try {
+        meta.assign((size_t)2 * MAX_TOKENS + 1 + (size_t)n_seqs * width + ahead, 0);
+    } catch (const std::bad_alloc&) {
+        return fail(JQ_ERR_OOM, "%s: out of host memory", who);
+    }
+    int32_t *starts = meta.data(), *lens = starts + MAX_TOKENS + 1, *tabs = lens + MAX_TOKENS, *pre = tabs + (size_t)n_seqs * width;
+    auto page_ok = [&](int page) { return page >= 0 && page < d->page_count; };
+    for (int i = 0; i < n_seqs; i++) {
+        starts[i + 1] = starts[i] + counts[i];
+        lens[i] = lengths[i];
+        for (int j = 0; j < (lengths[i] + d->page_size - 1) / d->page_size; j++) {
+            tabs[(size_t)i * width + j] = tables[(size_t)i * table_width + j];
+            if (!page_ok(tabs[(size_t)i * width + j])) {
+                return fail(JQ_ERR_INVALID, "%s: sequence %d has page %d of %d", who, i, tabs[(size_t)i * width + j], d->page_count);
+            }
+        }
+    }
+    for (int j = 0; j < ahead; j++) {
+        pre[j] = prefix[j];
+        if (!page_ok(pre[j])) {
+            return fail(JQ_ERR_INVALID, "%s: the prefix has page %d of %d", who, pre[j], d->page_count);
+        }
+    }
+    if (d->output == nullptr) {
+        return fail(JQ_ERR_INVALID, "%s: the output projection is not set", who);
+    }
+    for (size_t i = 0; i < d->lin.size(); i++) {
+        if (d->lin[i] == nullptr) {
+            return fail(JQ_ERR_INVALID, "%s: layer %d linear %d is not set", who, (int)(i / 7), (int)(i % 7));
+        }
+    }
+    // (out of pageable memory: staged before the call returns)
+    JQ_CUDA(cudaMemcpyAsync(d->paged_meta, meta.data(), meta.size() * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+    TokenArgs ta;
+    for (int i = 0; i < MAX_TOKENS; i++) {
+        ta.tokens[i] = i < total ? tokens_host[i] : 0;
+    }
+    ta.pos0 = 0;
+    d->cur_seq = 0;
+    d->cur_batch = false;
+    d->paged_sequences = n_seqs;
+    d->paged_width = width;
+    d->paged_prefix_pages = ahead;
+    d->paged_prefix = prefix_length;
+    rc = enqueue_forward(d, total, 1, &ta, s);
+    d->paged_sequences = 0;
+    *n_tokens = total;
+    return rc;
+}
+
+JQ_API int jq_decoder_forward_pages(jq_decoder* d, const int32_t* tokens_host, const int32_t* counts, int n_seqs, const int32_t* tables, int table_width, const int32_t* lengths,
+                                    const int32_t* prefix, int prefix_pages, int prefix_length, float* logits_host, int32_t* next_host, void* stream) {
+    int rc = check_decoder(d, "jq_decoder_forward_pages");
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    const DeviceGuard guard(d->device);
+    if (!guard.ok) {
+        return fail(JQ_ERR_CUDA, "jq_decoder_forward_pages: device %d", d->device);
+    }
+    const StatusScope scope(d->status);
+    const cudaStream_t s = stream != nullptr ? (cudaStream_t)stream : d->own_stream;
+    int T = 0;
+    rc = forward_pages(d, "jq_decoder_forward_pages", tokens_host, counts, n_seqs, tables, table_width, lengths, prefix, prefix_pages, prefix_length, s, &T);
+    if (rc != JQ_OK || (logits_host == nullptr && next_host == nullptr)) {
+        return rc;
+    }
+    if (logits_host != nullptr) {
+        JQ_CUDA(cudaMemcpyAsync(logits_host, d->logits, (size_t)T * d->vocab * sizeof(float), cudaMemcpyDeviceToHost, s));
+    }
+    if (next_host != nullptr) {
+        JQ_CUDA(cudaMemcpyAsync(d->host_stage + MAX_TOKENS + 1, d->argmax, T * sizeof(int), cudaMemcpyDeviceToHost, s));
+    }
+    JQ_CUDA(cudaStreamSynchronize(s));
+    rc = decoder_status(d, "jq_decoder_forward_pages");
+    for (int i = 0; i < T && rc == JQ_OK && next_host != nullptr; i++) {
+        next_host[i] = d->host_stage[MAX_TOKENS + 1 + i];
+    }
+    return rc;
+}
+
+JQ_API int jq_decoder_verify_pages(jq_decoder* d, const int32_t* tokens_host, int n_seqs, int drafts, const int32_t* tables, int table_width, const int32_t* lengths,
+                                   const int32_t* prefix, int prefix_pages, int prefix_length, const float* draft_probs, const float* uniforms, double temperature,
+                                   int32_t* accepted_host, int32_t* next_host, void* stream) {
+    int rc = check_decoder(d, "jq_decoder_verify_pages");
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (drafts < 0 || n_seqs < 1 || drafts >= MAX_TOKENS || n_seqs > MAX_TOKENS || n_seqs * (drafts + 1) > MAX_TOKENS || accepted_host == nullptr || next_host == nullptr ||
+        tokens_host == nullptr || !(temperature >= 0.0) || !std::isfinite(temperature) || (temperature > 0.0 && uniforms == nullptr)) {
+        return fail(JQ_ERR_INVALID, "jq_decoder_verify_pages: %d sequences with %d drafts (at most %d tokens in all), temperature %g", n_seqs, drafts, MAX_TOKENS, temperature);
+    }
+    const DeviceGuard guard(d->device);
+    if (!guard.ok) {
+        return fail(JQ_ERR_CUDA, "jq_decoder_verify_pages: device %d", d->device);
+    }
+    const StatusScope scope(d->status);
+    const cudaStream_t s = stream != nullptr ? (cudaStream_t)stream : d->own_stream;
+    const int rows = drafts + 1, total = n_seqs * rows;
+    int32_t counts[MAX_TOKENS], drafted[MAX_TOKENS];
+    for (int i = 0; i < n_seqs; i++) {
+        counts[i] = rows;
+        for (int j = 0; j < drafts; j++) {
+            drafted[i * drafts + j] = tokens_host[i * rows + j + 1];
+        }
+    }
+    int T = 0;
+    rc = forward_pages(d, "jq_decoder_verify_pages", tokens_host, counts, n_seqs, tables, table_width, lengths, prefix, prefix_pages, prefix_length, s, &T);
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    // small numbers, then the drafters' probabilities, then what the verification works in
+    int64_t need = 0;
+    rc = jq_verify_bytes(n_seqs, drafts, d->vocab, 1, &need);
+    const size_t q_bytes = draft_probs != nullptr && temperature > 0.0 ? (size_t)n_seqs * drafts * d->vocab * sizeof(float) : 0, small = 4 * 256;
+    uint8_t* space = nullptr;
+    if (rc == JQ_OK) {
+        rc = scratch_for_slot(s, VERIFY_SLOT, small + (q_bytes + 255) / 256 * 256 + (size_t)need, &space);
+    }
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    int32_t *const x = reinterpret_cast<int32_t*>(space), *const accepted = reinterpret_cast<int32_t*>(space + 512), *const next = reinterpret_cast<int32_t*>(space + 768);
+    float *const u = reinterpret_cast<float*>(space + 256), *const q = q_bytes > 0 ? reinterpret_cast<float*>(space + small) : nullptr;
+    cudaError_t e = cudaSuccess;
+    if (drafts > 0) e = cudaMemcpyAsync(x, drafted, (size_t)n_seqs * drafts * sizeof(int32_t), cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess && uniforms != nullptr) e = cudaMemcpyAsync(u, uniforms, (size_t)total * sizeof(float), cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess && q != nullptr) e = cudaMemcpyAsync(q, draft_probs, q_bytes, cudaMemcpyHostToDevice, s);
+    if (e != cudaSuccess) {
+        return cuda_fail(e, "jq_decoder_verify_pages");
+    }
+    rc = jq_verify_drafts(d->device, JQ_ELEM_F32, d->logits, (int64_t)rows * d->vocab, d->vocab, x, q, (int64_t)drafts * d->vocab, d->vocab, u, nullptr, n_seqs, drafts, d->vocab, 1,
+                          temperature, accepted, next, space + small + (q_bytes + 255) / 256 * 256, need, s);
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    JQ_CUDA(cudaMemcpyAsync(accepted_host, accepted, (size_t)n_seqs * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+    JQ_CUDA(cudaMemcpyAsync(next_host, next, (size_t)total * sizeof(int32_t), cudaMemcpyDeviceToHost, s));
+    JQ_CUDA(cudaStreamSynchronize(s));
+    const int code = read_status(d->status);
+    return code == 0 ? JQ_OK
+                     : (code == 98 ? fail(JQ_ERR_INVALID, "jq_decoder_verify_pages: a draft outside the vocabulary of %d", d->vocab)
+                                   : fail(JQ_ERR_TIMEOUT, "jq_decoder_verify_pages: a bounded wait on the device gave up (code %d)", code));
 }
 
 }  // extern "C"

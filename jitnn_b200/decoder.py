@@ -12,6 +12,7 @@ import numpy as np
 from . import _lib
 from ._lib import check
 from .ops import Tensor
+from .paged import _ELEM, RopeScaling
 
 _SLOT = {"wq": 0, "wk": 1, "wv": 2, "wo": 3, "w1": 4, "w3": 5, "w2": 6}
 
@@ -78,9 +79,10 @@ class LlamaDecoder:
     """With ``group`` (a torch.distributed process group of more than one rank, one process per GPU) the decoder is
     split by output rows of every linear: each rank keeps rows [rank * n / world, (rank + 1) * n / world) of each weight,
     the ranks exchange activations through peer buffers (set up here, collectively), and every rank must make the same
-    forward calls. Results are bitwise those of one GPU on the general kernels."""
+    forward calls. Results are bitwise those of one GPU on the general kernels. ``rope_scaling`` (a RopeScaling) rescales the rotation for a longer context, as the
+    reference's Llama does (Llama.java:109-121)."""
 
-    def __init__(self, layers, dim, heads, kv_heads, hidden, vocab, max_seq, eps=1e-5, rope_base=10000.0, device=0, group=None, sharded=False):
+    def __init__(self, layers, dim, heads, kv_heads, hidden, vocab, max_seq, eps=1e-5, rope_base=10000.0, device=0, group=None, sharded=False, rope_scaling=None):
         self.layers, self.dim, self.vocab, self.max_seq, self.device = layers, dim, vocab, max_seq, device
         self._weights = []  # keeps the borrowed weights alive
         self._pool = _PinnedPool()
@@ -90,6 +92,9 @@ class LlamaDecoder:
         L = _lib.load()
         check(L.jq_decoder_create(device, layers, dim, heads, kv_heads, hidden, vocab, max_seq, eps, rope_base, ctypes.byref(h)))
         self._h = h
+        if rope_scaling is not None:
+            freqs, magnitude = RopeScaling.frequencies(dim // heads, rope_base, rope_scaling)
+            check(L.jq_decoder_set_rope(h, (ctypes.c_double * len(freqs))(*freqs), magnitude))
         if sharded:
             self._set_up_shard(group)
 
@@ -186,6 +191,61 @@ class LlamaDecoder:
         check(_lib.load().jq_decoder_forward_batch(self._h, toks.ctypes.data, n, pos, None if logits is None else logits.ctypes.data,
                                                    nxt.ctypes.data, stream))
         return logits, nxt
+
+    def set_pages(self, pages, page_size=16, dtype="F16"):
+        """``pages`` pages of ``page_size`` keys (a power of two from 16 to 1024) for every layer, "F32", "F16" or "BF16"; what they held is lost, 0 releases them."""
+        if dtype not in _ELEM:
+            raise ValueError("pages of type %r (F32, F16 or BF16)" % (dtype,))
+        check(_lib.load().jq_decoder_set_pages(self._h, _ELEM[dtype], pages, page_size))
+
+    @staticmethod
+    def _paged(tables, lengths, prefix, prefix_length):
+        tables = [np.asarray(t, dtype=np.int32).reshape(-1) for t in tables]
+        lengths = np.ascontiguousarray(lengths, dtype=np.int32)
+        if len(tables) != lengths.size:
+            raise ValueError("%d tables of pages for %d lengths" % (len(tables), lengths.size))
+        padded = np.full((len(tables), max([1] + [t.size for t in tables])), -1, dtype=np.int32)
+        for row, t in zip(padded, tables):
+            row[: t.size] = t
+        prefix = np.ascontiguousarray([] if prefix is None else prefix, dtype=np.int32)
+        return padded, lengths, prefix, int(prefix_length)
+
+    def forward_pages(self, tokens, tables, lengths, prefix=None, prefix_length=0, want_logits=True, stream=None):
+        """New tokens of several sequences on the paged caches: ``tokens`` a list of each sequence's (up to 16 in all), ``tables`` of its pages, ``lengths`` how many keys of
+        its own it has with them; in front of those all sequences see the ``prefix_length`` keys on the pages ``prefix``. Returns (logits [tokens, vocab] or None,
+        next tokens [tokens]), one sequence after the other."""
+        padded, lengths, prefix, prefix_length = self._paged(tables, lengths, prefix, prefix_length)
+        counts = np.array([len(t) for t in tokens], dtype=np.int32)
+        if counts.size != lengths.size:
+            raise ValueError("tokens of %d sequences, %d lengths" % (counts.size, lengths.size))
+        toks = np.array([x for t in tokens for x in t], dtype=np.int32)
+        logits = self._pool.array((toks.size, self.vocab)) if want_logits else None
+        nxt = np.empty(toks.size, dtype=np.int32)
+        check(_lib.load().jq_decoder_forward_pages(self._h, toks.ctypes.data, counts.ctypes.data, counts.size, padded.ctypes.data, padded.shape[1], lengths.ctypes.data,
+                                                   prefix.ctypes.data, prefix.size, prefix_length, None if logits is None else logits.ctypes.data, nxt.ctypes.data, stream))
+        return logits, nxt
+
+    def verify_pages(self, tokens, tables, lengths, uniforms=None, draft_probs=None, temperature=0.0, prefix=None, prefix_length=0, stream=None):
+        """Speculative decoding: ``tokens`` [sequences, drafts + 1], each sequence's last token and its drafts, run as by forward_pages and verified (Speculative.verify) at
+        ``temperature``. Returns (accepted [sequences], tokens [sequences, drafts + 1])."""
+        padded, lengths, prefix, prefix_length = self._paged(tables, lengths, prefix, prefix_length)
+        toks = np.ascontiguousarray(tokens, dtype=np.int32)
+        if toks.ndim != 2 or toks.shape[0] != lengths.size or toks.shape[1] < 1:
+            raise ValueError("tokens of shape %s for %d sequences" % (list(toks.shape), lengths.size))
+        n, rows = toks.shape
+        if uniforms is not None:
+            uniforms = np.ascontiguousarray(uniforms, dtype=np.float32)
+            if uniforms.shape != (n, rows):
+                raise ValueError("uniforms of shape %s, needed %s" % (list(uniforms.shape), [n, rows]))
+        if draft_probs is not None:
+            draft_probs = np.ascontiguousarray(draft_probs, dtype=np.float32)
+            if draft_probs.shape != (n, rows - 1, self.vocab):
+                raise ValueError("draft_probs of shape %s, needed %s" % (list(draft_probs.shape), [n, rows - 1, self.vocab]))
+        accepted, out = np.empty(n, dtype=np.int32), np.empty((n, rows), dtype=np.int32)
+        check(_lib.load().jq_decoder_verify_pages(self._h, toks.ctypes.data, n, rows - 1, padded.ctypes.data, padded.shape[1], lengths.ctypes.data, prefix.ctypes.data, prefix.size,
+                                                  prefix_length, None if draft_probs is None else draft_probs.ctypes.data, None if uniforms is None else uniforms.ctypes.data,
+                                                  float(temperature), accepted.ctypes.data, out.ctypes.data, stream))
+        return accepted, out
 
     def close(self, collective=True):
         """Collective for a sharded decoder: the ranks unmap each other's buffers before any is freed."""
