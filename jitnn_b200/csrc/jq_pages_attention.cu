@@ -124,9 +124,16 @@ struct Plan {
 // How many thread blocks of the stream kernel an SM holds (by its registers).
 constexpr int stream_resident(int head_dim, int bytes) { return head_dim * bytes >= 512 ? 2 : 3; }
 
-// Rows of a key/value head that read the same keys: up to 16 go to the stream kernel, which reads the keys once for 8 or 16 rows; more go to the tile kernel, which takes 128 at
-// a time. It is made for 16-bit pages and heads of 64 and 128.
-constexpr int STREAM_ROWS = 16;
+// Which kernel: the stream kernel reads the keys once for 8 or 16 rows, the tile kernel (16-bit pages, heads of 64 and 128) for 128, but takes 10 us to begin and end an item.
+// A sequence's own keys, whose number only the device knows, by its rows per key/value head. 20 rows of 24 to 40 sequences behind a prefix: heads of 64 70 us here and
+// 71 there (FP32 rows 90 and 120), heads of 128 170 and 86 (206 and 145); 128 rows against 1000 keys, eight sequences: 34 and 33 us, 59 and 39.
+inline bool tile_takes_own(int head_dim, int64_t rows) { return rows > (head_dim == 64 ? 64 : 16); }
+// The prefix by its work. 8 key/value heads, bf16, heads of 64 / of 128: 128 rows against 256 keys 14 us here and 19 there / 17 and 21, 192 rows against 2048 keys 25 and 23 / 37 and 28,
+// 480 against 1024 29 and 28 / 48 and 40, against 4096 59 and 36 / 110 and 49.
+inline bool tile_takes_prefix(int head_dim, int kv_heads, int64_t rows, int64_t keys) { return (double)kv_heads * (double)rows * (double)keys * head_dim > 2.5e8; }
+// What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
+// heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
+constexpr int TILE_OVER = 3, STREAM_OVER = 4;
 
 Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length) {
     Plan plan;
@@ -136,8 +143,8 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
     }
     const int64_t group = heads / p->kv_heads, own = (tokens + sequences - 1) / sequences * group, shared = tokens * group;
     const bool tile = p->elem != JQ_ELEM_F32 && hd <= 128;
-    plan.tile_own = tile && own > STREAM_ROWS;
-    if (plan.tile_own || (tile && prefix_length > 0 && shared > STREAM_ROWS)) {
+    plan.tile_own = tile && tile_takes_own(hd, own);
+    if (plan.tile_own || (tile && prefix_length > 0 && tile_takes_prefix(hd, p->kv_heads, shared, prefix_length))) {
         const int resident = elem == p->elem ? 2 : 1;
         // (the prefix's units are known here; of the own keys the device knows)
         const int64_t units = (int64_t)p->kv_heads * ((shared + pages::TILE_BLOCK - 1) / pages::TILE_BLOCK) * ((prefix_length + pages::TILE_KEYS - 1) / pages::TILE_KEYS);
@@ -300,8 +307,8 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     auto floats = [&](int64_t at) { return reinterpret_cast<float*>(space + at); };
     auto pairs = [&](int64_t at) { return reinterpret_cast<float2*>(space + at); };
     const int ahead = prefix_length > 0 ? 1 : 0;
-    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 7, plan.tile_workers, floats(plan.tile_part), pairs(plan.tile_part_ml)};
-    const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, floats(plan.part), pairs(plan.part_ml)};
+    const Work tile{plan.tile_own ? 0 : sequences, sequences + ahead, 7, 7, plan.tile_workers, TILE_OVER, floats(plan.tile_part), pairs(plan.tile_part_ml)};
+    const Work few{0, sequences + (plan.tile_workers > 0 ? 0 : ahead), plan.rows == 8 ? 3 : 4, 4, plan.workers, STREAM_OVER, floats(plan.part), pairs(plan.part_ml)};
     a.own = plan.tile_own ? tile : few;
     a.pre = plan.tile_workers > 0 ? tile : few;
     a.wait_clocks = (long long)g_opt_wait_limit_us.load(std::memory_order_relaxed) * 2000;  // about 2 GHz

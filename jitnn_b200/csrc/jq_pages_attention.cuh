@@ -15,6 +15,7 @@ struct Work {
     int rows_shift;    // rows of a block, keys of a unit: powers of two
     int keys_shift;
     int workers;       // at most
+    int over;          // units that beginning and ending an item take the time of
     float* part;       // [slot][rows of a block][head_dim]
     float2* part_ml;   // maxima (of scores times log2 e) and sums
 };
@@ -44,11 +45,12 @@ struct Sequence {
     int keys;          // that its last row sees
     int reach;         // the same before it is cut to what the table of pages has, or below zero
     int blocks;        // of rows, per key/value head
-    int chunks;        // units of a block
-    __device__ int64_t units(int kv_heads) const { return (int64_t)kv_heads * blocks * chunks; }
+    int chunks;        // runs of keys
+    int cost;          // units of an item: its runs, and in front of them what beginning and ending it takes
+    __device__ int64_t units(int kv_heads) const { return (int64_t)kv_heads * blocks * cost; }
 };
 
-__device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int s, int rows_shift, int keys_shift) {
+__device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int s, int rows_shift, int keys_shift, int over) {
     Sequence q;
     if (s == a.b.sequences) {
         q.row0 = 0;
@@ -71,6 +73,7 @@ __device__ __forceinline__ Sequence sequence_at(const AttendArgs& a, int s, int 
     q.blocks = (int)(((int64_t)q.rows * a.group + (1 << rows_shift) - 1) >> rows_shift);
     q.chunks = (int)(((int64_t)q.keys + (1 << keys_shift) - 1) >> keys_shift);
     q.chunks = q.rows > 0 && q.chunks == 0 ? 1 : q.chunks;  // (rows without keys: an item that finds none)
+    q.cost = q.chunks + over;
     return q;
 }
 
@@ -90,42 +93,41 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t d) {
 
 struct Cut {
     int64_t total, per;
-    // What `found` says of a row of the item from unit item0 on.
-    __device__ __forceinline__ int2 found(int64_t item0, int chunks, int in_block) const {
-        const int first = worker_of(item0);
-        return make_int2(first, (worker_of(item0 + chunks - 1) - first + 1) << 8 | in_block);
+    int over;  // the items', where there are more units than workers (with fewer each of these is a worker's own)
+    // What `found` says of a row of the item whose first run of keys is unit `run0`.
+    __device__ __forceinline__ int2 found(int64_t run0, int chunks, int in_block) const {
+        const int first = worker_of(run0);
+        return make_int2(first, (worker_of(run0 + chunks - 1) - first + 1) << 8 | in_block);
     }
     __device__ __forceinline__ int worker_of(int64_t unit) const { return (int)quotient(unit, per); }
 };
 
-// By a whole warp: the units of sequences first .. end - 1 of a work, all of them together, and the units of a worker.
-__device__ __forceinline__ int64_t warp_sum(int64_t v) {
+// By a whole warp: how a work is cut.
+__device__ __forceinline__ Cut cut_of(const AttendArgs& a, const Work& w, int lane) {
+    int64_t runs = 0, items = 0;
+    for (int s = w.first + lane; s < w.last; s += 32) {
+        const Sequence q = sequence_at(a, s, w.rows_shift, w.keys_shift, 0);
+        runs += q.units(a.kv_heads);
+        items += (int64_t)a.kv_heads * q.blocks;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        v += __shfl_xor_sync(0xffffffffu, v, o);
+        runs += __shfl_xor_sync(0xffffffffu, runs, o);
+        items += __shfl_xor_sync(0xffffffffu, items, o);
     }
-    return v;
-}
-__device__ __forceinline__ int64_t units_before(const AttendArgs& a, const Work& w, int end, int lane) {
-    int64_t sum = 0;
-    for (int s = w.first + lane; s < end; s += 32) {
-        sum += sequence_at(a, s, w.rows_shift, w.keys_shift).units(a.kv_heads);
-    }
-    return warp_sum(sum);
-}
-__device__ __forceinline__ Cut cut_of(const Work& w, int64_t total) {
     Cut c;
-    c.total = total;
-    const int64_t used = total < w.workers ? total : w.workers;
-    c.per = used > 0 ? quotient(total + used - 1, used) : 1;
+    c.over = runs > w.workers ? w.over : 0;
+    c.total = runs + items * c.over;
+    const int64_t used = c.total < w.workers ? c.total : w.workers;
+    c.per = used > 0 ? quotient(c.total + used - 1, used) : 1;
     return c;
 }
 // The sequence that a unit is in, and the first unit of that sequence; by a whole warp.
-__device__ __forceinline__ int find_unit(const AttendArgs& a, const Work& w, int64_t unit, int lane, int64_t& base) {
+__device__ __forceinline__ int find_unit(const AttendArgs& a, const Work& w, int over, int64_t unit, int lane, int64_t& base) {
     int64_t before = 0;
     for (int s0 = w.first; s0 < w.last; s0 += 32) {
         const int s = s0 + lane;
-        const int64_t mine = s < w.last ? sequence_at(a, s, w.rows_shift, w.keys_shift).units(a.kv_heads) : 0;
+        const int64_t mine = s < w.last ? sequence_at(a, s, w.rows_shift, w.keys_shift, over).units(a.kv_heads) : 0;
         int64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {

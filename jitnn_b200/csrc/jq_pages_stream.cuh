@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
     uint8_t* const smem = all_smem + warp * S::Q_BYTES;
     const Work& work = a.own;
     const int worker = warp * (int)gridDim.x + (int)blockIdx.x;  // (few workers: on different SMs)
-    const Cut cut = cut_of(work, units_before(a, work, work.last, lane));
+    const Cut cut = cut_of(a, work, lane);
     int64_t begin = (int64_t)worker * cut.per;
     if (begin >= cut.total) {
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
     }
     const int64_t end = begin + cut.per < cut.total ? begin + cut.per : cut.total;
     int64_t base;
-    int s = find_unit(a, work, begin, lane, base);
-    Sequence sq = sequence_at(a, s, ROWS_SHIFT, KEYS_SHIFT);
+    int s = find_unit(a, work, cut.over, begin, lane, base);
+    Sequence sq = sequence_at(a, s, ROWS_SHIFT, KEYS_SHIFT, cut.over);
     const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
     const C* const k_pages = static_cast<const C*>(a.k_pages);
     const C* const v_pages = static_cast<const C*>(a.v_pages);
@@ -82,12 +82,17 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
         // ---- the next item, or the part of it that is this warp's
         while (begin >= base + sq.units(a.kv_heads)) {
             base += sq.units(a.kv_heads);
-            sq = sequence_at(a, ++s, ROWS_SHIFT, KEYS_SHIFT);
+            sq = sequence_at(a, ++s, ROWS_SHIFT, KEYS_SHIFT, cut.over);
         }
         const bool prefix = s == a.b.sequences;
-        const int64_t item = quotient(begin - base, sq.chunks), item0 = base + item * sq.chunks;
+        const int64_t item = quotient(begin - base, sq.cost), run0 = base + item * sq.cost + cut.over, behind = run0 + sq.chunks;
+        const int64_t from = begin < run0 ? run0 : begin, upto = end < behind ? end : behind;
+        begin = upto;
+        if (from >= upto) {  // (no run of it: another worker's)
+            continue;
+        }
         const int kvh = (int)quotient(item, sq.blocks), block = (int)(item - (int64_t)kvh * sq.blocks);
-        const int c0 = (int)(begin - item0), c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
+        const int c0 = (int)(from - run0), c1 = (int)(upto - run0);
         const int rows = sq.rows * a.group, row0 = block * ROWS;  // rows of the group: token * group + head
         const int* const table = prefix ? a.b.prefix : a.b.tables + s * a.b.table_stride;
         auto limit_of = [&](int r) { return row0 + r < rows ? keys_seen(a, sq, s, (row0 + r) / a.group) : sq.keys; };  // keys that row r of the block sees
@@ -460,7 +465,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 const int64_t token = sq.row0 + (row0 + r) / a.group;
                 const int head = kvh * a.group + (row0 + r) % a.group;
                 if (c0 == 0 && g == 0) {
-                    a.found[((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(item0, sq.chunks, r);
+                    a.found[((prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(run0, sq.chunks, r);
                 }
                 if (complete && !a.joined) {
                     T* const y = static_cast<T*>(a.out) + token * a.ot + head * a.oh;
@@ -483,7 +488,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
             }
         }
-        begin = item0 + c1;
     }
     // (behind the tile kernel: what waits for this kernel has waited for that one)
     asm volatile("griddepcontrol.wait;" ::: "memory");

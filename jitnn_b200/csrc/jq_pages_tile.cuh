@@ -138,33 +138,37 @@ __device__ __forceinline__ void copy_box(uint32_t to, const CUtensorMap* map, ui
 // What all of a thread block's roles go through alike: its items, each a run of tiles.
 struct Item {
     int s, kvh, row0, rows, c0, c1;
-    int64_t item0;
+    int64_t run0;
     bool prefix, complete;
 };
 struct Items {
     int64_t begin, end, base;
-    int s;
+    int s, over;
     Sequence sq;
     __device__ __forceinline__ bool next(const AttendArgs& a, Item& it) {
-        if (begin >= end) {
-            return false;
+        while (begin < end) {
+            while (begin >= base + sq.units(a.kv_heads)) {
+                base += sq.units(a.kv_heads);
+                sq = sequence_at(a, ++s, 7, 7, over);
+            }
+            const int64_t item = quotient(begin - base, sq.cost), run0 = base + item * sq.cost + over, behind = run0 + sq.chunks;
+            const int64_t from = begin < run0 ? run0 : begin, upto = end < behind ? end : behind;
+            begin = upto;
+            if (from >= upto) {  // (no run of it: another worker's)
+                continue;
+            }
+            it.s = s;
+            it.run0 = run0;
+            it.prefix = s == a.b.sequences;
+            it.kvh = (int)quotient(item, sq.blocks);
+            it.row0 = (int)(item - (int64_t)it.kvh * sq.blocks) * TILE_BLOCK;
+            it.rows = sq.rows * a.group;
+            it.c0 = (int)(from - run0);
+            it.c1 = (int)(upto - run0);
+            it.complete = it.c0 == 0 && it.c1 == sq.chunks;
+            return true;
         }
-        while (begin >= base + sq.units(a.kv_heads)) {
-            base += sq.units(a.kv_heads);
-            sq = sequence_at(a, ++s, 7, 7);
-        }
-        const int64_t item = quotient(begin - base, sq.chunks), item0 = base + item * sq.chunks;
-        it.s = s;
-        it.item0 = item0;
-        it.prefix = s == a.b.sequences;
-        it.kvh = (int)quotient(item, sq.blocks);
-        it.row0 = (int)(item - (int64_t)it.kvh * sq.blocks) * TILE_BLOCK;
-        it.rows = sq.rows * a.group;
-        it.c0 = (int)(begin - item0);
-        it.c1 = (int)((end < item0 + sq.chunks ? end : item0 + sq.chunks) - item0);
-        it.complete = it.c0 == 0 && it.c1 == sq.chunks;
-        begin = item0 + it.c1;
-        return true;
+        return false;
     }
 };
 
@@ -184,15 +188,16 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     asm volatile("griddepcontrol.launch_dependents;");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Work& work = a.pre;
-    const Cut cut = cut_of(work, units_before(a, work, work.last, lane));
+    const Cut cut = cut_of(a, work, lane);
     Items items;
     items.begin = (int64_t)blockIdx.x * cut.per;
     if (items.begin >= cut.total) {
         return;
     }
     items.end = items.begin + cut.per < cut.total ? items.begin + cut.per : cut.total;
-    items.s = find_unit(a, work, items.begin, lane, items.base);
-    items.sq = sequence_at(a, items.s, 7, 7);
+    items.over = cut.over;
+    items.s = find_unit(a, work, cut.over, items.begin, lane, items.base);
+    items.sq = sequence_at(a, items.s, 7, 7, cut.over);
     const uint32_t smem = (tc::smem_u32(raw_smem) + 1023u) & ~1023u;
     const uint32_t q_s = smem, k_s = smem + QP * L::Q_PART, v_s = k_s + KS * L::KV;
     auto bar = [&](int i) { return tc::smem_u32(&bars[i]); };
@@ -422,7 +427,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 const int64_t token = sq.row0 + i_token;
                 const int head = it.kvh * a.group + i_head;
                 if (real && it.c0 == 0) {
-                    a.found[((it.prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(it.item0, sq.chunks, row);
+                    a.found[((it.prefix ? (int64_t)a.b.tokens : 0) + token) * a.heads + head] = cut.found(it.run0, sq.chunks, row);
                 }
                 row_q[row] = real ? token * a.qt + head * a.qh : -1;
                 row_out[row] = !real      ? -1

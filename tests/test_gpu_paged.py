@@ -223,6 +223,24 @@ def check_attention(t, q, heads, kv, hd, act, cache, scale=None):
     return got
 
 
+@pytest.mark.parametrize("act,cache", TYPES[1:])
+@pytest.mark.parametrize("hd,rows,prefix,page", [(64, 4, 3905, 16), (128, 1, 4001, 64), (64, 1, 15700, 128)])
+def test_attention_behind_a_long_prefix(act, cache, hd, rows, prefix, page):
+    """More than 2.5e8 products with the prefix's keys, few rows a sequence: the prefix has a kernel of its own."""
+    n = 8 if rows > 1 else 16
+    t = Setup([rows] * n, [rows + 11 * i for i in range(n)], 2, hd, page, cache, prefix=prefix, pad=1, seed=21)
+    check_attention(t, normal(t.tokens, 32, hd, dtype=act, seed=21), 32, 2, hd, act, cache)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hd,rows,n", [(64, 1, 70), (128, 1, 70), (256, 1, 50), (64, 5, 23), (128, 3, 30)])
+def test_attention_of_many_short_sequences(act, cache, hd, rows, n):
+    """More runs of keys than workers: where one begins or ends, an item's first runs, its last ones or none of them may be a worker's."""
+    t = Setup([rows] * n, [(37 * i) % 290 for i in range(n)], 8, hd, 16, cache, prefix=40 if n == 23 else 0, seed=22)
+    heads = 128 if rows > 1 else 8
+    check_attention(t, normal(t.tokens, heads, hd, dtype=act, seed=22), heads, 8, hd, act, cache)
+
+
 @pytest.mark.parametrize("act,cache", TYPES)
 @pytest.mark.parametrize("hd", [64, 128, 256, 40])
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
