@@ -5,12 +5,13 @@
 // At temperature 0 the likeliest token (the first of equal ones) takes the place of both.
 //
 // The results are whole numbers that may not depend on how the work is cut, so everything is computed in double: the products u q of two floats are exact, sums of a
-// vocabulary's probabilities are good to 1e-14, and a cut in another place moves a token with a chance of about 1e-10.
+// vocabulary's probabilities are good to 1e-12, and a cut in another place moves a token with a chance of about 1e-10.
 //
 // Logits: stats_kernel takes the maximum and the sum of exponentials of chunks of all rows that count. choose_kernel is one cluster per sequence: it joins the chunks, finds the
 // row, adds up the row's weights (its second reading, from L2) and looks the token up. The exponential is table-driven (Tang 1989): 2^(t / 32) = 2^n 2^(j / 32) 2^(r / 32) with
-// the 32 values of the middle factor in a warp's lanes and a polynomial of the fifth degree, |r| <= 1/2, 13 double instructions where exp() takes about 48.
-// Bound: 64 of those a clock and SM, 11 us for the 16.8 million logits of 16 sequences with 8 rows of 131072, beside 10 us for reading them.
+// the 32 values of the middle factor in a warp's lanes and a polynomial of the fourth degree, |r| <= 1/2, 10 double instructions where exp() takes about 48.
+// Bound: each takes two of the turns in which an SM's quarters issue, some 17 others one: 37 turns for 32 values, 18 us for the 16.8 million logits of 16 sequences with 8 rows of 131072
+// (22 measured), beside 10 us for reading them; the choice behind it 11 us, half of which are latencies one after the other.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -22,7 +23,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int STATS_THREADS = 256, CHUNK_MOST = 8192;
+constexpr int STATS_THREADS = 128, STATS_RESIDENT = 9;  // (thread blocks of an SM, by their registers)
 constexpr int CHOOSE_THREADS = 512, CHOOSE_WARPS = CHOOSE_THREADS / 32, CLUSTER = 8;  // (the largest)
 
 struct Stat {
@@ -43,6 +44,7 @@ struct VerifyArgs {
     const int* counts;
     int sequences, drafts_most, vocab;
     double inverse;     // of the temperature
+    float far, reach;   // -690 and 600 of its units: what Exponential takes as zero, and where a sum moves to a larger maximum
     int *accepted, *tokens;
     Stat* stats;        // [row][chunks]
     int chunk, chunks;
@@ -55,26 +57,25 @@ __device__ __forceinline__ int count_of(const VerifyArgs& a, int b) {
     return n < 0 ? 0 : (n > a.drafts_most ? a.drafts_most : n);
 }
 
-// exp((x - top) inverse) of a warp's 32 numbers; every lane has 2^(lane / 32) in `entry`. Off by less than 4e-15 of it: the polynomial's remainder is (ln 2 / 64)^6 / 720 = 2.2e-15,
-// the roundings of t (whose integer part is at most 2^15 here) and of the products the rest.
+// exp((x - top) inverse) of a warp's 32 numbers; every lane has 2^(lane / 32) in `entry`. Off by less than 1.3e-12 of it, (ln 2 / 64)^5 / 120 = 1.25e-12 the polynomial's remainder
+// (with the sign of r, so that sums are far better); a degree more would take a thirteenth of the time for digits that no token depends on.
 struct Exponential {
     double to_32nds, entry;  // 32 / ln 2 times inverse
     float far;               // x - top below this: less than e^-690, taken as zero (minus infinity too)
-    __device__ __forceinline__ Exponential(double inverse, int lane) : to_32nds(inverse * 46.166241308446828384), entry(exp2(lane / 32.0)), far((float)(-690.0 / inverse)) {}
+    __device__ __forceinline__ Exponential(const VerifyArgs& a, int lane) : to_32nds(a.inverse * 46.166241308446828384), entry(exp2(lane * 0.03125)), far(a.far) {}
     // Of x far below, zero (ZERO), or something no larger than e^-690 (a NaN too).
     template <bool ZERO>
     __device__ __forceinline__ double of(float x, float top) const {
         if (!ZERO) {
             x = fmaxf(x, top + far);
         }
-        const double t = ((double)x - (double)top) * to_32nds;
-        const double shifted = t + 6755399441055744.0;  // 2^52 + 2^51: the nearest integer in the low bits
+        constexpr double NEAREST = 6755399441055744.0;  // 2^52 + 2^51: the nearest integer in the low bits
+        const double d = (double)x - (double)top, shifted = fma(d, to_32nds, NEAREST), r = fma(d, to_32nds, NEAREST - shifted);
         const int k = __double2loint(shifted);
-        const double r = t - (shifted - 6755399441055744.0);
         // (2^(r / 32) - 1) = sum (r ln 2 / 32)^i / i!
-        constexpr double A = 0.021660849392498290, A2 = A * A / 2, A3 = A * A * A / 6, A4 = A * A * A * A / 24, A5 = A * A * A * A * A / 120;
-        const double p = r * fma(r, fma(r, fma(r, fma(r, A5, A4), A3), A2), A);
-        const double e = __shfl_sync(0xffffffffu, entry, k & 31);
+        constexpr double A = 0.021660849392498290, A2 = A * A / 2, A3 = A * A * A / 6, A4 = A * A * A * A / 24;
+        const double p = r * fma(r, fma(r, fma(r, A4, A3), A2), A);
+        const double e = __shfl_sync(0xffffffffu, entry, k);
         const double v = fma(e, p, e);
         const double scaled = __hiloint2double(__double2hiint(v) + ((k & ~31) << 15), __double2loint(v));  // (times 2^(k / 32))
         return ZERO && x - top < far ? 0.0 : scaled;
@@ -111,11 +112,11 @@ __device__ __forceinline__ double warp_scan(double v, int lane) {  // sums up to
     return v;
 }
 
-// A chunk of a row in one reading, eight values a thread on their way at a time. SUMS: every thread adds exponentials up relative to the largest of its first eight numbers, which
-// in double need not be the largest of all: only a number e^600 times as large moves it. Else the largest and where it is first.
+// A chunk of a row in one reading, eight values a thread on their way while it works on the eight before. SUMS: every thread adds exponentials up relative to the largest of its first
+// eight numbers, which in double need not be the largest of all: only a number e^600 times as large moves it. Else the largest and where it is first.
 template <typename T, bool SUMS>
-__global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
-    constexpr int TAKE = 8, STEP = TAKE * STATS_THREADS;
+__global__ void __launch_bounds__(STATS_THREADS, STATS_RESIDENT) stats_kernel(VerifyArgs a) {
+    constexpr int RUN = 4, TAKE = 2 * RUN, APART = RUN * STATS_THREADS, STEP = 2 * APART;  // two runs of neighbouring values
     __shared__ double sums[STATS_THREADS / 32];
     __shared__ float tops[STATS_THREADS / 32];
     __shared__ int ats[STATS_THREADS / 32];
@@ -126,32 +127,48 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
     }
     const T* x = static_cast<const T*>(a.target) + b * a.tb + i * a.tr;
     const int c0 = blockIdx.x * a.chunk, c1 = c0 + a.chunk < a.vocab ? c0 + a.chunk : a.vocab;
-    const Exponential exponential(SUMS ? a.inverse : 1.0, lane);
-    const float reach = SUMS ? (float)(600.0 / a.inverse) : 0.0f;
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & (RUN * sizeof(T) - 1)) == 0;
+    const Exponential exponential(a, lane);
     float top = -INFINITY;
     int at = 0x7fffffff;
     double sum = 0.0;
-#pragma unroll 1
-    for (int j0 = c0 + (tid & ~31); j0 < c1; j0 += STEP) {  // (a warp's lanes stay together)
-        float v[TAKE];
-        if (j0 + 31 + (TAKE - 1) * STATS_THREADS < c1) {
+    auto take = [&](int j, float (&v)[TAKE]) {  // (behind the chunk: minus infinity)
 #pragma unroll
-            for (int n = 0; n < TAKE; n++) {
-                v[n] = to_float(x[j0 + lane + n * STATS_THREADS]);
-            }
-        } else {
+        for (int h = 0; h < 2; h++) {
+            const int from = j + h * APART;
+            if (wide && from + RUN <= c1) {
+                if constexpr (sizeof(T) == 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(x + from);
+                    v[4 * h] = f.x; v[4 * h + 1] = f.y; v[4 * h + 2] = f.z; v[4 * h + 3] = f.w;
+                } else {
+                    const uint2 f = *reinterpret_cast<const uint2*>(x + from);
+                    const T* const e = reinterpret_cast<const T*>(&f);
 #pragma unroll
-            for (int n = 0; n < TAKE; n++) {
-                v[n] = j0 + lane + n * STATS_THREADS < c1 ? to_float(x[j0 + lane + n * STATS_THREADS]) : -INFINITY;
+                    for (int n = 0; n < RUN; n++) {
+                        v[4 * h + n] = to_float(e[n]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < RUN; n++) {
+                    v[4 * h + n] = from + n < c1 ? to_float(x[from + n]) : -INFINITY;
+                }
             }
         }
+    };
+    float v[TAKE], v_next[TAKE];
+    take(c0 + tid * RUN, v);
+#pragma unroll 1
+    for (int j0 = c0; j0 < c1; j0 += STEP) {  // (a warp's lanes stay together)
+        const int j = j0 + tid * RUN;
+        take(j + STEP, v_next);
         if constexpr (SUMS) {
             float here = v[0];
 #pragma unroll
             for (int n = 1; n < TAKE; n++) {
                 here = fmaxf(here, v[n]);
             }
-            const bool far = here > top + reach;  // (top is minus infinity at first, and as long as nothing else has come)
+            const bool far = here > top + a.reach;  // (top is minus infinity at first, and as long as nothing else has come)
             if (__any_sync(0xffffffffu, far)) {
                 const double shrink = exponential.of<true>(top, far ? here : 0.0f);
                 sum = far && sum != 0.0 ? sum * shrink : sum;
@@ -166,11 +183,15 @@ __global__ void __launch_bounds__(STATS_THREADS) stats_kernel(VerifyArgs a) {
         } else {
 #pragma unroll
             for (int n = 0; n < TAKE; n++) {  // (in rising order: the first of equal ones stays)
-                const int j = j0 + lane + n * STATS_THREADS;
-                const bool larger = v[n] > top || (at == 0x7fffffff && v[n] == top && j < c1);
-                at = larger ? j : at;
+                const int here = j + (n & 3) + (n >> 2) * APART;
+                const bool larger = v[n] > top || (at == 0x7fffffff && v[n] == top && here < c1);
+                at = larger ? here : at;
                 top = larger ? v[n] : top;
             }
+        }
+#pragma unroll
+        for (int n = 0; n < TAKE; n++) {
+            v[n] = v_next[n];
         }
     }
     const float mine = top;
@@ -243,7 +264,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     if (tid == 0) {
         refused = 0x7fffffff;
     }
-    const Exponential exponential(FORM == LOGITS ? a.inverse : 1.0, lane);
+    const Exponential exponential(a, lane);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int count = count_of(a, b);
     const T* const target = static_cast<const T*>(a.target) + b * a.tb;
@@ -439,13 +460,21 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     }
 }
 
-// How a row is cut for its statistics: chunks of up to CHUNK_MOST values, shorter ones while that leaves SMs without a thread block.
-int chunk_of(int64_t rows, int vocab) {
-    int chunk = CHUNK_MOST;
-    while (chunk > 1024 && rows * ((vocab + chunk - 1) / chunk) < 4 * 148) {
-        chunk /= 2;
+// How a row is cut for its statistics: into as many chunks as fill the SMs' thread blocks once, twice, three or four times, whichever has them done first. A thread block's
+// beginning and end take the time of about 1024 values. (Chunks of 8192 throughout: 128 rows of 131072 30 us.)
+int chunk_of(int64_t rows, int64_t vocab) {
+    const int64_t room = 148 * STATS_RESIDENT;
+    int64_t best = 0, least = 0;
+    for (int64_t times = 1; times <= 4; times++) {
+        const int64_t fit = rows < 1 ? 1 : room * times / rows, most = (vocab + 511) / 512, chunks = fit < 1 ? 1 : (fit < most ? fit : most);
+        const int64_t chunk = ((vocab + chunks - 1) / chunks + 511) / 512 * 512;
+        const int64_t waves = (rows * ((vocab + chunk - 1) / chunk) + room - 1) / room, cost = waves * (chunk + 1024);
+        if (times == 1 || cost < least) {
+            best = chunk;
+            least = cost;
+        }
     }
-    return chunk;
+    return (int)best;
 }
 
 template <typename T, int FORM>
@@ -495,7 +524,7 @@ JQ_API int jq_verify_bytes(int64_t sequences, int64_t drafts, int64_t vocab, int
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: %lld sequences of %lld drafts, %lld tokens (at most 65535 rows, 4095 drafts, 2^30 tokens)", (long long)sequences,
                     (long long)drafts, (long long)vocab);
     }
-    const int64_t rows = sequences * (drafts + 1), chunk = chunk_of(rows, (int)vocab);
+    const int64_t rows = sequences * (drafts + 1), chunk = chunk_of(rows, vocab);
     *nbytes = logits != 0 ? rows * ((vocab + chunk - 1) / chunk) * (int64_t)sizeof(Stat) : 0;
     return JQ_OK;
 }
@@ -514,7 +543,7 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     if (!elem_ok(elem) || target == nullptr || (drafts == nullptr && drafts_most > 0) || accepted == nullptr || tokens == nullptr) {
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: null pointer, or element type %d", elem);
     }
-    if (logits != 0 ? !(temperature >= 0.0 && std::isfinite(temperature) && (temperature == 0.0 || std::isfinite(1.0 / temperature))) : false) {
+    if (logits != 0 ? !(temperature >= 0.0 && std::isfinite(temperature) && (temperature == 0.0 || std::isfinite(64.0 / temperature))) : false) {
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: temperature %g", temperature);
     }
     const int form = logits == 0 ? PROBABILITIES : (temperature == 0.0 ? GREEDY : LOGITS);
@@ -539,9 +568,11 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     a.drafts = drafts; a.u = uniforms; a.counts = counts;
     a.sequences = (int)sequences; a.drafts_most = (int)drafts_most; a.vocab = (int)vocab;
     a.inverse = form == LOGITS ? 1.0 / temperature : 1.0;
+    a.far = (float)(-690.0 / a.inverse);
+    a.reach = (float)(600.0 / a.inverse);
     a.accepted = accepted; a.tokens = tokens;
     a.stats = static_cast<Stat*>(workspace);
-    a.chunk = chunk_of(sequences * (drafts_most + 1), a.vocab);
+    a.chunk = chunk_of(sequences * (drafts_most + 1), vocab);
     a.chunks = (a.vocab + a.chunk - 1) / a.chunk;
     // eight thread blocks a sequence while all of them fit the GPU at once (two to an SM), and not more than leave a warp 256 values
     a.cluster = CLUSTER;
