@@ -211,7 +211,11 @@ int take_status_word(int** word) {
     if (g_status_free.empty()) {
         constexpr int WORDS = 1024;
         void* slab = nullptr;  // kept until the process ends: devices keep their words
-        JQ_CUDA(cudaHostAlloc(&slab, WORDS * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (the first call of all may be captured, or run while another thread captures)
+        JQ_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t e = cudaHostAlloc(&slab, WORDS * sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+        JQ_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        JQ_CUDA(e);
         memset(slab, 0, WORDS * sizeof(int));
         for (int i = 0; i < WORDS; i++) {
             g_status_free.push_back(static_cast<int*>(slab) + i);  // (one address on host and devices)

@@ -56,6 +56,11 @@ def _span(x):
     return x.data_ptr(), x.data_ptr() + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size() if x.numel() else x.data_ptr()
 
 
+def _overlap(x, y):
+    a, b = _span(x), _span(y)
+    return a[0] < b[1] and b[0] < a[1]
+
+
 def _output(out, x, what):
     """`out`, checked against x, which it may be, but not overlap otherwise; or a new tensor."""
     if out is None:
@@ -65,8 +70,7 @@ def _output(out, x, what):
     if out.numel() and out.stride(-1) != 1 or any(s == 0 and n > 1 for n, s in zip(out.shape, out.stride())):
         raise ValueError("%s: output of strides %s" % (what, list(out.stride())))
     if not (out.data_ptr() == x.data_ptr() and out.stride() == x.stride()):
-        a, b = _span(out), _span(x)
-        if a[0] < b[1] and b[0] < a[1]:
+        if _overlap(out, x):
             raise ValueError("%s: the output overlaps the input and is not the input" % what)
     return out
 
@@ -273,6 +277,8 @@ class PagedCache:
             if qcode != code or q.shape[0] != k.shape[0]:
                 raise ValueError("append: queries %s %s and keys %s %s" % (q.dtype, list(q.shape), k.dtype, list(k.shape)))
             y = _output(out, q, "append")
+            if y.data_ptr() != q.data_ptr() and any(_overlap(y, x) for x in (k, v)):
+                raise ValueError("append: the output overlaps the keys or the values")
             heads, qp, yp = q.shape[1], q.data_ptr(), y.data_ptr()
             strides = (ctypes.c_int64 * 8)(q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), y.stride(0), y.stride(1))
         if k.shape[0]:
