@@ -118,6 +118,7 @@ struct Plan {
     int workers = 0;           // its warps
     int tile_workers = 0;      // the tile kernel's thread blocks; 0: it is not launched
     bool tile_own = false;     // whether it takes own keys too, not the prefix alone
+    bool warp_a_row = false;   // how the joining kernel works
     int64_t part = 0, part_ml = 0, tile_part = 0, tile_part_ml = 0, whole = 0, whole_ml = 0, found = 0, bytes = 0;
 };
 
@@ -134,6 +135,10 @@ inline bool tile_takes_prefix(int head_dim, int kv_heads, int64_t rows, int64_t 
 // What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
 // heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
+
+// Whether one warp joins a row, or four do. bf16, 64 heads of 128, in all: 1 token against 4000 keys 21 us with one and 16 with four, 16 tokens against 1000 17.5 and 16.9,
+// 48 behind 2048 31 and 34, 120 behind 4096 53 and 66, 800 against 1000 72 and 108; 48 tokens of 32 heads behind 8192 keys, of whose partial results a row has 18, 145 and 142.
+inline bool warp_joins_row(int64_t rows, int64_t partial) { return rows > 1200 && (partial < 12 || rows > 4800); }
 
 Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length) {
     Plan plan;
@@ -154,6 +159,13 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
         plan.rows = own <= 8 || hd == 256 ? 8 : 16;
         plan.workers = 148 * stream_resident(hd, elem_bytes(p->elem)) * pages::STREAM_WARPS;
     }
+    // (an item that there are few of is cut into about as many pieces as there are workers for each; of the prefix's the length is known)
+    const int own_rows = plan.tile_own ? pages::TILE_BLOCK : plan.rows, shared_rows = plan.tile_workers > 0 ? pages::TILE_BLOCK : plan.rows;
+    const int64_t own_items = sequences * p->kv_heads * ((own + own_rows - 1) / own_rows), of_own = (plan.tile_own ? plan.tile_workers : plan.workers) / own_items;
+    const int64_t shared_items = p->kv_heads * ((shared + shared_rows - 1) / shared_rows), shared_workers = plan.tile_workers > 0 ? plan.tile_workers : plan.workers;
+    const int64_t runs = (prefix_length + (plan.tile_workers > 0 ? pages::TILE_KEYS : 16) - 1) / (plan.tile_workers > 0 ? pages::TILE_KEYS : 16);
+    const int64_t of_shared = runs / ((shared_items * runs + shared_workers) / shared_workers);
+    plan.warp_a_row = warp_joins_row(tokens * heads, of_own > of_shared ? of_own : of_shared);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
@@ -230,7 +242,13 @@ int launch_attend_head(const jq_pages* p, const AttendArgs& a, const Plan& plan,
             rc = launch_stream<T, C, HD, 2>(a, plan, s);
         }
     }
-    return rc != JQ_OK ? rc : launch_part(pages::attend_join_kernel<T, HD>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, s, a);
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (plan.warp_a_row) {
+        return launch_part(pages::attend_join_kernel<T, HD, 1>, dim3((unsigned)a.b.tokens, (unsigned)(a.heads + pages::JOIN_WARPS - 1) / pages::JOIN_WARPS), pages::JOIN_THREADS, 0, true, s, a);
+    }
+    return launch_part(pages::attend_join_kernel<T, HD, pages::JOIN_WARPS>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, s, a);
 }
 
 template <typename T, typename C>

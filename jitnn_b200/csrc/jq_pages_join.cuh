@@ -1,5 +1,5 @@
-// Joins what the workers have of a row: a thread block has one head of one token. Its warps take the partial results in turn, eight each at once, a lane each the maximum and
-// sum of 32. Which workers those are the one with the row's first keys has written down. (Worked out here from all lengths, it was most of this kernel: 15 us for 1536 rows.)
+// Joins what the workers have of a row (one head of one token), a lane each the maximum and sum of 32 partial results at a time. While there are fewer rows than warps the GPU holds, the
+// four warps of a thread block take a row's partial results in turn: few rows may have hundreds. With more rows a warp has a row. Which workers those are the one with the row's first keys has written down. (Worked out here from all lengths, it was most of this kernel: 15 us for 1536 rows.)
 #pragma once
 
 #include "jq_pages_attention.cuh"
@@ -10,17 +10,20 @@ namespace pages {
 
 constexpr int JOIN_WARPS = 4, JOIN_THREADS = 32 * JOIN_WARPS;
 
-template <typename T, int HD>
+template <typename T, int HD, int WARPS>
 __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a) {
-    constexpr int V = HD / 32;  // elements of a lane
+    constexpr int V = HD / 32, BATCH = WARPS == 1 ? 4 : 8;  // elements of a lane; partial results on their way at a time
     __shared__ float meet[JOIN_WARPS][HD];
     __shared__ float2 meet_ml[JOIN_WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, token = blockIdx.x, h = blockIdx.y;
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS, token = blockIdx.x, h = blockIdx.y * (JOIN_WARPS / WARPS) + (threadIdx.x >> 5) / WARPS;
+    if (h >= a.heads) {
+        return;
+    }
     T* const out = static_cast<T*>(a.out) + (int64_t)token * a.ot + h * a.oh;
     const bool real = token >= a.b.starts[0] && token < a.b.starts[a.b.sequences];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!real) {
-        for (int d = threadIdx.x; d < HD && a.fill; d += JOIN_THREADS) {
+        for (int d = 32 * warp + lane; d < HD && a.fill; d += 32 * WARPS) {
             out[d] = from_float<T>(0.0f);
         }
         return;
@@ -47,7 +50,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
     for (int j = 0; j < V; j++) {
         acc[j] = 0.0f;
     }
-    const int all = count0 + count1, each = (all + JOIN_WARPS - 1) / JOIN_WARPS;
+    const int all = count0 + count1, each = (all + WARPS - 1) / WARPS;
     const int mine = each * warp < all ? each * warp : all, upto = mine + each < all ? mine + each : all;
     for (int n0 = mine; n0 < upto; n0 += 32) {
         const int n = n0 + lane;
@@ -85,10 +88,10 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
             acc[j] *= shrink;
         }
         const int here = upto - n0 < 32 ? upto - n0 : 32;
-        for (int i0 = 0; i0 < here; i0 += 8) {
-            float v[8][V], x[8];
+        for (int i0 = 0; i0 < here; i0 += BATCH) {
+            float v[BATCH][V], x[BATCH];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < BATCH; i++) {
                 const int k = i0 + i < here ? i0 + i : i0;  // (the last ones twice, the second time for nothing)
                 const float* const p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(from), k)) + lane * V;
                 x[i] = __shfl_sync(0xffffffffu, weight, k);
@@ -100,7 +103,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
+            for (int i = 0; i < BATCH; i++) {
                 if (i0 + i < here) {
 #pragma unroll
                     for (int j = 0; j < V; j++) {
@@ -109,6 +112,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
                 }
             }
         }
+    }
+    if constexpr (WARPS == 1) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            out[lane * V + j] = from_float<T>(over(acc[j], l));
+        }
+        return;
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
