@@ -129,9 +129,13 @@ constexpr int stream_resident(int head_dim, int bytes) { return head_dim * bytes
 // A sequence's own keys, whose number only the device knows, by its rows per key/value head. 20 rows of 24 to 40 sequences behind a prefix: heads of 64 70 us here and
 // 71 there (FP32 rows 90 and 120), heads of 128 170 and 86 (206 and 145); 128 rows against 1000 keys, eight sequences: 34 and 33 us, 59 and 39.
 inline bool tile_takes_own(int head_dim, int64_t rows) { return rows > (head_dim == 64 ? 64 : 16); }
-// The prefix by its work. 8 key/value heads, bf16, heads of 64 / of 128: 128 rows against 256 keys 14 us here and 19 there / 17 and 21, 192 rows against 2048 keys 25 and 23 / 37 and 28,
-// 480 against 1024 29 and 28 / 48 and 40, against 4096 59 and 36 / 110 and 49.
-inline bool tile_takes_prefix(int head_dim, int kv_heads, int64_t rows, int64_t keys) { return (double)kv_heads * (double)rows * (double)keys * head_dim > 2.5e8; }
+// The prefix by its products: here their number counts, there the pairs of 128 rows and 128 keys (with 2 and 3 parts of FP32 rows twice and three times as dear), and what its
+// launch costs. 8 key/value heads of 128, bf16, up to 100 keys a sequence: 128 rows against 2048 keys 26 us here and 23 there, against 4096 40 and 26, 384 against 1024 37 and 28 (with up to
+// 1000 keys, which the two kernels read one after the other, 49 and 53); 32 key/value heads, 16 rows against 4096 30 and 38; heads of 64, 192 rows against 1024 19 and 22, against 8192 65 and 33.
+inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t rows, int64_t keys) {
+    const double pairs = (double)kv_heads * (double)((rows + 127) / 128) * (double)((keys + 127) / 128);
+    return (double)kv_heads * (double)rows * (double)keys * head_dim > 3e8 + parts * (head_dim == 64 ? 1.5e5 : 2e5) * pairs;
+}
 // What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
 // heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
@@ -148,8 +152,9 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
     }
     const int64_t group = heads / p->kv_heads, own = (tokens + sequences - 1) / sequences * group, shared = tokens * group;
     const bool tile = p->elem != JQ_ELEM_F32 && hd <= 128;
+    const int parts = elem == p->elem ? 1 : (p->elem == JQ_ELEM_F16 ? 2 : 3);  // of a row's FP32 numbers
     plan.tile_own = tile && tile_takes_own(hd, own);
-    if (plan.tile_own || (tile && prefix_length > 0 && tile_takes_prefix(hd, p->kv_heads, shared, prefix_length))) {
+    if (plan.tile_own || (tile && prefix_length > 0 && tile_takes_prefix(hd, parts, p->kv_heads, shared, prefix_length))) {
         const int resident = elem == p->elem ? 2 : 1;
         // (the prefix's units are known here; of the own keys the device knows)
         const int64_t units = (int64_t)p->kv_heads * ((shared + pages::TILE_BLOCK - 1) / pages::TILE_BLOCK) * ((prefix_length + pages::TILE_KEYS - 1) / pages::TILE_KEYS);

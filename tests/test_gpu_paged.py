@@ -224,9 +224,9 @@ def check_attention(t, q, heads, kv, hd, act, cache, scale=None):
 
 
 @pytest.mark.parametrize("act,cache", TYPES[1:])
-@pytest.mark.parametrize("hd,rows,prefix,page", [(64, 4, 3905, 16), (128, 1, 4001, 64), (64, 1, 15700, 128)])
+@pytest.mark.parametrize("hd,rows,prefix,page", [(64, 4, 3905, 16), (128, 1, 4001, 64), (64, 1, 15700, 128), (64, 4, 8200, 16), (128, 1, 6500, 64)])
 def test_attention_behind_a_long_prefix(act, cache, hd, rows, prefix, page):
-    """More than 2.5e8 products with the prefix's keys, few rows a sequence: the prefix has a kernel of its own."""
+    """Many products with the prefix's keys, few rows a sequence: on both sides of where the prefix gets a kernel of its own."""
     n = 8 if rows > 1 else 16
     t = Setup([rows] * n, [rows + 11 * i for i in range(n)], 2, hd, page, cache, prefix=prefix, pad=1, seed=21)
     check_attention(t, normal(t.tokens, 32, hd, dtype=act, seed=21), 32, 2, hd, act, cache)
