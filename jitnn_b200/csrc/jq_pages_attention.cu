@@ -122,8 +122,9 @@ struct Plan {
     int64_t part = 0, part_ml = 0, tile_part = 0, tile_part_ml = 0, whole = 0, whole_ml = 0, found = 0, bytes = 0;
 };
 
-// How many thread blocks of the stream kernel an SM holds (by its registers).
-constexpr int stream_resident(int head_dim, int bytes) { return head_dim * bytes >= 512 ? 2 : 3; }
+// How many thread blocks of the stream kernel an SM holds (by its registers; 16 rows of heads of 128 with three spilled hundreds of bytes: 16 sequences of 2 rows of 64 heads against
+// 1000 keys, bf16, 28 us, with two 21).
+constexpr int stream_resident(int head_dim, int bytes, int rows) { return head_dim * bytes >= 512 || head_dim * rows >= 2048 ? 2 : 3; }
 
 // Which kernel: the stream kernel reads the keys once for 8 or 16 rows, the tile kernel (16-bit pages, heads of 64 and 128) for 128, but takes 10 us to begin and end an item.
 // A sequence's own keys, whose number only the device knows, by its rows per key/value head. 20 rows of 24 to 40 sequences behind a prefix: heads of 64 70 us here and
@@ -136,6 +137,9 @@ inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t
     const double pairs = (double)kv_heads * (double)((rows + 127) / 128) * (double)((keys + 127) / 128);
     return (double)kv_heads * (double)rows * (double)keys * head_dim > 3e8 + parts * (head_dim == 64 ? 1.5e5 : 2e5) * pairs;
 }
+// Whether the stream kernel's blocks have 16 rows for the prefix's sake, although the sequences' own have up to 8. 64 heads of 128 on 8, FP32 rows on half precision, 16 sequences: 2048
+// keys 25 us with 16 and 28 with 8, 500 keys 16 and 16 (with 1000 own keys a sequence 23 and 21); 16 rows of each of 32 key/value heads, FP32 pages, 2048 keys 48 and 42.
+inline bool blocks_of_sixteen(int head_dim, int64_t kv_heads, int64_t rows, int64_t keys) { return rows >= 96 && (double)kv_heads * (double)rows * (double)keys * head_dim > 2.4e8; }
 // What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
 // heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
@@ -161,8 +165,8 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
         plan.tile_workers = (int)(!plan.tile_own && units < 148 * resident ? units : 148 * resident);
     }
     if (!plan.tile_own) {
-        plan.rows = own <= 8 || hd == 256 ? 8 : 16;
-        plan.workers = 148 * stream_resident(hd, elem_bytes(p->elem)) * pages::STREAM_WARPS;
+        plan.rows = hd <= 128 && (own > 8 || (plan.tile_workers == 0 && blocks_of_sixteen(hd, p->kv_heads, shared, prefix_length))) ? 16 : 8;
+        plan.workers = 148 * stream_resident(hd, elem_bytes(p->elem), plan.rows) * pages::STREAM_WARPS;
     }
     // (an item that there are few of is cut into about as many pieces as there are workers for each; of the prefix's the length is known)
     const int own_rows = plan.tile_own ? pages::TILE_BLOCK : plan.rows, shared_rows = plan.tile_workers > 0 ? pages::TILE_BLOCK : plan.rows;
@@ -223,7 +227,7 @@ template <typename T, typename C, int HD, int NB>
 int launch_stream(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
     static std::atomic<uint64_t> configured{0};
     constexpr int smem = pages::Stream<T, C, HD, NB>::SMEM;
-    auto kernel = pages::attend_stream_kernel<T, C, HD, NB, stream_resident(HD, sizeof(C))>;
+    auto kernel = pages::attend_stream_kernel<T, C, HD, NB, stream_resident(HD, sizeof(C), 8 * NB)>;
     const int rc = smem > 48 * 1024 ? large_smem(kernel, smem, configured) : JQ_OK;
     return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, plan.tile_workers > 0, s, a);
 }
