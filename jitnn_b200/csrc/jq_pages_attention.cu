@@ -127,9 +127,10 @@ struct Plan {
 constexpr int stream_resident(int head_dim, int bytes, int rows) { return head_dim * bytes >= 512 || head_dim * rows >= 2048 ? 2 : 3; }
 
 // Which kernel: the stream kernel reads the keys once for 8 or 16 rows, the tile kernel (16-bit pages, heads of 64 and 128) for 128, but takes 10 us to begin and end an item.
-// A sequence's own keys, whose number only the device knows, by its rows per key/value head. 20 rows of 24 to 40 sequences behind a prefix: heads of 64 70 us here and
-// 71 there (FP32 rows 90 and 120), heads of 128 170 and 86 (206 and 145); 128 rows against 1000 keys, eight sequences: 34 and 33 us, 59 and 39.
-inline bool tile_takes_own(int head_dim, int64_t rows) { return rows > (head_dim == 64 ? 64 : 16); }
+// A sequence's own keys, whose number only the device knows, by its rows per key/value head; 8 of those, up to 1000 keys. 40 sequences, heads of 64, FP32 rows on half precision: 32 rows 36 us
+// here and 66 there, 80 rows 73 and 68; bf16 33 and 43, 64 and 51. Heads of 128, 16 sequences: 32 rows 30 and 44, 48 rows 40 and 44, 80 rows 55 and 45; bf16 28 and 32, 37 and 35, 50 and 36, but with
+// a prefix of 2048 keys, which the tile kernel takes along, 20 rows 46 and 36, 32 rows 50 and 38.
+inline bool tile_takes_own(int head_dim, int parts, int64_t rows, int64_t prefix) { return rows > (head_dim == 64 ? 64 : (parts == 1 && prefix > 0 ? 16 : 32)); }
 // The prefix by its products: here their number counts, there the pairs of 128 rows and 128 keys (with 2 and 3 parts of FP32 rows twice and three times as dear), and what its
 // launch costs. 8 key/value heads of 128, bf16, up to 100 keys a sequence: 128 rows against 2048 keys 26 us here and 23 there, against 4096 40 and 26, 384 against 1024 37 and 28 (with up to
 // 1000 keys, which the two kernels read one after the other, 49 and 53); 32 key/value heads, 16 rows against 4096 30 and 38; heads of 64, 192 rows against 1024 19 and 22, against 8192 65 and 33.
@@ -157,7 +158,7 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
     const int64_t group = heads / p->kv_heads, own = (tokens + sequences - 1) / sequences * group, shared = tokens * group;
     const bool tile = p->elem != JQ_ELEM_F32 && hd <= 128;
     const int parts = elem == p->elem ? 1 : (p->elem == JQ_ELEM_F16 ? 2 : 3);  // of a row's FP32 numbers
-    plan.tile_own = tile && tile_takes_own(hd, own);
+    plan.tile_own = tile && tile_takes_own(hd, parts, own, prefix_length);
     if (plan.tile_own || (tile && prefix_length > 0 && tile_takes_prefix(hd, parts, p->kv_heads, shared, prefix_length))) {
         const int resident = elem == p->elem ? 2 : 1;
         // (the prefix's units are known here; of the own keys the device knows)
