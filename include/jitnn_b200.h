@@ -225,7 +225,7 @@ JQ_API int jq_quantize_q8_0(int device, const float* x, int64_t count, void* blo
  *                       mma.sync kernel declines; 1: all; 2: none.
  *   "wait_limit_us"     microseconds after which a kernel's wait for its own copies and tensor-core work gives up (default 2 000 000,
  *                       in the matrix and the rows kernel counted from the end of the kernel in front): the call returns JQ_ERR_TIMEOUT
- *                       or jq_device_status reports a code (1 to 8 matrix and rows kernel, 24 and 25 decode GEMVs, 64 + role
+ *                       or jq_device_status reports a code (1 to 8 matrix and rows kernel, 10 to 19 attention over pages, 24 and 25 decode GEMVs, 64 + role
  *                       tcgen05 GEMV), its outputs are undefined.
  */
 JQ_API int jq_set_option(const char* name, int64_t value);

@@ -2,10 +2,11 @@
 // the keys are the prefix) against tiles of 128 keys.
 //
 // Warps 0 to 7, two threads a row (a lane of tensor memory), each half of a tile's keys and half of a head's elements: queries into shared memory, then per tile the maximum of
-// the row's scores, its weights and their sum; and the sums over the values in registers. (With one thread a row a warp alone on its scheduler took five clocks an instruction.)
+// the row's scores, its weights and their sum. (With one thread a row a warp alone on its scheduler took five clocks an instruction.)
 // Warp 8 brings keys and values by tensor-map copies, a box for every page that a tile touches, and issues the products: S = Q K^T (tcgen05.mma,
 // 128 x 128, both operands in shared memory), O = P V (weights from tensor memory; values as they lie on the pages, elements of a head are the second operand's columns).
-// The instruction cuts off where it adds, so O only adds up a tile, and the threads add the tiles with the factor of the maximum (a sum of 8192 keys held in it was 4e-6 off).
+// The instruction cuts off where it adds (a sum of 8192 keys held in it was 4e-6 off). For FP32 rows O only adds up a tile, and the threads add the tiles in registers with the factor of the
+// maximum; 16-bit rows, whose rounding is a thousand times that, leave the sums in tensor memory, and only a maximum that rises by more than 2^8 has them scaled.
 // For 16-bit rows two thread blocks share an SM, one's products under the other's exponentials: weights take the place of the scores. FP32 rows are two half-precision
 // parts (with a power of two per row) or three bfloat16 parts, so many products for one, and weights likewise; their weights have columns of their own and, with
 // two parts, the scores two buffers, so that the next tile's are made meanwhile.
@@ -14,7 +15,8 @@
 // are cleared in shared memory, and the rows that do see such a key add it by themselves.
 //
 // Bound per tile and SM: the products' 1024 clocks at head size 128 (times the parts), the threads' 128 exponentials (1024 clocks at 16 a clock) and about 700 instructions a
-// warp, or 2800 clocks for 64 KB of pages where they come from memory.
+// warp, or 2800 clocks for 64 KB of pages where they come from memory. Measured, all launches of a call: 280 tokens of 32 heads of 128 on 8 behind 7182 keys, FP16, 81 us, 407 TFLOP/s; 48 tokens of
+// 64 heads behind 2048 keys, bf16, 30 us. What bounds it is one tile's chain: scores, maximum of both halves, weights, sums are 3.8 us, two of which share an SM.
 #pragma once
 
 #include "jq_pages_attention.cuh"

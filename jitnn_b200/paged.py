@@ -155,6 +155,8 @@ class Rope:
             if tuple(t.shape[:-2]) != lead or t.shape[-1] != hd or t.dtype is not xs[0].dtype:
                 raise ValueError("%s: %s %s beside %s %s" % (what, t.dtype, list(t.shape), xs[0].dtype, list(xs[0].shape)))
         ys = tuple(_output(o, t, what) for o, t in zip(outs, xs))
+        if len(xs) == 2 and all(t.numel() for t in xs) and (ys[0].data_ptr() in (ys[1].data_ptr(), xs[1].data_ptr()) or ys[1].data_ptr() == xs[0].data_ptr()):
+            raise ValueError("%s: one tensor is the other's output" % what)
         batch, seq = (1,) + lead if len(lead) == 1 else lead
         strides = (ctypes.c_int64 * (6 * len(xs)))()
         for i, t in enumerate(v for p in zip(xs, ys) for v in p):

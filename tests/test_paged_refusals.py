@@ -150,7 +150,9 @@ def test_construction_refused(stub, make, message):
     (lambda r: r.rotate((rows(4, 2, 64), rows(4, 2, 32)), 0), "beside"), (lambda r: r.rotate(rows(4, 2, 64), rows(3, dtype=I32)), "positions"), (lambda r: r.rotate(rows(4, 2, 64), rows(4)), "positions"),
     (lambda r: r.rotate(rows(4, 2, 64), 0, out=rows(4, 2, 64, dtype=F16)), "output"), (lambda r: r.rotate(rows(4, 2, 64), 0, out=rows(4, 3, 64)), "output"),
     (lambda r: r.rotate(rows(4, 2, 64), 0, out=rows(4, 64, 2).transpose(1, 2)), "strides"), (lambda r: r.rotate(rows(4, 2, 64), 0, out=rows(1, 2, 64).expand(4, 2, 64)), "strides"),
-    (lambda r: (lambda x: r.rotate(x[1:], 0, out=x[:-1]))(rows(5, 2, 64)), "overlaps"), (lambda r: r.backward(rows(4, 2, 64), rows(4, dtype=torch.int16)), "rotation backward: positions")])
+    (lambda r: (lambda x: r.rotate(x[1:], 0, out=x[:-1]))(rows(5, 2, 64)), "overlaps"), (lambda r: (lambda x: r.rotate((x, x), 0, out=(x, x)))(rows(4, 2, 64)), "the other's output"),
+    (lambda r: (lambda x, y: r.rotate((x, y), 0, out=(y, x)))(rows(4, 2, 64), rows(4, 2, 64)), "the other's output"),
+    (lambda r: (lambda x, y: r.rotate((x, y), 0, out=(y, None)))(rows(4, 2, 64), rows(4, 2, 64)), "the other's output"), (lambda r: r.backward(rows(4, 2, 64), rows(4, dtype=torch.int16)), "rotation backward: positions")])
 def test_rotation_refused(stub, call, message):
     rope = Rope(100, 64, device=-1)
     with pytest.raises(ValueError, match=message):
