@@ -438,7 +438,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
  * Draft i is kept while uniforms[i] q_i(x_i) < p_i(x_i); then one token comes by the inverse distribution function at uniforms[drafts_most]: behind the first refused draft j from
  * max(p_j - q_j, 0) over its sum (p_j where that is zero), behind the last draft from p. accepted[s] = the drafts kept, tokens [sequences, drafts_most + 1] = those, the
  * further token, and -1 in the rest. Temperature 0: the likeliest token (the first of equal ones) instead, uniforms and draft_probs are not read. No drafts at
- * all is sampling. All in double. A weight that is NaN counts as zero; where no weight is left the token is the last. A draft outside the vocabulary is refused and leaves status 98.
+ * all is sampling. A temperature above 0 is from 1e-300 to 1e30. All in double. A weight that is NaN counts as zero; where no weight is left the token is the last. A draft outside the vocabulary is refused and leaves status 98.
  * workspace: jq_verify_bytes (which also holds the limits of the sizes) of device memory at a 16-byte aligned address.
  */
 JQ_API int jq_verify_bytes(int64_t sequences, int64_t drafts_most, int64_t vocab, int logits, int64_t* nbytes);

@@ -63,12 +63,9 @@ struct Exponential {
     double to_32nds, entry;  // 32 / ln 2 times inverse
     float far;               // x - top below this: less than e^-690, taken as zero (minus infinity too)
     __device__ __forceinline__ Exponential(const VerifyArgs& a, int lane) : to_32nds(a.inverse * 46.166241308446828384), entry(exp2(lane * 0.03125)), far(a.far) {}
-    // Of x far below, zero (ZERO), or something no larger than e^-690 (a NaN too).
+    // Of x far below, zero (ZERO), or something no larger than 2^-1022 (of a NaN too). How far is a difference of floats: the sum of top and `far` may round to top, at a low temperature.
     template <bool ZERO>
     __device__ __forceinline__ double of(float x, float top) const {
-        if (!ZERO) {
-            x = fmaxf(x, top + far);
-        }
         constexpr double NEAREST = 6755399441055744.0;  // 2^52 + 2^51: the nearest integer in the low bits
         const double d = (double)x - (double)top, shifted = fma(d, to_32nds, NEAREST), r = fma(d, to_32nds, NEAREST - shifted);
         const int k = __double2loint(shifted);
@@ -77,8 +74,11 @@ struct Exponential {
         const double p = r * fma(r, fma(r, fma(r, A4, A3), A2), A);
         const double e = __shfl_sync(0xffffffffu, entry, k);
         const double v = fma(e, p, e);
-        const double scaled = __hiloint2double(__double2hiint(v) + ((k & ~31) << 15), __double2loint(v));  // (times 2^(k / 32))
-        return ZERO && x - top < far ? 0.0 : scaled;
+        const int high = __double2hiint(v) + ((k & ~31) << 15);  // (times 2^(k / 32))
+        if (ZERO) {
+            return x - top < far ? 0.0 : __hiloint2double(high, __double2loint(v));
+        }
+        return __hiloint2double(x - top >= far ? high : 0, __double2loint(v));
     }
 };
 
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(STATS_THREADS, STATS_RESIDENT) stats_kernel(Ve
             for (int n = 1; n < TAKE; n++) {
                 here = fmaxf(here, v[n]);
             }
-            const bool far = here > top + a.reach;  // (top is minus infinity at first, and as long as nothing else has come)
+            const bool far = here - top > a.reach;  // (top is minus infinity at first, and as long as nothing else has come)
             if (__any_sync(0xffffffffu, far)) {
                 const double shrink = exponential.of<true>(top, far ? here : 0.0f);
                 sum = far && sum != 0.0 ? sum * shrink : sum;
@@ -543,8 +543,8 @@ JQ_API int jq_verify_drafts(int device, int elem, const void* target, int64_t ta
     if (!elem_ok(elem) || target == nullptr || (drafts == nullptr && drafts_most > 0) || accepted == nullptr || tokens == nullptr) {
         return fail(JQ_ERR_INVALID, "jq_verify_drafts: null pointer, or element type %d", elem);
     }
-    if (logits != 0 ? !(temperature >= 0.0 && std::isfinite(temperature) && (temperature == 0.0 || std::isfinite(64.0 / temperature))) : false) {
-        return fail(JQ_ERR_INVALID, "jq_verify_drafts: temperature %g", temperature);
+    if (logits != 0 && temperature != 0.0 && !(temperature >= 1e-300 && temperature <= 1e30)) {
+        return fail(JQ_ERR_INVALID, "jq_verify_drafts: temperature %g (0, or from 1e-300 to 1e30)", temperature);
     }
     const int form = logits == 0 ? PROBABILITIES : (temperature == 0.0 ? GREEDY : LOGITS);
     if (form != GREEDY && uniforms == nullptr) {

@@ -39,8 +39,8 @@ def _cuda(x, what, device, dims):
     return x if x.stride(-1) == 1 else x.contiguous()
 
 
-def _whole(x, what, device, shape):
-    """An int32 CUDA tensor of that shape on `device`."""
+def _whole(x, what, device, shape, copy=True):
+    """An int32 CUDA tensor of that shape on `device`, contiguous, of which without `copy` nothing else may be made: it is read later."""
     torch = _t()
     if not isinstance(x, torch.Tensor) or x.dtype is not torch.int32:
         raise ValueError("%s: an int32 CUDA tensor is needed, got %s" % (what, x.dtype if isinstance(x, torch.Tensor) else type(x).__name__))
@@ -48,6 +48,8 @@ def _whole(x, what, device, shape):
         raise ValueError("%s of shape %s, needed %s" % (what, list(x.shape), list(shape)))
     if x.get_device() != device:
         raise ValueError("%s on %s, needed on cuda:%d" % (what, x.device, device))
+    if not copy and not x.is_contiguous():
+        raise ValueError("%s of strides %s, needed contiguous" % (what, list(x.stride())))
     return x.contiguous()
 
 
@@ -194,22 +196,25 @@ class PagedBatch:
     """Which rows of a call belong to which sequence and where their keys lie (int32 CUDA tensors, read when the kernels run; checked here, once).
 
     Rows ``starts[s] .. starts[s + 1] - 1`` are the newest of sequence s, which has ``lengths[s]`` keys of its own once they are appended, key i on page
-    ``tables[s, i // page_size]``. In front of them all sequences see the ``prefix_length`` keys on the pages ``prefix``."""
+    ``tables[s, i // page_size]``. In front of them all sequences see the ``prefix_length`` keys on the pages ``prefix``. Nothing is copied: what is changed in the tensors afterwards
+    counts for the calls behind."""
 
     def __init__(self, tables, starts, lengths, prefix=None, prefix_length=0):
         torch = _t()
         if not isinstance(tables, torch.Tensor) or tables.dim() != 2 or tables.dtype is not torch.int32 or not tables.is_cuda or 0 in tables.shape:
             raise ValueError("tables of pages: an int32 CUDA tensor [sequences, pages] is needed")
         self.device = tables.get_device()
-        self.tables = tables if tables.stride(1) == 1 or tables.shape[1] == 1 else tables.contiguous()
+        if tables.stride(1) != 1 and tables.shape[1] != 1:
+            raise ValueError("tables of pages of strides %s (a sequence's page numbers are to be next to each other)" % list(tables.stride()))
+        self.tables = tables
         sequences = tables.shape[0]
-        self.starts = _whole(starts, "starts", self.device, (sequences + 1,))
-        self.lengths = _whole(lengths, "lengths", self.device, (sequences,))
+        self.starts = _whole(starts, "starts", self.device, (sequences + 1,), copy=False)
+        self.lengths = _whole(lengths, "lengths", self.device, (sequences,), copy=False)
         self.prefix, self.prefix_length = None, int(prefix_length)
         if prefix is not None:
             if not isinstance(prefix, torch.Tensor) or prefix.dim() != 1:
                 raise ValueError("prefix: an int32 CUDA tensor [pages] is needed")
-            self.prefix = _whole(prefix, "prefix", self.device, prefix.shape)
+            self.prefix = _whole(prefix, "prefix", self.device, prefix.shape, copy=False)
         if self.prefix_length < 0 or (self.prefix_length > 0 and self.prefix is None):
             raise ValueError("a prefix of %d keys on %s" % (self.prefix_length, "no pages" if self.prefix is None else "%d pages" % self.prefix.numel()))
         self._rows = (self.tables.data_ptr(), self.tables.stride(0), self.tables.shape[1], self.starts.data_ptr(), self.lengths.data_ptr(), sequences)

@@ -90,7 +90,7 @@ def verify(target, drafts, uniforms, draft_probs=None, counts=None, temperature=
 
         def row(i):
             x = target[b, i].double()
-            return x if temperature is None else torch.softmax(x / temperature, -1)
+            return x if temperature is None else torch.softmax((x - x.max()) / temperature, -1)  # (1e10 / 1e-300 is above the largest double)
 
         def likeliest(i):
             x = target[b, i].double()

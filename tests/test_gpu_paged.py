@@ -232,6 +232,14 @@ def test_attention_behind_a_long_prefix(act, cache, hd, rows, prefix, page):
     check_attention(t, normal(t.tokens, 32, hd, dtype=act, seed=21), 32, 2, hd, act, cache)
 
 
+@pytest.mark.parametrize("act,cache", [(F32, F32), (F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("rows,lengths,prefix,page", [([500, 1, 40], [500, 1030, 700], 1300, 256), ([3, 2], [1024, 2049], 1025, 1024), ([700], [900], 0, 512)])
+def test_attention_of_prompts_and_of_large_pages(act, cache, heads, kv, hd, rows, lengths, prefix, page):
+    t = Setup(rows, lengths, kv, hd, page, cache, prefix=prefix, seed=23)
+    check_attention(t, normal(t.tokens, heads, hd, dtype=act, seed=23), heads, kv, hd, act, cache)
+
+
 @pytest.mark.parametrize("act,cache", TYPES)
 @pytest.mark.parametrize("hd,rows,n", [(64, 1, 70), (128, 1, 70), (256, 1, 50), (64, 5, 23), (128, 3, 30)])
 def test_attention_of_many_short_sequences(act, cache, hd, rows, n):

@@ -187,6 +187,20 @@ def test_a_generation_step_in_a_graph_beside_another():
     assert device_status(0) == 0
 
 
+def test_what_is_read_later_is_not_copied():
+    """A batch's numbers are read when the kernels run: changed in place they count, and tensors that would have to be copied are refused."""
+    pages, batch, rope, q, k, v = made()
+    before = pages.attention(q, batch)
+    batch.lengths.copy_(whole(9, 70, 1))
+    after, again = pages.attention(q, batch), pages.attention(q, PagedBatch(batch.tables, batch.starts, whole(9, 70, 1), prefix=batch.prefix, prefix_length=21))
+    assert torch.equal(after, again) and not torch.equal(after, before)
+    numbers = torch.zeros(4, 2, dtype=I32, device="cuda")
+    for change in ({"starts": numbers[:, 0]}, {"lengths": numbers[:3, 1]}, {"tables": batch.tables.t().contiguous().t()}, {"prefix": numbers[:2, 0], "prefix_length": 21}):
+        args = {"tables": batch.tables, "starts": batch.starts, "lengths": batch.lengths, **change}
+        with pytest.raises(ValueError, match="strides"):
+            PagedBatch(**args)
+
+
 def test_two_rows_for_one_place():
     """Two sequences on the same pages: where both write, either's key may stand, whole."""
     pages, _, _, q, k, v = made()

@@ -41,6 +41,20 @@ def test_verify(dtype, temperature, sequences, drafts, vocab, drafter, ragged):
     assert device_status(0) == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [1e-300, 1e-40, 1e-20, 1e-9, 1e-7, 1e-5, 1e4, 1e30])
+@pytest.mark.parametrize("size", [1e-3, 3.0, 1e4, 1e10, 1e30])
+def test_logits_and_temperatures_of_any_size(dtype, temperature, size):
+    """From all but one weight zero to all weights the same; logits whose steps are far above the temperature, equal ones and masked ones (minus infinity) among them."""
+    c = case(4, 3, 5003, dtype, 1.0, False, False, seed=11, size=size)
+    c["temperature"] = temperature
+    c["target"][0, :, ::7] = c["target"][0].amax(-1, keepdim=True)
+    c["target"][1, :, 100:] = -math.inf
+    c["drafts"][2] = c["target"][2, :3].argmax(-1).int()
+    check(c)
+    assert device_status(0) == 0
+
+
 def test_each_way_out():
     """All kept, none kept, refused in between; the drafter's own distribution: p and q are the same, the token comes from p."""
     c = case(64, 4, 50, torch.float32, None, True, False, seed=1, size=1.0)

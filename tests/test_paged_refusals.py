@@ -88,7 +88,7 @@ def test_verification_refused(lib):
 
     for change, message in (({"elem": 3}, "element type"), ({"target": None}, "null pointer"), ({"drafts": None}, "null pointer"), ({"accepted": None}, "null pointer"),
                             ({"uniforms": None}, "uniform numbers"), ({"uniforms": None, "logits": 0}, "uniform numbers"), ({"temperature": -1.0}, "temperature"),
-                            ({"temperature": math.nan}, "temperature"), ({"temperature": math.inf}, "temperature"), ({"temperature": 1e-320}, "temperature"),
+                            ({"temperature": math.nan}, "temperature"), ({"temperature": 1e31}, "temperature"), ({"temperature": math.inf}, "temperature"), ({"temperature": 1e-320}, "temperature"),
                             ({"temperature": 1e-307}, "temperature"), ({"space": None}, "workspace"), ({"space": 264}, "workspace"), ({"size": 127}, "workspace")):
         refused(lib, call(**change), message)
     assert lib.jq_verify_drafts(0, 0, None, 0, 0, None, None, 0, 0, None, None, 0, 3, 10, 1, 1.0, None, None, None, 0, None) == 0  # nothing to do
