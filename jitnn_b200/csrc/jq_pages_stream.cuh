@@ -62,6 +62,8 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
     constexpr int ROWS_SHIFT = NB == 1 ? 3 : 4, KEYS_SHIFT = 4;
     static_assert(ROWS == 1 << ROWS_SHIFT && CHUNK == 1 << KEYS_SHIFT, "");
     constexpr int PRODUCTS = KP > QP ? KP : QP;  // parts i and j meet where i + j < PRODUCTS
+    // Half-precision weights are times 2^15, which the end takes off: one at 2^-29 of the largest has all its bits, where it would be one of the type's smallest, or none, at 2^-24
+    constexpr float UP = BF ? 1.0f : 32768.0f;
     extern __shared__ __align__(16) uint8_t all_smem[];
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -319,8 +321,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                     sc[nb][j] = exp2_fast(sc[nb][j] - from);
                     sc[nb][j + 2] = exp2_fast(sc[nb][j + 2] - from);
                 }
-                // (half-precision parts: weights times 2^15, which the end takes off; a key at 2^-24 of the maximum has 16 bits left)
-                constexpr float UP = QP == 2 ? 32768.0f : 1.0f;
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     split_pair<BF, QP>(sc[nb][2 * j] * UP, sc[nb][2 * j + 1] * UP, pw[nb][j]);
@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                         }
                     }
                 }
-                constexpr float UP = QP == 2 ? 32768.0f : 1.0f;
                 for (int key = 0; key < CHUNK && key < left; key++) {
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
@@ -452,7 +451,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
         }
         // ---- what the warp has of the item. A lane has elements 64 v + 8 g + 2 i and the one behind it of rows 2 t and 2 t + 1
         const bool complete = c0 == 0 && c1 == sq.chunks;
-        constexpr float DOWN = QP == 2 ? 1.0f / 32768.0f : 1.0f;
+        constexpr float DOWN = 1.0f / UP, L_DOWN = QP == 1 ? DOWN : 1.0f;
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
@@ -461,6 +460,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 for (int o = 4; o < 32; o <<= 1) {
                     l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], o);
                 }
+                l[nb][j] *= L_DOWN;
                 const int r = nb * 8 + 2 * t + j;
                 if (row0 + r >= rows) {
                     continue;

@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 }
                 }
             };
-            constexpr float UP = QP == 2 ? 32768.0f : 1.0f;  // (half-precision parts of weights: times 2^15)
+            constexpr float UP = BF ? 1.0f : (QP == 2 ? 32768.0f : 128.0f);  // (half-precision weights, so that small ones keep their bits; where they may be 2^8, times 2^7)
             const float f = factor > 0.0f ? factor : 1.0f;
             for (int i = 0;; i++, n++) {
                 const int key0 = (it.c0 + i) * TILE_KEYS + half * KEYS;  // this thread's first

@@ -314,6 +314,22 @@ def test_a_few_large_weights_among_many_small_ones(act, cache):
     check_attention(t, q, 1, 1, 64, act, cache, scale=1.0)
 
 
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hd,rows,prefix", [(64, 1, 0), (128, 3, 100), (64, 40, 0), (128, 40, 100), (256, 1, 0)])
+def test_small_weights_keep_their_bits(act, cache, hd, rows, prefix):
+    """A key 16 above all others whose values are zero: the result is made of weights of 1.1e-7."""
+    t = Setup([rows], [1000], 1, hd, 16, cache, prefix=prefix, seed=24)
+    q = torch.zeros(rows, 2, hd, dtype=act)
+    q[:, :, 0] = 1.0
+    t.k[..., 0] = 0.0
+    t.v.abs_()
+    t.k[int(t.tables[0, 100 // 16]), 0, 100 % 16, 0] = 16.0
+    t.v[int(t.tables[0, 100 // 16]), 0, 100 % 16] = 0.0
+    t.cache.k.copy_(t.k)
+    t.cache.v.copy_(t.v)
+    check_attention(t, q, 2, 1, hd, act, cache, scale=1.0)
+
+
 @pytest.mark.parametrize("act,cache", [(F32, F16), (BF16, BF16)])
 def test_strides_orders_and_outputs(act, cache):
     t = Setup([1, 3, 2], [40, 50, 5], 2, 64, 16, cache, prefix=30, pad=2, seed=7)
