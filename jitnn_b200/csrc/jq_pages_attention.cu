@@ -138,9 +138,15 @@ inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t
     const double pairs = (double)kv_heads * (double)((rows + 127) / 128) * (double)((keys + 127) / 128);
     return (double)kv_heads * (double)rows * (double)keys * head_dim > 3e8 + parts * (head_dim == 64 ? 1.5e5 : 2e5) * pairs;
 }
-// Whether the stream kernel's blocks have 16 rows for the prefix's sake, although the sequences' own have up to 8. 64 heads of 128 on 8, FP32 rows on half precision, 16 sequences: 2048
-// keys 25 us with 16 and 28 with 8, 500 keys 16 and 16 (with 1000 own keys a sequence 23 and 21); 16 rows of each of 32 key/value heads, FP32 pages, 2048 keys 48 and 42.
-inline bool blocks_of_sixteen(int head_dim, int64_t kv_heads, int64_t rows, int64_t keys) { return rows >= 96 && (double)kv_heads * (double)rows * (double)keys * head_dim > 2.4e8; }
+// Rows of the stream kernel's blocks. Heads of 128, 16 sequences, bf16: 16 own rows against 1000 keys 21 us with 16 and 22 with 8, 32 rows 28 and 30. Heads of 64, half precision, where more and shorter
+// items are worth a second reading of the keys: 16 rows 17.4 and 15.5, 32 rows 20.5 and 20.1 (FP32 34 and 37), 20 rows against 200 keys 13 and 11, but behind 1023 keys 32 and 37.
+// For a prefix even where own rows are up to 8: 64 heads of 128 on 8, FP32 rows on half precision, 16 sequences: 2048 keys 25 us with 16 and 28 with 8, 500 keys 16 and 16 (with 1000 own
+// keys a sequence 23 and 21); 16 rows of each of 32 key/value heads, FP32 pages, 2048 keys 48 and 42. 16 rows of heads of 256 do not fit the registers.
+inline int stream_rows(int head_dim, int64_t own, int64_t kv_heads, int64_t shared, int64_t prefix) {
+    const double products = (double)kv_heads * (double)shared * (double)prefix * head_dim;
+    const bool sixteen = own > 8 ? head_dim == 128 || own >= 32 || products > 1e8 : shared >= 96 && products > 2.4e8;
+    return head_dim <= 128 && sixteen ? 16 : 8;
+}
 // What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
 // heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
@@ -166,7 +172,7 @@ Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t seq
         plan.tile_workers = (int)(!plan.tile_own && units < 148 * resident ? units : 148 * resident);
     }
     if (!plan.tile_own) {
-        plan.rows = hd <= 128 && (own > 8 || (plan.tile_workers == 0 && blocks_of_sixteen(hd, p->kv_heads, shared, prefix_length))) ? 16 : 8;
+        plan.rows = stream_rows(hd, own, p->kv_heads, shared, plan.tile_workers == 0 ? prefix_length : 0);
         plan.workers = 148 * stream_resident(hd, elem_bytes(p->elem), plan.rows) * pages::STREAM_WARPS;
     }
     // (an item that there are few of is cut into about as many pieces as there are workers for each; of the prefix's the length is known)
