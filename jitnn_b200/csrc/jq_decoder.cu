@@ -2702,6 +2702,19 @@ static int forward_pages(jq_decoder* d, const char* who, const int32_t* tokens_h
             return fail(JQ_ERR_INVALID, "%s: layer %d linear %d is not set", who, (int)(i / 7), (int)(i % 7));
         }
     }
+    int64_t need_bytes = 0;  // (nearly always there already: a shorter prefix may take other kernels)
+    rc = jq_pages_attention_bytes(d->paged[0], JQ_ELEM_F32, d->heads, total, n_seqs, prefix_length, &need_bytes);
+    if (rc != JQ_OK) {
+        return rc;
+    }
+    if (need_bytes > d->paged_space_bytes) {
+        JQ_CUDA(cudaDeviceSynchronize());
+        cudaFree(d->paged_space);
+        d->paged_space = nullptr;
+        d->paged_space_bytes = 0;
+        JQ_CUDA(cudaMalloc(&d->paged_space, need_bytes));
+        d->paged_space_bytes = need_bytes;
+    }
     // (out of pageable memory: staged before the call returns)
     JQ_CUDA(cudaMemcpyAsync(d->paged_meta, meta.data(), meta.size() * sizeof(int32_t), cudaMemcpyHostToDevice, s));
     TokenArgs ta;
@@ -2760,7 +2773,7 @@ JQ_API int jq_decoder_verify_pages(jq_decoder* d, const int32_t* tokens_host, in
         return rc;
     }
     if (drafts < 0 || n_seqs < 1 || drafts >= MAX_TOKENS || n_seqs > MAX_TOKENS || n_seqs * (drafts + 1) > MAX_TOKENS || accepted_host == nullptr || next_host == nullptr ||
-        tokens_host == nullptr || !(temperature >= 0.0) || !std::isfinite(temperature) || (temperature > 0.0 && uniforms == nullptr)) {
+        tokens_host == nullptr || !(temperature == 0.0 || (temperature >= 1e-300 && temperature <= 1e30)) || (temperature > 0.0 && uniforms == nullptr)) {
         return fail(JQ_ERR_INVALID, "jq_decoder_verify_pages: %d sequences with %d drafts (at most %d tokens in all), temperature %g", n_seqs, drafts, MAX_TOKENS, temperature);
     }
     const DeviceGuard guard(d->device);

@@ -312,7 +312,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
         return fail(JQ_ERR_INVALID, "jq_pages_attention: %s queries on %s pages (FP32 queries, or the pages' type)", elem_name(elem), elem_name(p->elem));
     }
     if (heads > 65535 || q == nullptr || out == nullptr || strides == nullptr || tokens > 0x7fffffff || table_width > 0x7fffffff || prefix_length > 0x7fffffff ||
-        !std::isfinite(scale)) {
+        !std::isfinite(scale * 1.5f)) {  // (times log2 e)
         return fail(JQ_ERR_INVALID, "jq_pages_attention: %lld rows of %d query heads, scale %g", (long long)tokens, heads, scale);
     }
     if (prefix_length > 0 && (prefix == nullptr || prefix_width * p->page_size < prefix_length)) {

@@ -157,6 +157,8 @@ def test_refusals():
         dec.verify_pages([[1, 2]], [[0]], [2], temperature=1.0)
     with pytest.raises(ValueError, match="temperature -1"):
         dec.verify_pages([[1, 2]], [[0]], [2], temperature=-1.0)
+    with pytest.raises(ValueError, match="temperature 1e"):
+        dec.verify_pages([[1, 2]], [[0]], [2], uniforms=[[0.5, 0.5]], temperature=1e31)
     with pytest.raises(ValueError, match="uniforms of shape"):
         dec.verify_pages([[1, 2]], [[0]], [2], uniforms=[[0.5]], temperature=1.0)
     with pytest.raises(ValueError, match="outside the vocabulary"):

@@ -201,6 +201,15 @@ def test_what_is_read_later_is_not_copied():
             PagedBatch(**args)
 
 
+def test_scales_that_are_no_numbers_are_refused():
+    pages, batch, rope, q, k, v = made()
+    for scale in (float("nan"), float("inf"), 1e39, 3e38):
+        with pytest.raises(ValueError, match="scale"):
+            pages.attention(q, batch, scale=scale)
+        with Slow(), pytest.raises(ValueError, match="scale"):
+            pages.attention(q, batch, scale=scale)
+
+
 def test_two_rows_for_one_place():
     """Two sequences on the same pages: where both write, either's key may stand, whole."""
     pages, _, _, q, k, v = made()
