@@ -47,6 +47,8 @@ __device__ __forceinline__ void store_run(Out* to, const Run<In, V>& from) {
 template <typename T, typename C, int V, bool INTERLEAVED, int ITEMS>
 __global__ void __launch_bounds__(256, V == 1 ? 1 : 4) append_kernel(AppendArgs a) {
     __shared__ int found[2];  // sequence and own position
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched programmatically
+    asm volatile("griddepcontrol.launch_dependents;");
     const int row = blockIdx.x, u = threadIdx.x, lanes = blockDim.y, tid = threadIdx.y * blockDim.x + u, threads = blockDim.x * lanes;
     if (tid == 0) {
         found[0] = -1;
@@ -140,7 +142,7 @@ template <typename T, typename C, int V, bool INTERLEAVED>
 void launch_append(const AppendArgs& a, cudaStream_t s) {
     constexpr int ITEMS = 4;
     const HeadGrid g(a.head_dim, V, a.heads + 2 * a.kv_heads, ITEMS);
-    append_kernel<T, C, V, INTERLEAVED, ITEMS><<<dim3((unsigned)a.b.tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), 0, s>>>(a);
+    launch_behind(append_kernel<T, C, V, INTERLEAVED, ITEMS>, dim3((unsigned)a.b.tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), s, a);
 }
 
 template <typename T, typename C>

@@ -212,15 +212,15 @@ int large_smem(K kernel, int smem, std::atomic<uint64_t>& configured) {  // the 
     return JQ_OK;
 }
 
-// Behind a kernel of this call (`behind`): programmatically, all of this call's kernels but the joining one work at the same time.
+// Programmatically: the first kernel waits at its beginning for what is in front of the call, all of this call's kernels but the joining one work at the same time.
 template <typename K, typename... More>
-int launch_part(K kernel, dim3 grid, int threads, int smem, bool behind, cudaStream_t s, const AttendArgs& a, const More&... more) {
+int launch_part(K kernel, dim3 grid, int threads, int smem, cudaStream_t s, const AttendArgs& a, const More&... more) {
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = behind ? 1 : 0;
+    cfg.numAttrs = 1;
     cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
@@ -236,7 +236,7 @@ int launch_stream(const AttendArgs& a, const Plan& plan, cudaStream_t s) {
     constexpr int smem = pages::Stream<T, C, HD, NB>::SMEM;
     auto kernel = pages::attend_stream_kernel<T, C, HD, NB, stream_resident(HD, sizeof(C), 8 * NB)>;
     const int rc = smem > 48 * 1024 ? large_smem(kernel, smem, configured) : JQ_OK;
-    return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, plan.tile_workers > 0, s, a);
+    return rc != JQ_OK ? rc : launch_part(kernel, dim3((unsigned)(plan.workers / pages::STREAM_WARPS)), pages::STREAM_THREADS, smem, s, a);
 }
 
 template <typename T, typename C, int HD>
@@ -247,7 +247,7 @@ int launch_attend_head(const jq_pages* p, const AttendArgs& a, const Plan& plan,
             static std::atomic<uint64_t> configured{0};
             constexpr int smem = pages::Tile<T, C, HD>::SMEM;
             rc = large_smem(pages::attend_tile_kernel<T, C, HD>, smem, configured);
-            rc = rc != JQ_OK ? rc : launch_part(pages::attend_tile_kernel<T, C, HD>, dim3((unsigned)plan.tile_workers), pages::TILE_THREADS, smem, false, s, a, p->k_map, p->v_map);
+            rc = rc != JQ_OK ? rc : launch_part(pages::attend_tile_kernel<T, C, HD>, dim3((unsigned)plan.tile_workers), pages::TILE_THREADS, smem, s, a, p->k_map, p->v_map);
         }
     }
     if (rc == JQ_OK && plan.rows == 8) {
@@ -262,9 +262,9 @@ int launch_attend_head(const jq_pages* p, const AttendArgs& a, const Plan& plan,
         return rc;
     }
     if (plan.warp_a_row) {
-        return launch_part(pages::attend_join_kernel<T, HD, 1>, dim3((unsigned)a.b.tokens, (unsigned)(a.heads + pages::JOIN_WARPS - 1) / pages::JOIN_WARPS), pages::JOIN_THREADS, 0, true, s, a);
+        return launch_part(pages::attend_join_kernel<T, HD, 1>, dim3((unsigned)a.b.tokens, (unsigned)(a.heads + pages::JOIN_WARPS - 1) / pages::JOIN_WARPS), pages::JOIN_THREADS, 0, s, a);
     }
-    return launch_part(pages::attend_join_kernel<T, HD, pages::JOIN_WARPS>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, true, s, a);
+    return launch_part(pages::attend_join_kernel<T, HD, pages::JOIN_WARPS>, dim3((unsigned)a.b.tokens, (unsigned)a.heads), pages::JOIN_THREADS, 0, s, a);
 }
 
 template <typename T, typename C>
@@ -349,6 +349,7 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
     a.whole = reinterpret_cast<float*>(space + plan.whole);
     a.whole_ml = reinterpret_cast<float2*>(space + plan.whole_ml);
     a.joined = prefix_length > 0 ? 1 : 0;
+    a.stream_first = plan.tile_workers == 0 ? 1 : 0;
     a.found = reinterpret_cast<int2*>(space + plan.found);
     a.scale = scale;
     a.fill = fill != 0;

@@ -37,6 +37,7 @@ struct AttendArgs {
     int joined;        // whether they are
     int2* found;       // for every row and head, of its own keys and of the prefix: the first worker that has some of them, and how many have (256 times that, and the row's
                        // place in its block); the worker of the item's first unit says it. [2][token][head]
+    int stream_first;  // whether no tile kernel is in front of the stream kernel
     long long wait_clocks;
 };
 

@@ -22,6 +22,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
     T* const out = static_cast<T*>(a.out) + (int64_t)token * a.ot + h * a.oh;
     const bool real = token >= a.b.starts[0] && token < a.b.starts[a.b.sequences];
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     if (!real) {
         for (int d = 32 * warp + lane; d < HD && a.fill; d += 32 * WARPS) {
             out[d] = from_float<T>(0.0f);

@@ -65,6 +65,9 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
     // Half-precision weights are times 2^15, which the end takes off: one at 2^-29 of the largest has all its bits, where it would be one of the type's smallest, or none, at 2^-24
     constexpr float UP = BF ? 1.0f : 32768.0f;
     extern __shared__ __align__(16) uint8_t all_smem[];
+    if (a.stream_first) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // for whatever is in front of this call
+    }
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* const smem = all_smem + warp * S::Q_BYTES;
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
             }
         }
     }
-    // (behind the tile kernel: what waits for this kernel has waited for that one)
+    // (behind the tile kernel, beside which this one works: what waits for this kernel has waited for that one)
     asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 

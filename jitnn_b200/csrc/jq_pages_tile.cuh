@@ -187,6 +187,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     __shared__ uint32_t bad_keys[2][4];
     __shared__ float tops[2][2][TILE_BLOCK], sums[TILE_BLOCK];  // of either half
     __shared__ int64_t row_q[TILE_BLOCK], row_out[TILE_BLOCK];  // where a row's queries are, and its results go; -1: there is no such row
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for whatever is in front of this call
     asm volatile("griddepcontrol.launch_dependents;");
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Work& work = a.pre;

@@ -45,6 +45,8 @@ struct RopeArgs {
 // Measured: 4096 tokens of 64 + 8 heads of 128, bf16, 28.0 us, 5.4 TB/s (82 % of a copy's); one token of 32 + 32, FP32, 2.9 us, the time of a launch.
 template <typename T, int V, bool INTERLEAVED, int ITEMS>
 __global__ void __launch_bounds__(256, V == 1 ? 1 : 4) rope_kernel(RopeArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched programmatically
+    asm volatile("griddepcontrol.launch_dependents;");
     const int pair_units = a.half / V, u = threadIdx.x, lanes = blockDim.y;
     const uint32_t token = blockIdx.x, b = token / (uint32_t)a.seq, t = token - b * (uint32_t)a.seq;
     const int heads = a.t[0].heads + a.t[1].heads;
@@ -110,7 +112,7 @@ template <typename T, int V, bool INTERLEAVED>
 void launch_rope(const RopeArgs& a, int64_t tokens, cudaStream_t s) {
     constexpr int ITEMS = 4;
     const HeadGrid g(a.head_dim, V, a.t[0].heads + a.t[1].heads, ITEMS);
-    rope_kernel<T, V, INTERLEAVED, ITEMS><<<dim3((unsigned)tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), 0, s>>>(a);
+    launch_behind(rope_kernel<T, V, INTERLEAVED, ITEMS>, dim3((unsigned)tokens, (unsigned)g.blocks), dim3((unsigned)g.units, (unsigned)g.lanes), s, a);
 }
 
 template <typename T>

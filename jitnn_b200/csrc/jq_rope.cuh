@@ -122,6 +122,22 @@ struct Turns {
     }
 };
 
+// A kernel that waits for the one in front by itself (griddepcontrol.wait) and so may be scheduled while that one ends; check_launch says how it went.
+template <typename Args>
+inline void launch_behind(void (*kernel)(Args), dim3 grid, dim3 block, cudaStream_t s, const Args& args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = s;
+    cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+
 // How a row's heads are laid on thread blocks: `units` threads a head (2 V elements each), `lanes` heads beside one another, ITEMS of them one after the other a thread.
 struct HeadGrid {
     int units, lanes, blocks;

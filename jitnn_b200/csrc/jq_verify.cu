@@ -16,7 +16,7 @@
 
 #include <cmath>
 
-#include "jq_pages.cuh"
+#include "jq_rope.cuh"
 
 namespace jq {
 namespace {
@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(STATS_THREADS, STATS_RESIDENT) stats_kernel(Ve
     __shared__ double sums[STATS_THREADS / 32];
     __shared__ float tops[STATS_THREADS / 32];
     __shared__ int ats[STATS_THREADS / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched programmatically
     asm volatile("griddepcontrol.launch_dependents;");
     const int row = blockIdx.y, b = row / (a.drafts_most + 1), i = row % (a.drafts_most + 1), tid = threadIdx.x, lane = tid & 31;
     if (i > count_of(a, b)) {
@@ -266,6 +267,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     }
     const Exponential exponential(a, lane);
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     const int count = count_of(a, b);
     const T* const target = static_cast<const T*>(a.target) + b * a.tb;
     __syncthreads();
@@ -481,7 +483,7 @@ template <typename T, int FORM>
 int launch_verify(const VerifyArgs& a, cudaStream_t s) {
     const int64_t rows = (int64_t)a.sequences * (a.drafts_most + 1);
     if constexpr (FORM != PROBABILITIES) {
-        stats_kernel<T, FORM == LOGITS><<<dim3((unsigned)a.chunks, (unsigned)rows), STATS_THREADS, 0, s>>>(a);
+        launch_behind(stats_kernel<T, FORM == LOGITS>, dim3((unsigned)a.chunks, (unsigned)rows), dim3(STATS_THREADS), s, a);
         count_launch();
         const int rc = check_launch("stats_kernel");
         if (rc != JQ_OK) {
@@ -498,7 +500,7 @@ int launch_verify(const VerifyArgs& a, cudaStream_t s) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = FORM == PROBABILITIES ? 1 : 2;  // behind the statistics programmatically
+    cfg.numAttrs = 2;
     cfg.gridDim = dim3((unsigned)(a.sequences * blocks));
     cfg.blockDim = dim3(CHOOSE_THREADS);
     cfg.stream = s;

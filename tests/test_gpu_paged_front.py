@@ -187,6 +187,50 @@ def test_a_generation_step_in_a_graph_beside_another():
     assert device_status(0) == 0
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_kernels_in_front_and_on_other_streams(captured):
+    """Calls behind kernels that make their inputs, row after row of them, and behind two streams at once; what comes behind them sees their results."""
+    pages, batch, rope, q, k, v = made(act=F16, cache=F16)
+    fixed = [q * (i + 1) for i in range(6)]
+    want = [pages.attention(rope.rotate(x, 3), batch) for x in fixed]
+    u, drafts = torch.rand(3, 2, device="cuda"), torch.zeros(3, 1, dtype=I32, device="cuda")
+    logits = torch.randn(3, 2, 40000, device="cuda")
+    tokens = Speculative.verify(logits * 2, drafts, u, temperature=1.0)[1]
+    side, buffer, lengths = torch.cuda.Stream(), torch.empty_like(q), batch.lengths.clone()
+    torch.cuda.synchronize()
+
+    def run():
+        got, here = [], torch.cuda.current_stream()
+        for x in fixed:
+            side.wait_stream(here)
+            with torch.cuda.stream(side):
+                batch.lengths.zero_()
+                batch.lengths.add_(lengths)
+            buffer.fill_(7.0)
+            buffer.copy_(x)
+            turned = rope.rotate(buffer, 3)
+            here.wait_stream(side)
+            got.append(pages.attention(turned, batch) * 1)
+            batch.lengths.zero_()
+            batch.lengths.add_(lengths)
+            got.append(pages.attention(rope.rotate(buffer, 3), batch))
+            got.append(Speculative.verify(logits + logits, drafts, u, temperature=1.0)[1] + 0)
+        return got
+
+    if captured:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = run()
+        for _ in range(20):
+            g.replay()
+    else:
+        for _ in range(20):
+            got = run()
+    torch.cuda.synchronize()
+    for i in range(6):
+        assert torch.equal(got[3 * i], want[i]) and torch.equal(got[3 * i + 1], want[i]) and torch.equal(got[3 * i + 2], tokens)
+
+
 def test_what_is_read_later_is_not_copied():
     """A batch's numbers are read when the kernels run: changed in place they count, and tensors that would have to be copied are refused."""
     pages, batch, rope, q, k, v = made()
