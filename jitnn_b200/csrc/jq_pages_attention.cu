@@ -132,8 +132,8 @@ constexpr int stream_resident(int head_dim, int bytes, int rows) { return head_d
 // a prefix of 2048 keys, which the tile kernel takes along, 20 rows 46 and 36, 32 rows 50 and 38.
 inline bool tile_takes_own(int head_dim, int parts, int64_t rows, int64_t prefix) { return rows > (head_dim == 64 ? 64 : (parts == 1 && prefix > 0 ? 16 : 32)); }
 // The prefix by its products: here their number counts, there the pairs of 128 rows and 128 keys (with 2 and 3 parts of FP32 rows twice and three times as dear), and what its
-// launch costs. 8 key/value heads of 128, bf16, up to 100 keys a sequence: 128 rows against 2048 keys 26 us here and 23 there, against 4096 40 and 26, 384 against 1024 37 and 28 (with up to
-// 1000 keys, which the two kernels read one after the other, 49 and 53); 32 key/value heads, 16 rows against 4096 30 and 38; heads of 64, 192 rows against 1024 19 and 22, against 8192 65 and 33.
+// launch costs. 8 key/value heads of 128, bf16, up to 100 own keys a sequence: 128 rows against 2048 keys 24 us here and 23 there, against 4096 32 and 26, 384 against 1024 31 and 27 (with up to
+// 1000 own keys 47 and 43); 32 key/value heads, 16 rows against 4096 30 and 36; heads of 64, 192 rows against 1024 19 and 21, against 2048 26 and 24.
 inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t rows, int64_t keys) {
     const double pairs = (double)kv_heads * (double)((rows + 127) / 128) * (double)((keys + 127) / 128);
     return (double)kv_heads * (double)rows * (double)keys * head_dim > 3e8 + parts * (head_dim == 64 ? 1.5e5 : 2e5) * pairs;
