@@ -282,6 +282,27 @@ print("the same")
 """ % (ROOT, ROOT + "/tests")
 
 
-def test_the_first_call_of_a_process_in_a_capture():
-    done = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300)
+FIRST_STEP = """
+import sys; sys.path[:0] = [%r, %r]
+import torch
+from jitnn_b200 import PagedBatch, PagedCache, Rope
+whole = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+for hd, tokens in ((64, 1), (128, 40)):
+    k, v = (torch.randn(20, 1, 16, hd, device="cuda").half() for _ in range(2))
+    pages, rope = PagedCache(20, 16, 1, hd, dtype="F16", k=k, v=v), Rope(400, hd)
+    batch = PagedBatch(torch.arange(10, device="cuda", dtype=torch.int32).view(1, 10), whole(0, tokens), whole(100), prefix=torch.arange(10, 20, device="cuda", dtype=torch.int32), prefix_length=150)
+    q, n = torch.randn(tokens, 4, hd, device="cuda").half(), torch.randn(tokens, 1, hd, device="cuda").half()
+    step = lambda: pages.attention(pages.append(rope.rotate(q, 0), n, n, batch, rope=rope), batch)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    assert torch.equal(got, step()) and torch.isfinite(got).all()
+print("the same")
+""" % (ROOT, ROOT + "/tests")
+
+
+@pytest.mark.parametrize("program", [FIRST, FIRST_STEP], ids=["verification", "step"])
+def test_the_first_call_of_a_process_in_a_capture(program):
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "the same" in done.stdout, done.stderr[-2000:]
