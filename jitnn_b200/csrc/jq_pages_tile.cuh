@@ -223,6 +223,11 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     Item it;
     // (a wait that gives up sets the abort flag, on which all others end too: every role goes on to its end without waiting or issuing anything)
     auto wait = [&](uint32_t b, uint32_t parity, int code) { return tc::mbar_wait(b, parity, abort_flag, a.status, code, a.wait_clocks); };
+    // Where the page of a key of an item is, in the pages' rows of heads; -1 where the cache does not have it (rows that nobody waits for any more go on with whatever stands in the flags of missing keys)
+    auto page_row = [&](const int* table, int key, int kvh) -> int64_t {
+        const int page = table[key >> a.page_shift];
+        return page >= 0 && page < a.pages ? (int64_t)page * a.kv_heads + kvh : -1;
+    };
 
     uint32_t tmem = 0;
     auto begin_products = [&] {  // everybody: the barriers are made, and the columns allocated
@@ -398,20 +403,14 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             }
             ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
         }
-        // copies that nobody has waited for are waited for here (with a limit): they write to this thread block's memory
-        if (!ok && lane == 0) {
-            const long long t0 = clock64();
-            for (int values = 0; values < 2; values++) {
-                const int stages = values ? VS : KS, upto = values ? values_brought : keys_brought;
-                for (int i = upto > stages ? upto - stages : 0; i < upto; i++) {
-                    while (!tc::mbar_try((values ? v_full : k_full) + 8 * (i % stages), (i / stages) & 1) && clock64() - t0 < a.wait_clocks) {
-                    }
-                }
-            }
-        }
     } else {
         // ---- rows
         begin_products();
+        auto wait_warp = [&](uint32_t b, uint32_t parity, int code) {  // (warp-wide instructions come next)
+            const bool got = wait(b, parity, code);
+            __syncwarp();
+            return got;
+        };
         const int half = warp >> 2, row = tid & (TILE_BLOCK - 1);
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);  // (a warp reaches 32 lanes, from lane 32 (warp % 4) on)
         constexpr int KEYS = TILE_KEYS / 2, DIMS = HD / 2;  // of a thread
@@ -419,9 +418,18 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         constexpr int CH = 16;  // scores that it holds at a time. (Loops are rolled up: a small call's instructions come from memory, 50 clocks each)
         const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(TILE_ROW_THREADS) : "memory"); };  // all of these warps
+        auto meet_any = [](bool mine) {  // the same, and whether one of them says so
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any)
+                         : "r"((uint32_t)mine), "n"(TILE_ROW_THREADS)
+                         : "memory");
+            return any != 0;
+        };
         int n = 0;
-        bool ok = true;
-        while (items.next(a, it)) {
+        // Where a thread has given up it goes on until the next tile's meeting, behind which all of them leave: what else it does on the way, its meetings too, goes by what everybody has
+        bool ok = true, given_up = false;
+        while (!given_up && items.next(a, it)) {
             const Sequence& sq = items.sq;
             const int r = it.row0 + row, tiles = it.c1 - it.c0, i_token = r / a.group, i_head = r - i_token * a.group;
             const bool real = r < it.rows, direct = it.complete && !a.joined, some = __any_sync(0xffffffffu, real);  // (a warp without rows only keeps the others company)
@@ -525,7 +533,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             }
             auto add_o = [&](int tile) {  // O of a tile to the sums
                 if constexpr (IN_REGISTERS) {
-                ok = wait(o_full, tile & 1, 17) && ok;
+                ok = wait_warp(o_full, tile & 1, 17) && ok;
                 tc::fence_after_sync();
 #pragma unroll
                 for (int h = 0; h < DIMS / CH; h++) {
@@ -565,7 +573,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     }
                 };
                 if (i < tiles) {
-                    ok = wait(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
+                    ok = wait_warp(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
                     tc::fence_after_sync();
                     gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3];
                     edge = key0 - half * KEYS + TILE_KEYS > least || gone != 0;
@@ -594,9 +602,9 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         for (int key = 0; key < KEYS; key++) {
                             float v = tile_ld1(scores + key);
                             const int j = key0 + key;
-                            if (v != v && real && j < limit && (gone >> (key / 16) & 1) == 0) {
-                                const C* const k = static_cast<const C*>(a.k_pages) +
-                                                   (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD;
+                            const int64_t page = v != v && real && j < limit && (gone >> (key / 16) & 1) == 0 ? page_row(table, j, it.kvh) : -1;
+                            if (page >= 0) {
+                                const C* const k = static_cast<const C*>(a.k_pages) + (page * a.page_size + (j & (a.page_size - 1))) * HD;
                                 const T* const q = static_cast<const T*>(a.q) + row_q[row];
                                 v = 0.0f;
 #pragma unroll 1
@@ -609,12 +617,15 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         tile_st_done();
                     }
                     tops[n & 1][half][row] = top;
-                    meet();
+                    given_up = meet_any(!ok);
+                    if (given_up) {
+                        break;
+                    }
                     top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 }
                 if constexpr (!IN_REGISTERS) {
                     if (i == tiles) {
-                        ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                        ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
                         tc::fence_after_sync();
                         break;
                     }
@@ -622,7 +633,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     const bool far = top > m + 8.0f;
                     const float shrink = far ? exp2_fast(m - top) : 1.0f;
                     if (i > 0 && __any_sync(0xffffffffu, far)) {
-                        ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                        ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
                         tc::fence_after_sync();
 #pragma unroll 1
                         for (int h = 0; h < DIMS / CH; h++) {
@@ -687,7 +698,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     // two threads look at a key's values
                     constexpr int PIECES = HD / 16;
                     const int st = n % VS, key = key0 - half * KEYS + row;
-                    ok = wait(v_full + 8 * st, (n / VS) & 1, 19) && ok;
+                    ok = wait_warp(v_full + 8 * st, (n / VS) & 1, 19) && ok;
                     const uint32_t at = v_s + st * L::KV + row * 128;
                     bool off = false;
 #pragma unroll 1
@@ -726,7 +737,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                             less = 1.0f;
                         } else {
                             if (i > 0) {
-                                ok = wait(o_full, (n - 1) & 1, 17) && ok;
+                                ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
                                 tc::fence_after_sync();
                             } else {  // the sums begin here
                                 const uint32_t none[16] = {};
@@ -751,8 +762,11 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                                 p += BF ? __uint_as_float(word << 16) : __half2float(__ushort_as_half((unsigned short)word));
                             }
                             const int j = key0 - half * KEYS + k;
-                            const C* const v = static_cast<const C*>(a.v_pages) +
-                                               (((int64_t)table[j >> a.page_shift] * a.kv_heads + it.kvh) * a.page_size + (j & (a.page_size - 1))) * HD + half * DIMS;
+                            const int64_t page = page_row(table, j, it.kvh);
+                            if (page < 0) {
+                                continue;
+                            }
+                            const C* const v = static_cast<const C*>(a.v_pages) + (page * a.page_size + (j & (a.page_size - 1))) * HD + half * DIMS;
                             if constexpr (IN_REGISTERS) {
                                 if (j < limit) {
 #pragma unroll
@@ -776,6 +790,9 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 tc::mbar_arrive(p_full);
             }
             tc::fence_before_sync();
+            if (given_up) {
+                break;
+            }
             // ---- what the thread block has of the item. Its warps' rows, some elements at a time, through the queries' memory (their products are done), so that they go out in lines
             if (half == 1) {
                 sums[row] = l;
@@ -837,6 +854,15 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         }
     }
     tc::fence_before_sync();
+    __syncthreads();
+    // Where some role has given up, copies and products may be under way that nobody has waited for: they write to this thread block's shared and tensor memory, and end long
+    // before this millisecond is over, which does not go by the limit that has just run out
+    if (*abort_flag != 0) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {
+            __nanosleep(1000);
+        }
+    }
     __syncthreads();
     if (warp == 0) {
         tc::fence_after_sync();
