@@ -416,7 +416,8 @@ JQ_API int jq_rope_apply(const jq_rope* r, int elem, int count, const void* cons
  *                     likewise (heads 0: no queries; rope NULL: no rotation). strides (elements): token and head of q, k, v, q_out. Rows are FP32, or of the pages' type.
  *                     q_out may be q. A position that the table of rotations does not have gives NaN queries, stores nothing and leaves status 97.
  * jq_pages_attention  out [tokens, heads, head_dim]: softmax(scale q . k) v over the prefix and the own keys up to the row's position; a row that sees no key, or only keys whose
- *                     scores are negative infinities, gives zeros.
+ *                     scores are negative infinities, gives zeros. Infinite and NaN values of keys that a row sees make of its elements what the formula says (times a weight that
+ *                     is zero in 32 bits an infinity is NaN); those of other keys do not reach it.
  *                     strides: token and head of q and out. heads is a multiple of kv_heads, which neighbouring heads share. prefix has prefix_width pages.
  *                     workspace: jq_pages_attention_bytes of device memory at a 256-byte aligned address.
  */

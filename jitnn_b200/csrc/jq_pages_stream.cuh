@@ -167,15 +167,6 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
         least = limit_of(0);
         float acc[NB][2 * KB][4];  // O^T: HD / 16 blocks of 16 elements x 8 rows
         float m[NB][2], l[NB][2];
-#pragma unroll
-        for (int nb = 0; nb < NB; nb++) {
-#pragma unroll
-            for (int i = 0; i < 2 * KB; i++) {
-                acc[nb][i][0] = acc[nb][i][1] = acc[nb][i][2] = acc[nb][i][3] = 0.0f;
-            }
-            m[nb][0] = m[nb][1] = -INFINITY;
-            l[nb][0] = l[nb][1] = 0.0f;
-        }
         // ---- the warp's chunks
         constexpr int KH = S::AHEAD ? KB : 1, VH = S::AHEAD ? VB : 1;
         uint4 kr[KH][2][W], vr[VH][4][W];
@@ -213,243 +204,272 @@ __global__ void __launch_bounds__(STREAM_THREADS, RESIDENT) attend_stream_kernel
                 }
             }
         };
-        int c = c0;
-        int page = page_of(c), page_next = page_of(c + 1);
-        int64_t at = rows_at(c, page);
-        if (S::AHEAD && c < c1) {
-            load_k(at, sq.keys - c * CHUNK, 0);
-        }
-        for (; c < c1; c++) {
-            const int left = sq.keys - c * CHUNK;  // keys from here on
-            if constexpr (S::AHEAD) {
-                load_v(at, left, 0);
-            }
-            float sc[NB][4], small[NB][4];  // products of the first parts, and all others
+        // The parts of a number, of weights, of FP32 values, make something else of an infinite value than the number does (a part of zero times infinity is none). Where sums are not
+        // finite in the end, all of it once more, looking at the values of every chunk
+#pragma unroll 1
+        for (int turn = 0; turn < 2; turn++) {
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) {
-                sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.0f;
-                small[nb][0] = small[nb][1] = small[nb][2] = small[nb][3] = 0.0f;
-            }
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                uint32_t x[4][KP], y[4][KP];
-                if constexpr (!S::AHEAD) {
-                    load_k(at, left, kb);
+                for (int i = 0; i < 2 * KB; i++) {
+                    acc[nb][i][0] = acc[nb][i][1] = acc[nb][i][2] = acc[nb][i][3] = 0.0f;
                 }
-                parts_of_run<KP, W, BF>(kr[S::AHEAD ? kb : 0][0], x);
-                parts_of_run<KP, W, BF>(kr[S::AHEAD ? kb : 0][1], y);
+                m[nb][0] = m[nb][1] = -INFINITY;
+                l[nb][0] = l[nb][1] = 0.0f;
+            }
+            int c = c0;
+            int page = page_of(c), page_next = page_of(c + 1);
+            int64_t at = rows_at(c, page);
+            if (S::AHEAD && c < c1) {
+                load_k(at, sq.keys - c * CHUNK, 0);
+            }
+            for (; c < c1; c++) {
+                const int left = sq.keys - c * CHUNK;  // keys from here on
+                if constexpr (S::AHEAD) {
+                    load_v(at, left, 0);
+                }
+                float sc[NB][4], small[NB][4];  // products of the first parts, and all others
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
-#pragma unroll
-                    for (int p = QP - 1; p >= 0; p--) {
-                        const uint4 q = load_shared16(smem + (((kb * QP + p) * NB + nb) * 32 + lane) * 16);
-#pragma unroll
-                        for (int i = KP - 1; i >= 0; i--) {
-                            if (i + p < PRODUCTS) {
-                                mma<BF>(i + p > 0 ? small[nb] : sc[nb], x[0][i], y[0][i], x[1][i], y[1][i], q.x, q.y);
-                                mma<BF>(i + p > 0 ? small[nb] : sc[nb], x[2][i], y[2][i], x[3][i], y[3][i], q.z, q.w);
-                            }
-                        }
-                    }
-                }
-            }
-            const int64_t at_now = at;
-            if (at_now < 0 && left > 0) {
-                note_status(a.status, STATUS_PAGE);
-            }
-            page = page_next;
-            page_next = page_of(c + 2);
-            at = rows_at(c + 1, page);
-            if (S::AHEAD && c + 1 < c1) {
-                load_k(at, left - CHUNK, 0);
-            }
-            const bool edge = c * CHUNK + CHUNK > least || at_now < 0;  // some row does not see all of the chunk
-            // ---- scores that are not numbers: in parts an infinity is infinity - infinity too. They are worked out again, one product after the other
-            bool odd = false;
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (PRODUCTS > 1) {
-                        sc[nb][i] += small[nb][i];
-                    }
-                    sc[nb][i] *= factor[nb][i & 1];
-                    odd = odd || sc[nb][i] != sc[nb][i];
-                }
-            }
-            if (__any_sync(0xffffffffu, odd)) {
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = row0 + nb * 8 + 2 * t + (i & 1), key = g + 8 * (i >> 1);
-                        if (sc[nb][i] != sc[nb][i]) {
-                            float sum = 0.0f;
-                            if (r < rows && key < left && at_now >= 0) {
-                                const T* x = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + r / a.group) * a.qt + (int64_t)(kvh * a.group + r % a.group) * a.qh;
-                                for (int d = 0; d < HD; d++) {
-                                    sum = fmaf(to_float(x[d]), to_float(k_pages[at_now + key * HD + d]), sum);
-                                }
-                            }
-                            sc[nb][i] = sum * to_log2;
-                        }
-                    }
-                }
-            }
-            // ---- running maximum and weights; a row's keys are in the eight lanes of one t
-            uint32_t pw[NB][2][QP];
-            float less[NB][2];  // what the sums so far are multiplied with
-#pragma unroll
-            for (int nb = 0; nb < NB; nb++) {
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (c * CHUNK + g + 8 * (i >> 1) >= limit[nb][i & 1] || at_now < 0) {
-                            sc[nb][i] = -INFINITY;
-                        }
-                    }
-                }
-                float top[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    top[j] = fmaxf(sc[nb][j], sc[nb][j + 2]);
-                    top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 4));
-                    top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
-                    top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
-                    top[j] = fmaxf(top[j], m[nb][j]);
-                    const float from = top[j] == -INFINITY ? 0.0f : top[j], shrink = exp2_fast(m[nb][j] - from);
-                    m[nb][j] = top[j];
-                    l[nb][j] *= shrink;
-                    less[nb][j] = shrink;
-                    sc[nb][j] = exp2_fast(sc[nb][j] - from);
-                    sc[nb][j + 2] = exp2_fast(sc[nb][j + 2] - from);
+                    sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.0f;
+                    small[nb][0] = small[nb][1] = small[nb][2] = small[nb][3] = 0.0f;
                 }
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    split_pair<BF, QP>(sc[nb][2 * j] * UP, sc[nb][2 * j + 1] * UP, pw[nb][j]);
-                    if constexpr (QP == 1) {
-                        if constexpr (BF) {
-                            l[nb][0] += __uint_as_float(pw[nb][j][0] << 16);
-                            l[nb][1] += __uint_as_float(pw[nb][j][0] & 0xffff0000u);
-                        } else {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pw[nb][j][0]));
-                            l[nb][0] += f.x;
-                            l[nb][1] += f.y;
-                        }
-                    } else {
-                        l[nb][0] += sc[nb][2 * j];
-                        l[nb][1] += sc[nb][2 * j + 1];
-                    }
-                }
-            }
-            // ---- values. Where some row does not see a key whose value is not finite, its weight of zero would still make a NaN: then only the rows that see it add it
-            bool bad = false;
-            if (edge) {
-#pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
+                for (int kb = 0; kb < KB; kb++) {
+                    uint32_t x[4][KP], y[4][KP];
                     if constexpr (!S::AHEAD) {
-                        load_v(at_now, left, vb);
+                        load_k(at, left, kb);
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-#pragma unroll
-                        for (int w = 0; w < W; w++) {
-                            bad = bad || not_finite<W>(vr[S::AHEAD ? vb : 0][j][w], BF);
-                        }
-                    }
-                }
-                bad = __any_sync(0xffffffffu, bad);
-            }
-            if (bad) {
-#pragma unroll
-                for (int nb = 0; nb < NB; nb++) {
-#pragma unroll
-                    for (int i = 0; i < 2 * KB; i++) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            acc[nb][i][j] *= less[nb][j & 1];
-                        }
-                    }
-                }
-                for (int key = 0; key < CHUNK && key < left; key++) {
+                    parts_of_run<KP, W, BF>(kr[S::AHEAD ? kb : 0][0], x);
+                    parts_of_run<KP, W, BF>(kr[S::AHEAD ? kb : 0][1], y);
 #pragma unroll
                     for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            const float lo = __shfl_sync(0xffffffffu, sc[nb][j], (key & 7) * 4 + t), hi = __shfl_sync(0xffffffffu, sc[nb][j + 2], (key & 7) * 4 + t);
-                            const float p = (key < 8 ? lo : hi) * UP;
-                            if (c * CHUNK + key < limit[nb][j]) {
+                        for (int p = QP - 1; p >= 0; p--) {
+                            const uint4 q = load_shared16(smem + (((kb * QP + p) * NB + nb) * 32 + lane) * 16);
 #pragma unroll
-                                for (int i = 0; i < 2 * KB; i++) {
-                                    const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
-                                    acc[nb][i][j] = fmaf(p, to_float(v_pages[at_now + key * HD + d]), acc[nb][i][j]);
-                                    acc[nb][i][j + 2] = fmaf(p, to_float(v_pages[at_now + key * HD + d + 1]), acc[nb][i][j + 2]);
+                            for (int i = KP - 1; i >= 0; i--) {
+                                if (i + p < PRODUCTS) {
+                                    mma<BF>(i + p > 0 ? small[nb] : sc[nb], x[0][i], y[0][i], x[1][i], y[1][i], q.x, q.y);
+                                    mma<BF>(i + p > 0 ? small[nb] : sc[nb], x[2][i], y[2][i], x[3][i], y[3][i], q.z, q.w);
                                 }
                             }
                         }
                     }
                 }
-            } else {
-                uint32_t pt[NB][2][QP];
+                const int64_t at_now = at;
+                if (at_now < 0 && left > 0) {
+                    note_status(a.status, STATUS_PAGE);
+                }
+                page = page_next;
+                page_next = page_of(c + 2);
+                at = rows_at(c + 1, page);
+                if (S::AHEAD && c + 1 < c1) {
+                    load_k(at, left - CHUNK, 0);
+                }
+                const bool edge = c * CHUNK + CHUNK > least || at_now < 0;  // some row does not see all of the chunk
+                // ---- scores that are not numbers: in parts an infinity is infinity - infinity too. They are worked out again, one product after the other
+                bool odd = false;
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++) {
 #pragma unroll
-                    for (int p = 0; p < QP; p++) {
-                        pt[nb][0][p] = transpose8(pw[nb][0][p]);
-                        pt[nb][1][p] = transpose8(pw[nb][1][p]);
+                    for (int i = 0; i < 4; i++) {
+                        if constexpr (PRODUCTS > 1) {
+                            sc[nb][i] += small[nb][i];
+                        }
+                        sc[nb][i] *= factor[nb][i & 1];
+                        odd = odd || sc[nb][i] != sc[nb][i];
                     }
                 }
+                if (__any_sync(0xffffffffu, odd)) {
 #pragma unroll
-                for (int vb = 0; vb < VB; vb++) {
-                    if constexpr (!S::AHEAD) {
-                        load_v(at_now, left, vb);
+                    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int r = row0 + nb * 8 + 2 * t + (i & 1), key = g + 8 * (i >> 1);
+                            if (sc[nb][i] != sc[nb][i]) {
+                                float sum = 0.0f;
+                                if (r < rows && key < left && at_now >= 0) {
+                                    const T* x = static_cast<const T*>(a.q) + (int64_t)(sq.row0 + r / a.group) * a.qt + (int64_t)(kvh * a.group + r % a.group) * a.qh;
+                                    for (int d = 0; d < HD; d++) {
+                                        sum = fmaf(to_float(x[d]), to_float(k_pages[at_now + key * HD + d]), sum);
+                                    }
+                                }
+                                sc[nb][i] = sum * to_log2;
+                            }
+                        }
+                    }
+                }
+                // ---- running maximum and weights; a row's keys are in the eight lanes of one t
+                uint32_t pw[NB][2][QP];
+                float less[NB][2];  // what the sums so far are multiplied with
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) {
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (c * CHUNK + g + 8 * (i >> 1) >= limit[nb][i & 1] || at_now < 0) {
+                                sc[nb][i] = -INFINITY;
+                            }
+                        }
+                    }
+                    float top[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        top[j] = fmaxf(sc[nb][j], sc[nb][j + 2]);
+                        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 4));
+                        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 8));
+                        top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 16));
+                        top[j] = fmaxf(top[j], m[nb][j]);
+                        const float from = top[j] == -INFINITY ? 0.0f : top[j], shrink = exp2_fast(m[nb][j] - from);
+                        m[nb][j] = top[j];
+                        l[nb][j] *= shrink;
+                        less[nb][j] = shrink;
+                        sc[nb][j] = exp2_fast(sc[nb][j] - from);
+                        sc[nb][j + 2] = exp2_fast(sc[nb][j + 2] - from);
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {  // elements 8 g + 2 i and 8 g + 2 i + 1 of four keys: rows g and g + 8 of the operand
-                        uint32_t x0[KP], x1[KP], x2[KP], x3[KP];
-                        if constexpr (W == 1) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const uint4& v = vr[S::AHEAD ? vb : 0][j][0];
-                                w[j] = i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
+                    for (int j = 0; j < 2; j++) {
+                        split_pair<BF, QP>(sc[nb][2 * j] * UP, sc[nb][2 * j + 1] * UP, pw[nb][j]);
+                        if constexpr (QP == 1) {
+                            if constexpr (BF) {
+                                l[nb][0] += __uint_as_float(pw[nb][j][0] << 16);
+                                l[nb][1] += __uint_as_float(pw[nb][j][0] & 0xffff0000u);
+                            } else {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&pw[nb][j][0]));
+                                l[nb][0] += f.x;
+                                l[nb][1] += f.y;
                             }
-                            x0[0] = __byte_perm(w[0], w[1], 0x5410);
-                            x1[0] = __byte_perm(w[0], w[1], 0x7632);
-                            x2[0] = __byte_perm(w[2], w[3], 0x5410);
-                            x3[0] = __byte_perm(w[2], w[3], 0x7632);
                         } else {
-                            float e[4], o[4];
+                            l[nb][0] += sc[nb][2 * j];
+                            l[nb][1] += sc[nb][2 * j + 1];
+                        }
+                    }
+                }
+                // ---- values. Where some row does not see a key whose value is not finite, its weight of zero would still make a NaN: then only the rows that see it add it
+                bool bad = false;
+                if (edge || turn > 0) {
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                const uint4& v = vr[S::AHEAD ? vb : 0][j][i >> 1];
-                                e[j] = __uint_as_float((i & 1) == 0 ? v.x : v.z);
-                                o[j] = __uint_as_float((i & 1) == 0 ? v.y : v.w);
-                            }
-                            split_pair<BF, KP>(e[0], e[1], x0);
-                            split_pair<BF, KP>(o[0], o[1], x1);
-                            split_pair<BF, KP>(e[2], e[3], x2);
-                            split_pair<BF, KP>(o[2], o[3], x3);
+                    for (int vb = 0; vb < VB; vb++) {
+                        if constexpr (!S::AHEAD) {
+                            load_v(at_now, left, vb);
                         }
 #pragma unroll
+                        for (int j = 0; j < 4; j++) {
+#pragma unroll
+                            for (int w = 0; w < W; w++) {
+                                bad = bad || not_finite<W>(vr[S::AHEAD ? vb : 0][j][w], BF);
+                            }
+                        }
+                    }
+                    bad = __any_sync(0xffffffffu, bad);
+                }
+                if (bad) {
+#pragma unroll
+                    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+                        for (int i = 0; i < 2 * KB; i++) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                acc[nb][i][j] *= less[nb][j & 1];
+                            }
+                        }
+                    }
+                    for (int key = 0; key < CHUNK && key < left; key++) {
+#pragma unroll
                         for (int nb = 0; nb < NB; nb++) {
-                            float chunk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int p = QP - 1; p >= 0; p--) {
+                            for (int j = 0; j < 2; j++) {
+                                const float lo = __shfl_sync(0xffffffffu, sc[nb][j], (key & 7) * 4 + t), hi = __shfl_sync(0xffffffffu, sc[nb][j + 2], (key & 7) * 4 + t);
+                                const float p = (key < 8 ? lo : hi) * UP;
+                                if (c * CHUNK + key < limit[nb][j]) {
 #pragma unroll
-                                for (int n = KP - 1; n >= 0; n--) {
-                                    if (n + p < PRODUCTS) {
-                                        mma<BF>(chunk, x0[n], x1[n], x2[n], x3[n], pt[nb][0][p], pt[nb][1][p]);
+                                    for (int i = 0; i < 2 * KB; i++) {
+                                        const int d = (i >> 2) * 64 + g * 8 + (i & 3) * 2;
+                                        acc[nb][i][j] = fmaf(p, to_float(v_pages[at_now + key * HD + d]), acc[nb][i][j]);
+                                        acc[nb][i][j + 2] = fmaf(p, to_float(v_pages[at_now + key * HD + d + 1]), acc[nb][i][j + 2]);
                                     }
                                 }
                             }
+                        }
+                    }
+                } else {
+                    uint32_t pt[NB][2][QP];
 #pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                acc[nb][vb * 4 + i][j] = fmaf(acc[nb][vb * 4 + i][j], less[nb][j & 1], chunk[j]);
+                    for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+                        for (int p = 0; p < QP; p++) {
+                            pt[nb][0][p] = transpose8(pw[nb][0][p]);
+                            pt[nb][1][p] = transpose8(pw[nb][1][p]);
+                        }
+                    }
+#pragma unroll
+                    for (int vb = 0; vb < VB; vb++) {
+                        if constexpr (!S::AHEAD) {
+                            load_v(at_now, left, vb);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {  // elements 8 g + 2 i and 8 g + 2 i + 1 of four keys: rows g and g + 8 of the operand
+                            uint32_t x0[KP], x1[KP], x2[KP], x3[KP];
+                            if constexpr (W == 1) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    const uint4& v = vr[S::AHEAD ? vb : 0][j][0];
+                                    w[j] = i == 0 ? v.x : (i == 1 ? v.y : (i == 2 ? v.z : v.w));
+                                }
+                                x0[0] = __byte_perm(w[0], w[1], 0x5410);
+                                x1[0] = __byte_perm(w[0], w[1], 0x7632);
+                                x2[0] = __byte_perm(w[2], w[3], 0x5410);
+                                x3[0] = __byte_perm(w[2], w[3], 0x7632);
+                            } else {
+                                float e[4], o[4];
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    const uint4& v = vr[S::AHEAD ? vb : 0][j][i >> 1];
+                                    e[j] = __uint_as_float((i & 1) == 0 ? v.x : v.z);
+                                    o[j] = __uint_as_float((i & 1) == 0 ? v.y : v.w);
+                                }
+                                split_pair<BF, KP>(e[0], e[1], x0);
+                                split_pair<BF, KP>(o[0], o[1], x1);
+                                split_pair<BF, KP>(e[2], e[3], x2);
+                                split_pair<BF, KP>(o[2], o[3], x3);
+                            }
+#pragma unroll
+                            for (int nb = 0; nb < NB; nb++) {
+                                float chunk[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                for (int p = QP - 1; p >= 0; p--) {
+#pragma unroll
+                                    for (int n = KP - 1; n >= 0; n--) {
+                                        if (n + p < PRODUCTS) {
+                                            mma<BF>(chunk, x0[n], x1[n], x2[n], x3[n], pt[nb][0][p], pt[nb][1][p]);
+                                        }
+                                    }
+                                }
+#pragma unroll
+                                for (int j = 0; j < 4; j++) {
+                                    acc[nb][vb * 4 + i][j] = fmaf(acc[nb][vb * 4 + i][j], less[nb][j & 1], chunk[j]);
+                                }
                             }
                         }
                     }
                 }
+            }
+            float probe[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+#pragma unroll
+                for (int i = 0; i < 2 * KB; i++) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        probe[j] = fmaf(acc[nb][i][j], 0.0f, probe[j]);
+                    }
+                }
+            }
+            const float odd_sums = (probe[0] + probe[1]) + (probe[2] + probe[3]);
+            if (!__any_sync(0xffffffffu, odd_sums != odd_sums)) {
+                break;
             }
         }
         // ---- what the warp has of the item. A lane has elements 64 v + 8 g + 2 i and the one behind it of rows 2 t and 2 t + 1

@@ -12,7 +12,7 @@
 // two parts, the scores two buffers, so that the next tile's are made meanwhile.
 //
 // A row that does not see a key must not get anything of it, and 0 x NaN is one: in tiles that not every row sees whole, values that are not finite, and those behind the last key,
-// are cleared in shared memory, and the rows that do see such a key add it by themselves.
+// are cleared in shared memory, and the rows that do see such a key add it by themselves. Sums that are not finite in the end are worked out once more from the values that are not.
 //
 // Bound per tile and SM: the products' 1024 clocks at head size 128 (times the parts), the threads' 128 exponentials (1024 clocks at 16 a clock) and about 700 instructions a
 // warp, or 2800 clocks for 64 KB of pages where they come from memory. Measured, all launches of a call: 280 tokens of 32 heads of 128 on 8 behind 7182 keys, FP16, 81 us, 407 TFLOP/s; 48 tokens of
@@ -792,6 +792,83 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             tc::fence_before_sync();
             if (given_up) {
                 break;
+            }
+            // ---- sums that are not finite. The parts of a weight, or one that is zero in 16 bits, make something else of an infinite value than the weight does: all elements that
+            // some key has a value for that is not finite, once more from those keys alone. (A warp's rows go through the item's keys together.)
+            {
+                float probe = 0.0f;
+                if constexpr (IN_REGISTERS) {
+#pragma unroll
+                    for (int i = 0; i < DIMS; i++) {
+                        probe = fmaf(acc[i], 0.0f, probe);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int h = 0; h < DIMS / CH; h++) {
+                        float o[CH];
+                        tile_ld<CH>(o, mine + L::O_AT + half * DIMS + CH * h);
+                        tile_ld_done();
+#pragma unroll
+                        for (int i = 0; i < CH; i++) {
+                            probe = fmaf(o[i], 0.0f, probe);
+                        }
+                    }
+                }
+                if (__any_sync(0xffffffffu, real && probe != probe)) {
+                    const int* const table = it.prefix ? a.b.prefix : a.b.tables + it.s * a.b.table_stride;
+                    const int behind = (int64_t)it.c1 * TILE_KEYS < sq.keys ? it.c1 * TILE_KEYS : sq.keys;
+                    uint64_t begun = 0;  // elements of this row that have such a value
+#pragma unroll 1
+                    for (int j = it.c0 * TILE_KEYS; j < behind; j++) {
+                        const int64_t page = page_row(table, j, it.kvh);
+                        if (page < 0) {
+                            continue;
+                        }
+                        const int64_t at = (page * a.page_size + (j & (a.page_size - 1))) * HD;
+                        const C* const v = static_cast<const C*>(a.v_pages) + at + half * DIMS;
+                        uint64_t bad = 0;
+#pragma unroll 1
+                        for (int d = 0; d < DIMS; d += 8) {
+                            if (not_finite<1>(*reinterpret_cast<const uint4*>(v + d), BF)) {
+#pragma unroll 1
+                                for (int i = d; i < d + 8; i++) {
+                                    bad |= (uint64_t)(!isfinite(to_float(v[i]))) << i;
+                                }
+                            }
+                        }
+                        if (bad == 0) {
+                            continue;
+                        }
+                        float p = 0.0f;
+                        if (real && j < limit) {
+                            const C* const k = static_cast<const C*>(a.k_pages) + at;
+                            const T* const q = static_cast<const T*>(a.q) + row_q[row];
+#pragma unroll 1
+                            for (int d = 0; d < HD; d++) {
+                                p = fmaf(to_float(q[d]), to_float(k[d]), p);
+                            }
+                            p = exp2_fast(fmaf(p, a.scale * 1.4426950408889634f, m == -INFINITY ? 0.0f : -m)) * UP;
+                        }
+                        auto sum_of = [&](float sum, int d) {
+                            const float more = p * to_float(v[d]);
+                            return (bad >> d & 1) == 0 || !real || j >= limit ? sum : ((begun >> d & 1) == 0 ? more : sum + more);
+                        };
+                        if constexpr (IN_REGISTERS) {
+#pragma unroll
+                            for (int d = 0; d < DIMS; d++) {
+                                acc[d] = sum_of(acc[d], d);
+                            }
+                        } else {
+#pragma unroll 1
+                            for (int d = 0; d < DIMS; d++) {
+                                const uint32_t o = mine + L::O_AT + half * DIMS + d;
+                                tile_st1(o, sum_of(tile_ld1(o), d));
+                            }
+                            tile_st_done();
+                        }
+                        begun |= real && j < limit ? bad : 0;
+                    }
+                }
             }
             // ---- what the thread block has of the item. Its warps' rows, some elements at a time, through the queries' memory (their products are done), so that they go out in lines
             if (half == 1) {
