@@ -184,6 +184,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
     __shared__ __align__(8) uint64_t bars[2 * (KS + VS) + 5];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word, gone_ring[4], o_begun;  // o_begun: an item's sums have been begun by the rows
+    __shared__ int gone_on[2];  // of this tile and the last: a row's thread has given up and goes on
     __shared__ uint32_t bad_keys[2][4];
     __shared__ float tops[2][2][TILE_BLOCK], sums[TILE_BLOCK];  // of either half
     __shared__ int64_t row_q[TILE_BLOCK], row_out[TILE_BLOCK];  // where a row's queries are, and its results go; -1: there is no such row
@@ -213,7 +214,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             tc::mbar_init(bar(i), i == REST + 2 || i == REST + 4 ? TILE_ROW_THREADS : 1);
         }
         abort_word = 0;
-        o_begun = 0;
+        o_begun = gone_on[0] = gone_on[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -407,7 +408,8 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         // ---- rows
         begin_products();
         auto wait_warp = [&](uint32_t b, uint32_t parity, int code) {  // (warp-wide instructions come next)
-            const bool got = wait(b, parity, code);
+            uint32_t got = wait(b, parity, code) ? 1u : 0u;
+            asm volatile("" : "+r"(got));  // (no copy of what follows for each answer: 10 % of a prefix's time with three parts)
             __syncwarp();
             return got;
         };
@@ -418,18 +420,11 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
         constexpr int CH = 16;  // scores that it holds at a time. (Loops are rolled up: a small call's instructions come from memory, 50 clocks each)
         const bool wide = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && (a.qt * (int)sizeof(T)) % 16 == 0 && (a.qh * (int)sizeof(T)) % 16 == 0;
         auto meet = [] { asm volatile("bar.sync 1, %0;" ::"n"(TILE_ROW_THREADS) : "memory"); };  // all of these warps
-        auto meet_any = [](bool mine) {  // the same, and whether one of them says so
-            uint32_t any;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                         : "=r"(any)
-                         : "r"((uint32_t)mine), "n"(TILE_ROW_THREADS)
-                         : "memory");
-            return any != 0;
-        };
         int n = 0;
-        // Where a thread has given up it goes on until the next tile's meeting, behind which all of them leave: what else it does on the way, its meetings too, goes by what everybody has
-        bool ok = true, given_up = false;
-        while (!given_up && items.next(a, it)) {
+        // A thread that has given up goes on to the end with whatever is there. What it meets the others for goes by what all of them have: not by the flags of missing keys, which may be
+        // written while it reads them, so that it tells the others first
+        uint32_t ok = 1;
+        while (items.next(a, it)) {
             const Sequence& sq = items.sq;
             const int r = it.row0 + row, tiles = it.c1 - it.c0, i_token = r / a.group, i_head = r - i_token * a.group;
             const bool real = r < it.rows, direct = it.complete && !a.joined, some = __any_sync(0xffffffffu, real);  // (a warp without rows only keeps the others company)
@@ -533,7 +528,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
             }
             auto add_o = [&](int tile) {  // O of a tile to the sums
                 if constexpr (IN_REGISTERS) {
-                ok = wait_warp(o_full, tile & 1, 17) && ok;
+                ok &= wait_warp(o_full, tile & 1, 17);
                 tc::fence_after_sync();
 #pragma unroll
                 for (int h = 0; h < DIMS / CH; h++) {
@@ -573,7 +568,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     }
                 };
                 if (i < tiles) {
-                    ok = wait_warp(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18) && ok;
+                    ok &= wait_warp(s_full + 8 * (n % L::BUFS), (n / L::BUFS) & 1, 18);
                     tc::fence_after_sync();
                     gone = reinterpret_cast<volatile int*>(gone_ring)[n & 3];
                     edge = key0 - half * KEYS + TILE_KEYS > least || gone != 0;
@@ -617,15 +612,15 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         tile_st_done();
                     }
                     tops[n & 1][half][row] = top;
-                    given_up = meet_any(!ok);
-                    if (given_up) {
-                        break;
+                    if (ok == 0) {
+                        gone_on[n & 1] = 1;
                     }
+                    meet();
                     top = fmaxf(fmaxf(top, tops[n & 1][half ^ 1][row]) * f, m);
                 }
                 if constexpr (!IN_REGISTERS) {
                     if (i == tiles) {
-                        ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
+                        ok &= wait_warp(o_full, (n - 1) & 1, 17);
                         tc::fence_after_sync();
                         break;
                     }
@@ -633,7 +628,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                     const bool far = top > m + 8.0f;
                     const float shrink = far ? exp2_fast(m - top) : 1.0f;
                     if (i > 0 && __any_sync(0xffffffffu, far)) {
-                        ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
+                        ok &= wait_warp(o_full, (n - 1) & 1, 17);
                         tc::fence_after_sync();
 #pragma unroll 1
                         for (int h = 0; h < DIMS / CH; h++) {
@@ -694,11 +689,11 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 }
                 l = fmaf(l, less, sum0 + sum1);
                 tile_st_done();
-                if (edge) {
+                if (edge && reinterpret_cast<volatile int*>(gone_on)[n & 1] == 0) {  // (the same for all: nobody writes this one before all have met again)
                     // two threads look at a key's values
                     constexpr int PIECES = HD / 16;
                     const int st = n % VS, key = key0 - half * KEYS + row;
-                    ok = wait_warp(v_full + 8 * st, (n / VS) & 1, 19) && ok;
+                    ok &= wait_warp(v_full + 8 * st, (n / VS) & 1, 19);
                     const uint32_t at = v_s + st * L::KV + row * 128;
                     bool off = false;
 #pragma unroll 1
@@ -737,7 +732,7 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                             less = 1.0f;
                         } else {
                             if (i > 0) {
-                                ok = wait_warp(o_full, (n - 1) & 1, 17) && ok;
+                                ok &= wait_warp(o_full, (n - 1) & 1, 17);
                                 tc::fence_after_sync();
                             } else {  // the sums begin here
                                 const uint32_t none[16] = {};
@@ -790,9 +785,6 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 tc::mbar_arrive(p_full);
             }
             tc::fence_before_sync();
-            if (given_up) {
-                break;
-            }
             // ---- sums that are not finite. The parts of a weight, or one that is zero in 16 bits, make something else of an infinite value than the weight does: all elements that
             // some key has a value for that is not finite, once more from those keys alone. (A warp's rows go through the item's keys together.)
             {
