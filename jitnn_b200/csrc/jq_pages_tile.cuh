@@ -6,7 +6,7 @@
 // Warp 8 brings keys and values by tensor-map copies, a box for every page that a tile touches, and issues the products: S = Q K^T (tcgen05.mma,
 // 128 x 128, both operands in shared memory), O = P V (weights from tensor memory; values as they lie on the pages, elements of a head are the second operand's columns).
 // The instruction cuts off where it adds (a sum of 8192 keys held in it was 4e-6 off). For FP32 rows O only adds up a tile, and the threads add the tiles in registers with the factor of the
-// maximum; 16-bit rows, whose rounding is a thousand times that, leave the sums in tensor memory, and only a maximum that rises by more than 2^8 has them scaled.
+// maximum; 16-bit rows, whose rounding is a thousand times that, leave the sums in tensor memory, and only a maximum that rises (with bfloat16 by more than 2^8) has them scaled.
 // For 16-bit rows two thread blocks share an SM, one's products under the other's exponentials: weights take the place of the scores. FP32 rows are two half-precision
 // parts (with a power of two per row) or three bfloat16 parts, so many products for one, and weights likewise; their weights have columns of their own and, with
 // two parts, the scores two buffers, so that the next tile's are made meanwhile.
@@ -542,7 +542,9 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                 }
                 }
             };
-            constexpr float UP = BF ? 1.0f : (QP == 2 ? 32768.0f : 128.0f);  // (half-precision weights, so that small ones keep their bits; where they may be 2^8, times 2^7)
+            // Half-precision weights are times 2^15, as the stream kernel's: off by 2^-40 of the largest at most. So they may not be above one, where bfloat16 ones may be up to 2^8. (With 2^7
+            // and 2^8 a weight 20 below the largest was 10 % off; with 2^13 and 2^2 one 21 below 0.2 %. 280 tokens of 32 heads behind 7182 keys 87 us, with those 84 and 85.)
+            constexpr float UP = BF ? 1.0f : 32768.0f, LAG = BF ? 8.0f : 0.0f;
             const float f = factor > 0.0f ? factor : 1.0f;
             for (int i = 0;; i++, n++) {
                 const int key0 = (it.c0 + i) * TILE_KEYS + half * KEYS;  // this thread's first
@@ -624,8 +626,8 @@ __global__ void __launch_bounds__(TILE_THREADS, Tile<T, C, HD>::RESIDENT)
                         tc::fence_after_sync();
                         break;
                     }
-                    // The sums stay as they are, and weights may be up to 2^8, until a maximum is more than that above the one they go by (or is the first)
-                    const bool far = top > m + 8.0f;
+                    // The sums stay as they are, and weights may be up to 2^LAG, until a maximum is more than that above the one they go by (or is the first)
+                    const bool far = top > m + LAG;
                     const float shrink = far ? exp2_fast(m - top) : 1.0f;
                     if (i > 0 && __any_sync(0xffffffffu, far)) {
                         ok &= wait_warp(o_full, (n - 1) & 1, 17);

@@ -76,3 +76,23 @@ def test_an_infinite_value_alone(act, cache, hd, rows):
     t.cache.k[page, 0, slot, 0] = 500.0  # times 8 over at most 12: e^-333 for the others
     t.cache.v[page, 0, slot, 7], t.cache.v[page, 0, slot, 8] = math.inf, -math.inf
     assert check_classes(t, q, 1, hd, act, cache) == rows * 2 * 2
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hd,rows,prefix", [(64, [1], 0), (64, [70], 0), (128, [40], 0), (128, [40], 300), (64, [4] * 8, 8200), (128, [2] * 16, 4100)])
+@pytest.mark.parametrize("far", [16, 18, 20, 21])
+def test_weights_of_keys_far_below_the_largest(act, cache, hd, rows, prefix, far):
+    """A key that far above all others, whose value is zero: the result is made of weights down to 7.6e-10, by each kernel."""
+    t = Setup(rows, [max(900, n) for n in rows] if len(rows) == 1 else rows, 1, hd, 16, cache, prefix=prefix, seed=43)
+    heads = 2 if len(rows) == 1 else 32
+    q = torch.zeros(t.tokens, heads, hd, dtype=act)
+    q[:, :, 0] = 1.0
+    t.k[..., 0] = 0.0
+    t.v.abs_()
+    page, slot = (int(t.prefix[5]), 3) if prefix else (int(t.tables[0, 5]), 3)
+    t.k[page, 0, slot, 0] = float(far)
+    t.v[page, 0, slot] = 0.0
+    t.v.mul_(1000.0)  # (so that results are among the type's ordinary numbers)
+    t.cache.k.copy_(t.k)
+    t.cache.v.copy_(t.v)
+    check_attention(t, q, heads, 1, hd, act, cache, scale=1.0)
