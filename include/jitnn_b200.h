@@ -435,7 +435,8 @@ JQ_API int jq_pages_attention(const jq_pages* p, int elem, int heads, const void
 /*
  * Verification of drafted tokens (speculative sampling; the reference has no generation loop). target [sequences, drafts_most + 1, vocab] are the target's logits (`logits` non-zero, at
  * `temperature`) or probabilities behind each draft, draft_probs [sequences, drafts_most, vocab] FP32 the drafter's (NULL: all on the draft), drafts and counts (NULL:
- * drafts_most each) int32, uniforms FP32 [sequences, drafts_most + 1] numbers in [0, 1). Strides are elements; drafts and uniforms are contiguous.
+ * drafts_most each) int32, uniforms FP32 [sequences, drafts_most + 1] numbers in [0, 1) (a negative one counts as 0; one
+ * from 1 on, or NaN, draws the last token that has any weight). Strides are elements; drafts and uniforms are contiguous.
  * Draft i is kept while uniforms[i] q_i(x_i) < p_i(x_i); then one token comes by the inverse distribution function at uniforms[drafts_most]: behind the first refused draft j from
  * max(p_j - q_j, 0) over its sum (p_j where that is zero), behind the last draft from p. accepted[s] = the drafts kept, tokens [sequences, drafts_most + 1] = those, the
  * further token, and -1 in the rest. Temperature 0: the likeliest token (the first of equal ones) instead, uniforms and draft_probs are not read. No drafts at

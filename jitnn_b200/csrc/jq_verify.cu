@@ -256,7 +256,7 @@ __device__ __forceinline__ void join_chunks(const VerifyArgs& a, const Exponenti
 template <typename T, int FORM>
 __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     __shared__ double of_warp[2][CHOOSE_WARPS], upto[CLUSTER * CHOOSE_WARPS + 1];  // a warp's weight; the weight in front of each warp of the cluster
-    __shared__ int last_some;    // the last warp that has any weight
+    __shared__ int taken;        // the warp of the cluster that the token falls to: the last with any weight that begins at the aim or in front of it
     __shared__ double row_sum[CHOOSE_WARPS];  // of the last row that each warp has looked at, which one of them goes on with: p = exp((x - top) / temperature) / sum
     __shared__ float row_top[CHOOSE_WARPS];
     __shared__ int row_at[CHOOSE_WARPS], refused;
@@ -270,6 +270,11 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
     asm volatile("griddepcontrol.launch_dependents;");
     const int count = count_of(a, b);
     const T* const target = static_cast<const T*>(a.target) + b * a.tb;
+    auto uniform = [&](int i) {  // (a negative number is zero)
+        const double u = (double)a.u[(int64_t)b * rows + i];
+        return u < 0.0 ? 0.0 : u;
+    };
+    const double u_token = FORM == GREEDY ? 0.0 : uniform(a.drafts_most);
     __syncthreads();
     // ---- the first refused draft: every thread block finds it by itself, a warp a draft
     for (int i = warp; i <= count; i += CHOOSE_WARPS) {
@@ -300,7 +305,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
                 p = exponential.of<true>(t, top) / sum;
             }
             const double q = a.q != nullptr ? (double)a.q[b * a.qb + i * a.qr + x] : 1.0;
-            good = (double)a.u[(int64_t)b * rows + i] * q < p;
+            good = uniform(i) * q < p;
         }
         if (!good) {
             if (lane == 0) {
@@ -390,26 +395,27 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
             if (warp == 0) {
                 constexpr int N = CLUSTER * CHOOSE_WARPS / 32;  // (of smaller clusters the last have nothing)
                 double part[N], run = 0.0;
-                int last = -1;
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     const int w = lane * N + n;
                     part[n] = w < blocks * CHOOSE_WARPS ? *cluster.map_shared_rank(&of_warp[round][w % CHOOSE_WARPS], w / CHOOSE_WARPS) : 0.0;
                     run += part[n];
-                    last = part[n] > 0.0 ? w : last;
                 }
                 const double scan = warp_scan(run, lane);
                 double here = __shfl_up_sync(0xffffffffu, scan, 1);
                 here = lane == 0 ? 0.0 : here;
+                const double all = __shfl_sync(0xffffffffu, scan, 31), aim = u_token * all;
+                int last = -1;
 #pragma unroll
                 for (int n = 0; n < N; n++) {
                     upto[lane * N + n] = here;
+                    last = part[n] > 0.0 && (!(aim < all) || here <= aim) ? lane * N + n : last;
                     here += part[n];
                 }
                 last = __reduce_max_sync(0xffffffffu, last);
                 if (lane == 31) {
-                    upto[CLUSTER * CHOOSE_WARPS] = here;
-                    last_some = last;
+                    upto[CLUSTER * CHOOSE_WARPS] = all;
+                    taken = last;
                 }
             }
             __syncthreads();
@@ -422,8 +428,8 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
         }
         asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // nobody's sums go away while others read them
         // the warp whose run the aim falls into; with a uniform number of 1 or more, or none at all, the last that has any weight
-        const double aim = (double)a.u[(int64_t)b * rows + a.drafts_most] * total;
-        if (aim < total ? upto[me] <= aim && aim < upto[me + 1] : me == last_some) {
+        const double aim = u_token * total;
+        if (me == taken) {
             const double scan = warp_scan(mine, lane) + upto[me];
             const unsigned over = __ballot_sync(0xffffffffu, mine > 0.0 && scan > aim), some = __ballot_sync(0xffffffffu, mine > 0.0);
             const int chosen = over != 0u ? __ffs(over) - 1 : 31 - __clz(some);  // (not found by a rounding of the sums: the last with any weight)
@@ -444,7 +450,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) choose_kernel(VerifyArgs a) {
                 a.tokens[(int64_t)b * rows + j] = found >= 0 ? found : (positive >= 0 ? positive : a.vocab - 1);
             }
         }
-        if (rank == 0 && tid == 0 && last_some < 0) {
+        if (rank == 0 && tid == 0 && taken < 0) {
             a.tokens[(int64_t)b * rows + j] = a.vocab - 1;  // no weight anywhere
         }
         __syncwarp();
