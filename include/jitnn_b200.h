@@ -409,7 +409,8 @@ JQ_API int jq_rope_apply(const jq_rope* r, int elem, int count, const void* cons
  * appended, key i on page tables[s * table_stride + i / page_size]. In front of their own keys all sequences see the prefix_length keys on the pages prefix[0 ..].
  * A row's own position is lengths[s] - (starts[s + 1] - row); where that is negative the row has no keys of its own and none is stored. Rows outside
  * starts[0] .. starts[sequences] - 1 belong to no sequence: their outputs are left as they were, or become zero where `fill`. tables, starts, lengths and prefix are read on the device, at
- * every replay of a graph anew. A page id outside the cache, or a position outside the table of pages, is not touched (its keys are not seen, its rows not stored) and leaves status 96
+ * every replay of a graph anew. The keys of a table and a prefix together are at most
+ * 2^31 - 256. A page id outside the cache, or a position outside the table of pages, is not touched (its keys are not seen, its rows not stored) and leaves status 96
  * for jq_device_status. Where two rows of a call have the same page and slot, either is stored.
  *
  * jq_pages_append     k and v [tokens, kv_heads, head_dim] to their pages, k rotated at prefix_length + own position first, and q_out [tokens, heads, head_dim] = q rotated

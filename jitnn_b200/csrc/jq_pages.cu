@@ -168,8 +168,8 @@ int check_batch(const jq_pages* p, const Batch& b, const char* who) {
     if (b.tables == nullptr || b.starts == nullptr || b.lengths == nullptr || b.sequences < 1 || b.table_width < 1) {
         return fail(JQ_ERR_INVALID, "%s: %d sequences of %d pages", who, b.sequences, b.table_width);
     }
-    if (b.prefix_length < 0 || (int64_t)b.table_width * p->page_size + b.prefix_length > 0x7fffffff) {
-        return fail(JQ_ERR_INVALID, "%s: a prefix of %d keys and %d pages of %d: positions are below 2^31", who, b.prefix_length, b.table_width, p->page_size);
+    if (b.prefix_length < 0 || (int64_t)b.table_width * p->page_size + b.prefix_length > 0x7fffff00) {  // (a tile of keys behind the last still has a number)
+        return fail(JQ_ERR_INVALID, "%s: a prefix of %d keys and %d pages of %d: positions are below 2^31 - 256", who, b.prefix_length, b.table_width, p->page_size);
     }
     return JQ_OK;
 }

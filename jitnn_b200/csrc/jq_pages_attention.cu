@@ -42,11 +42,16 @@ __global__ void __launch_bounds__(128) attend_row_kernel(AttendArgs a) {
         }
         return;
     }
-    const int own = found[1] >= 0 ? found[1] + 1 : 0, keys = a.b.prefix_length + own;
+    // (a length beyond what the table of pages has is cut to that, as in the other kernels: prefix and table together have less than 2^31 - 256 keys)
+    const int64_t most = (int64_t)a.b.table_width * a.page_size;
+    const int own = found[1] < 0 ? 0 : (int)(found[1] < most ? found[1] + 1 : most), keys = a.b.prefix_length + own;
+    if (found[1] >= most && tid == 0) {
+        note_status(a.status, STATUS_PAGE);
+    }
     const C* const kp = static_cast<const C*>(a.k_pages);
     const C* const vp = static_cast<const C*>(a.v_pages);
     float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int j0 = 0; j0 < keys; j0 += 128) {
+    for (int j0 = 0; j0 < keys; j0 += 128) {  // (fewer than 2^31 - 256)
         const int j = j0 + tid;
         int64_t at = -1;
         if (j < keys) {
