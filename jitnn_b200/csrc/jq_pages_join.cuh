@@ -20,16 +20,19 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
         return;
     }
     T* const out = static_cast<T*>(a.out) + (int64_t)token * a.ot + h * a.oh;
-    const bool real = token >= a.b.starts[0] && token < a.b.starts[a.b.sequences];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    if (!real) {
+    // (asked for together; of a row of no sequence nobody has said anything, and nothing is made of it)
+    const bool one = a.joined == 0;
+    const int64_t mine_at = (int64_t)token * a.heads + h;
+    const int row_first = a.b.starts[0], row_end = a.b.starts[a.b.sequences];
+    const int2 said0 = a.found[mine_at], said1 = a.found[one ? mine_at : (int64_t)a.b.tokens * a.heads + mine_at];
+    if (token < row_first || token >= row_end) {
         for (int d = 32 * warp + lane; d < HD && a.fill; d += 32 * WARPS) {
             out[d] = from_float<T>(0.0f);
         }
         return;
     }
-    const bool one = a.joined == 0;
     // (where the starts are in no order nobody may have said anything: whatever stands there stays in range)
     auto in_range = [](int2 f, const Work& w, int& first, int& count, int& in_block) {
         first = f.x < 0 || f.x >= w.workers ? 0 : f.x;
@@ -37,14 +40,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(AttendArgs a)
         count = count < 1 ? 1 : (count > w.workers - first ? w.workers - first : count);
         in_block = f.y & ((1 << w.rows_shift) - 1);
     };
-    const int64_t mine_at = (int64_t)token * a.heads + h;
     int first0, count0, block0, first1 = 0, count1 = 0, block1 = 0;
-    in_range(a.found[mine_at], a.own, first0, count0, block0);
+    in_range(said0, a.own, first0, count0, block0);
     if (one && count0 == 1) {
         return;  // it is there already
     }
     if (!one) {
-        in_range(a.found[(int64_t)a.b.tokens * a.heads + mine_at], a.pre, first1, count1, block1);
+        in_range(said1, a.pre, first1, count1, block1);
     }
     float m = -INFINITY, l = 0.0f, acc[V];
 #pragma unroll
