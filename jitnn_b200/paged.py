@@ -160,9 +160,6 @@ class Rope:
         if len(xs) == 2 and all(t.numel() for t in xs) and (ys[0].data_ptr() in (ys[1].data_ptr(), xs[1].data_ptr()) or ys[1].data_ptr() == xs[0].data_ptr()):
             raise ValueError("%s: one tensor is the other's output" % what)
         batch, seq = (1,) + lead if len(lead) == 1 else lead
-        strides = (ctypes.c_int64 * (6 * len(xs)))()
-        for i, t in enumerate(v for p in zip(xs, ys) for v in p):
-            strides[3 * i: 3 * i + 3] = ((0,) if len(lead) == 1 else ()) + tuple(t.stride()[:-1])
         at, size, pb, pt, offset = None, 0, 0, 0, 0
         if isinstance(positions, torch.Tensor):
             if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in (lead, lead[-1:]):
@@ -174,9 +171,13 @@ class Rope:
         else:
             offset = int(positions)
         L = _lib.load()
-        vps = ctypes.c_void_p * len(xs)
-        if all(t.numel() for t in xs):
-            check(L.jq_rope_apply(h, code, len(xs), vps(*(t.data_ptr() for t in xs)), vps(*(t.data_ptr() for t in ys)), (ctypes.c_int * len(xs))(*(t.shape[-2] for t in xs)),
+        turned = [p for p in zip(xs, ys) if p[0].numel()]  # (queries without keys, or keys without queries, are rotated alone)
+        if turned:
+            n, vps = len(turned), ctypes.c_void_p * len(turned)
+            strides = (ctypes.c_int64 * (6 * n))()
+            for i, t in enumerate(v for p in turned for v in p):
+                strides[3 * i: 3 * i + 3] = ((0,) if len(lead) == 1 else ()) + tuple(t.stride()[:-1])
+            check(L.jq_rope_apply(h, code, n, vps(*(x.data_ptr() for x, _ in turned)), vps(*(y.data_ptr() for _, y in turned)), (ctypes.c_int * n)(*(x.shape[-2] for x, _ in turned)),
                                   hd, strides, batch, seq, at, size, pb, pt, offset, inverse, _raw_stream(torch, self.device)))
         return ys if pair else ys[0]
 
