@@ -1,4 +1,4 @@
-"""Paged attention where numbers are not ordinary: infinities and NaN that a row sees or does not, by each of its kernels."""
+"""Paged attention's numbers, by each of its kernels: infinities and NaN in values, keys and queries, weights far below the largest, and that rows of 32 bits keep them."""
 import math
 
 import pytest
@@ -96,3 +96,81 @@ def test_weights_of_keys_far_below_the_largest(act, cache, hd, rows, prefix, far
     t.cache.k.copy_(t.k)
     t.cache.v.copy_(t.v)
     check_attention(t, q, heads, 1, hd, act, cache, scale=1.0)
+
+
+def check_scores(t, q, kv, hd, act, cache):
+    """Keys that are not finite, as the formula has them: a score of minus infinity weighs nothing, one of infinity or NaN makes its row NaN; rows that do not see the key are what they were."""
+    got = t.cache.attention(q.cuda(), t.batch).cpu()
+    kinds = set()
+    for row, k, v in rows_of(t, q, hd):
+        heads, group = q.shape[1], q.shape[1] // kv
+        for h in range(heads):
+            keys = k[:, h // group].double()
+            s = (keys * q[row, h].double()).sum(-1) / math.sqrt(hd)
+            plain = torch.isfinite(keys).all(-1)
+            if torch.isnan(s).any() or (s == math.inf).any():
+                assert torch.isnan(got[row, h]).all(), "row %d, head %d" % (row, h)
+                kinds.add("nan")
+                continue
+            assert (s[~plain] == -math.inf).all()
+            kinds.add("zero" if not plain.all() else "plain")
+            want, size, score = oracle.attention(q[row, h: h + 1], k[plain][:, h // group: h // group + 1], v[plain][:, h // group: h // group + 1], 1 / math.sqrt(hd))
+            within(got[row, h: h + 1], want, oracle.attention_bound(want, size, score, hd, len(k), act, cache), "row %d, head %d" % (row, h))
+    no_status()
+    return kinds
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hd,rows,lengths,prefix", SHAPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("place", ["first", "newest"])
+def test_keys_that_are_not_finite(act, cache, hd, rows, lengths, prefix, bad, place):
+    """One element of a key: infinite scores have the sign of the query's element. Another key is minus infinity all over for one head, whose queries are positive."""
+    t = Setup(rows, lengths, 2, hd, 16, cache, prefix=prefix, seed=44)
+    q = normal(t.tokens, 8 if t.tokens > 8 else 4, hd, dtype=act, seed=44)
+    group = q.shape[1] // 2
+    q[:, :group] = q[:, :group].abs() + 0.25
+    own = 1 if place == "first" else lengths[0] - 1
+    t.cache.k[int(t.tables[0, own // 16]), 1, own % 16, 5] = bad
+    own = 2 if place == "first" else lengths[0] - 1
+    t.cache.k[int(t.tables[0, own // 16]), 0, own % 16] = -math.inf
+    kinds = check_scores(t, q, 2, hd, act, cache)
+    assert "zero" in kinds and ("nan" in kinds or (t.tokens < 9 and bad == bad))  # (few queries may all have the sign that makes minus infinity)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("hd,rows,lengths,prefix", SHAPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_not_finite(act, cache, hd, rows, lengths, prefix, bad):
+    """An element of one row's queries, or all of them: that row is NaN, the others are what they were to the bit."""
+    t = Setup(rows, lengths, 2, hd, 16, cache, prefix=prefix, seed=45)
+    q = normal(t.tokens, 8 if t.tokens > 8 else 4, hd, dtype=act, seed=45).cuda()
+    clean = t.cache.attention(q, t.batch)
+    row, other = 0, t.starts[1] - 1
+    q[row, 0], q[other, -1, 3] = bad, bad
+    got = t.cache.attention(q, t.batch)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    hit[row, 0] = hit[other, -1] = True
+    assert torch.isnan(got[hit]).all()
+    bits = torch.int32 if act is torch.float32 else torch.int16
+    assert torch.equal(got[~hit].view(bits), clean[~hit].view(bits))
+    no_status()
+
+
+@pytest.mark.parametrize("cache", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hd,rows,lengths,prefix", SHAPES + [(128, [1], [577], 0), (64, [200], [1100], 0), (128, [100], [600], 900)])
+def test_rows_of_32_bits_keep_them(cache, hd, rows, lengths, prefix):
+    """The root mean square of the error is at most 1e-6 of the results'. A weight is off by up to 2^-22 of itself as parts of 22 bits, by 2^-22 for its exponential, and by its score's error: hd
+    products exact to 2^-22 with random signs, 2^-22 of their root of squares, which is about 1 for normal numbers; sums and the quotient are rounded to 2^-24. Errors of different keys have no common
+    sign, so that of the result they make at most 2^-22 (1 + 1 + 1 + 1/2) = 8.3e-7. (Queries and keys as one half-precision number each, 3.3e-4, or queries as one bfloat16 number,
+    1.6e-3, are within attention_bound for many of these shapes.)"""
+    t = Setup(rows, lengths, 2, hd, 16, cache, prefix=prefix, seed=46)
+    q = normal(t.tokens, 8 if t.tokens > 8 else 4, hd, seed=46)
+    got = t.cache.attention(q.cuda(), t.batch).cpu().double()
+    off = size = 0.0
+    for row, k, v in rows_of(t, q, hd):
+        want = oracle.attention(q[row], k, v, 1 / math.sqrt(hd))[0]
+        off += float(((got[row] - want) ** 2).sum())
+        size += float((want ** 2).sum())
+    assert math.sqrt(off / size) <= 1e-6, math.sqrt(off / size)
+    no_status()
