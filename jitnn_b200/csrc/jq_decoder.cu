@@ -10,6 +10,8 @@
 
 #include <cmath>
 #include <cstring>
+#include <new>
+#include <utility>
 #include <vector>
 
 #include "jq_common.cuh"
@@ -1281,10 +1283,16 @@ static void free_pages(jq_decoder* d) {
     d->page_count = 0;
 }
 
-// cos / sin tables in double, stored as float (ops/Rope.java:84-101)
+// cos / sin tables in double, stored as float (ops/Rope.java:84-101). (One that is out of host memory leaves them as they are.)
 static cudaError_t fill_rope_tables(jq_decoder* d) {
     const int half = d->head_dim / 2;
-    std::vector<float> c((size_t)d->max_seq * half), s((size_t)d->max_seq * half);
+    std::vector<float> c, s;
+    try {
+        c.resize((size_t)d->max_seq * half);
+        s.resize((size_t)d->max_seq * half);
+    } catch (const std::bad_alloc&) {
+        return cudaErrorMemoryAllocation;
+    }
     for (int t = 0; t < d->max_seq; t++) {
         for (int i = 0; i < half; i++) {
             const double angle = t * d->rope_freqs[i];
@@ -1461,11 +1469,15 @@ JQ_API int jq_decoder_create(int device, int layers, int dim, int heads, int kv_
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&d->own_stream, cudaStreamNonBlocking);
     if (e == cudaSuccess && take_status_word(&d->status) != JQ_OK) e = cudaErrorMemoryAllocation;
     if (e == cudaSuccess) {
-        for (int i = 0; i < head_dim / 2; i++) {
-            d->rope_freqs.push_back(std::pow((double)rope_base, -2.0 * i / head_dim));
+        try {
+            for (int i = 0; i < head_dim / 2; i++) {
+                d->rope_freqs.push_back(std::pow((double)rope_base, -2.0 * i / head_dim));
+            }
+            d->rope_magnitude = 1.0;
+            e = fill_rope_tables(d);
+        } catch (const std::bad_alloc&) {
+            e = cudaErrorMemoryAllocation;
         }
-        d->rope_magnitude = 1.0;
-        e = fill_rope_tables(d);
     }
     if (prev >= 0) {
         cudaSetDevice(prev);
@@ -2553,6 +2565,11 @@ JQ_API int jq_decoder_set_rope(jq_decoder* d, const double* freqs, double magnit
     if (freqs == nullptr || !std::isfinite(magnitude)) {
         return fail(JQ_ERR_INVALID, "jq_decoder_set_rope: null frequencies, or magnitude %g", magnitude);
     }
+    for (int i = 0; i < d->head_dim / 2; i++) {
+        if (!std::isfinite(freqs[i])) {
+            return fail(JQ_ERR_INVALID, "jq_decoder_set_rope: frequency %d is %g", i, freqs[i]);
+        }
+    }
     const DeviceGuard guard(d->device);
     if (!guard.ok) {
         return fail(JQ_ERR_CUDA, "jq_decoder_set_rope: device %d", d->device);
@@ -2564,13 +2581,29 @@ JQ_API int jq_decoder_set_rope(jq_decoder* d, const double* freqs, double magnit
         if (rc != JQ_OK) {
             return rc;
         }
+    }
+    // both kinds of caches are rotated by the same frequencies, by the old ones where this fails
+    std::vector<double> before;
+    try {
+        before.assign(freqs, freqs + d->head_dim / 2);
+    } catch (const std::bad_alloc&) {
+        jq_rope_free(rope);
+        return fail(JQ_ERR_OOM, "jq_decoder_set_rope: out of host memory");
+    }
+    d->rope_freqs.swap(before);
+    std::swap(d->rope_magnitude, magnitude);
+    const cudaError_t e = fill_rope_tables(d);
+    if (e != cudaSuccess) {
+        d->rope_freqs.swap(before);
+        d->rope_magnitude = magnitude;
+        jq_rope_free(rope);
+        return cuda_fail(e, "jq_decoder_set_rope");
+    }
+    if (rope != nullptr) {
         jq_rope_free(d->rope);
         d->rope = rope;
     }
-    d->rope_freqs.assign(freqs, freqs + d->head_dim / 2);
-    d->rope_magnitude = magnitude;
-    const cudaError_t e = fill_rope_tables(d);
-    return e == cudaSuccess ? JQ_OK : cuda_fail(e, "jq_decoder_set_rope");
+    return JQ_OK;
 }
 
 JQ_API int jq_decoder_set_pages(jq_decoder* d, int elem, int pages, int page_size) {

@@ -194,6 +194,11 @@ JQ_API int jq_rope_create(int device, int64_t positions, int dim, const double* 
     if (positions < 1 || positions > (int64_t)1 << 24 || dim < 2 || dim % 2 != 0 || dim > 512 || freqs == nullptr || !std::isfinite(magnitude)) {
         return fail(JQ_ERR_INVALID, "jq_rope_create: %lld positions (1 to 2^24) of %d elements (an even number up to 512)", (long long)positions, dim);
     }
+    for (int i = 0; i < dim / 2; i++) {
+        if (!std::isfinite(freqs[i])) {
+            return fail(JQ_ERR_INVALID, "jq_rope_create: frequency %d is %g", i, freqs[i]);
+        }
+    }
     int count = 0;
     JQ_CUDA(cudaGetDeviceCount(&count));
     if (device < 0 || device >= count) {
