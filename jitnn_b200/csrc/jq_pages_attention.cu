@@ -132,13 +132,18 @@ struct Plan {
 constexpr int stream_resident(int head_dim, int bytes, int rows) { return head_dim * bytes >= 512 || head_dim * rows >= 2048 ? 2 : 3; }
 
 // Which kernel: the stream kernel reads the keys once for 8 or 16 rows, the tile kernel (16-bit pages, heads of 64 and 128) for 128, but takes 10 us to begin and end an item.
-// A sequence's own keys, whose number only the device knows, by its rows per key/value head; 8 of those, up to 1000 keys. 40 sequences, heads of 64, FP32 rows on half precision: 32 rows 36 us
-// here and 66 there, 80 rows 73 and 68; bf16 33 and 43, 64 and 51. Heads of 128, 16 sequences: 32 rows 30 and 44, 48 rows 40 and 44, 80 rows 55 and 45; bf16 28 and 32, 37 and 35, 50 and 36, but with
-// a prefix of 2048 keys, which the tile kernel takes along, 20 rows 46 and 36, 32 rows 50 and 38.
-inline bool tile_takes_own(int head_dim, int parts, int64_t rows, int64_t prefix) { return rows > (head_dim == 64 ? 64 : (parts == 1 && prefix > 0 ? 16 : 32)); }
+// A sequence's own keys, whose number only the device knows, by its rows per key/value head: of all sequences the average, so that a prompt beside many single tokens is read by the
+// kernel that suits neither best. 16 sequences of up to 700 keys, heads of 128, us here and there. bf16: 32 rows 24.4 and 27.7, 48 rows 30.0 and 29.0, 64 rows 34 and 30; behind 200 keys, which the tile
+// kernel takes along, 32 rows 29.9 and 30.9, 40 rows 33.9 and 32.3; behind 600 24 rows 31.6 and 31.7, 32 rows 36 and 32, behind 2048 16 rows 34 and 30, 24 rows 36 and 29.
+// FP32 on half precision: 48 rows 32 and 36, 64 rows 38 and 37, 96 rows 51 and 38; behind 200 keys 64 rows 50 and 49; behind 600 40 rows 46 and 47, 48 rows 52 and 48; behind 2048 24 rows 44 and 41, 40 rows
+// 55 and 48. Heads of 64 against 1000 keys: bf16 64 rows 28 and 30, FP32 64 rows 31 and 37, 80 rows 73 and 68 (40 sequences).
+inline bool tile_takes_own(int head_dim, int parts, int64_t rows, int64_t prefix) {
+    return rows > (head_dim == 64 ? 64 : (parts == 1 ? 32 : 64) >> (prefix >= 512 ? 1 : 0));
+}
 // The prefix by its products: here their number counts, there the pairs of 128 rows and 128 keys (with 2 and 3 parts of FP32 rows twice and three times as dear), and what its
-// launch costs. 8 key/value heads of 128, bf16, up to 100 own keys a sequence: 128 rows against 2048 keys 24 us here and 23 there, against 4096 32 and 26, 384 against 1024 31 and 27 (with up to
-// 1000 own keys 47 and 43); 32 key/value heads, 16 rows against 4096 30 and 36; heads of 64, 192 rows against 1024 19 and 21, against 2048 26 and 24.
+// launch costs. bf16, up to 100 own keys a sequence, us here and there: 8 key/value heads of 128, 128 rows against 2048 keys 24.3 and 23.3, against 4096 33 and 26, 192 rows against 1024 27.0 and 26.6,
+// against 2048 33 and 30; 32 key/value heads, 16 rows against 4096 30 and 37; heads of 64, 192 rows against 1024 20 and 22, against 2048 27 and 25, against 4096 31 and 27. Over 64 such shapes, half of them with
+// up to 1000 own keys, this takes 0.3 % longer than the better of both, with 1.5e8 in place of 3e8 0.6 % (FP32 rows on half precision 0.4 and 0.6, on bfloat16 0.3 and 0.1).
 inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t rows, int64_t keys) {
     const double pairs = (double)kv_heads * (double)((rows + 127) / 128) * (double)((keys + 127) / 128);
     return (double)kv_heads * (double)rows * (double)keys * head_dim > 3e8 + parts * (head_dim == 64 ? 1.5e5 : 2e5) * pairs;
