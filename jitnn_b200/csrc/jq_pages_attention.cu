@@ -150,19 +150,22 @@ inline bool tile_takes_prefix(int head_dim, int parts, int64_t kv_heads, int64_t
 }
 // Rows of the stream kernel's blocks. Heads of 128, 16 sequences, bf16: 16 own rows against 1000 keys 21 us with 16 and 22 with 8, 32 rows 28 and 30. Heads of 64, half precision, where more and shorter
 // items are worth a second reading of the keys: 16 rows 17.4 and 15.5, 32 rows 20.5 and 20.1 (FP32 34 and 37), 20 rows against 200 keys 13 and 11, but behind 1023 keys 32 and 37.
-// For a prefix even where own rows are up to 8: 64 heads of 128 on 8, FP32 rows on half precision, 16 sequences: 2048 keys 25 us with 16 and 28 with 8, 500 keys 16 and 16 (with 1000 own
-// keys a sequence 23 and 21); 16 rows of each of 32 key/value heads, FP32 pages, 2048 keys 48 and 42. 16 rows of heads of 256 do not fit the registers.
+// For a prefix even where own rows are up to 8, us with 16 and with 8. 64 heads of 128 on 8, bf16, up to 100 own keys a sequence: 16 sequences behind 700 keys 16.7 and 16.9, behind 1500 21.7 and 22.1, behind 2500
+// 26.4 and 29.4; 32 heads on 8, 24 sequences behind 2500 23.6 and 25.4; 64 heads of 64 on 8, 40 sequences behind 1500 24.5 and 28.1; 16 rows of each of 32 key/value heads behind 2500, which gain nothing, 24.8 and
+// 23.6. Over 268 shapes of bf16, of FP32 on half precision and of FP32 pages, half of them with up to 1000 own keys, 0.6 % over the better of both, always with 8 rows 3.1 %. 16 rows of heads of 256 do not fit the
+// registers.
 inline int stream_rows(int head_dim, int64_t own, int64_t kv_heads, int64_t shared, int64_t prefix) {
     const double products = (double)kv_heads * (double)shared * (double)prefix * head_dim;
-    const bool sixteen = own > 8 ? head_dim == 128 || own >= 32 || products > 1e8 : shared >= 96 && products > 2.4e8;
+    const bool sixteen = own > 8 ? head_dim == 128 || own >= 32 || products > 1e8 : shared >= 96 && products > 1.5e8;
     return head_dim <= 128 && sixteen ? 16 : 8;
 }
 // What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
 // heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
 
-// Whether one warp joins a row, or four do. bf16, 64 heads of 128, in all: 1 token against 4000 keys 21 us with one and 16 with four, 16 tokens against 1000 17.5 and 16.9,
-// 48 behind 2048 31 and 34, 120 behind 4096 53 and 66, 800 against 1000 72 and 108; 48 tokens of 32 heads behind 8192 keys, of whose partial results a row has 18, 145 and 142.
+// Whether one warp joins a row, or four do. bf16, in all, us with one and with four: 8 tokens of 64 heads of 128 against up to 1000 keys 17.1 and 13.7, 16 tokens 18.5 and 17.3, 24 tokens 21.2 and 21.6, 100 tokens
+// 50.5 and 59.9. In between a row may have many partial results, of a long prefix: 48 tokens of 32 heads behind 4096 keys 40.9 and 39.0, behind 8192 40.1 and 38.1, of heads of 64 34.5 and 33.0, 24 of 64 heads
+// behind 4096 36.1 and 33.5, 64 of 32 behind 8192 42.0 and 41.3; without a prefix 48 of 32 29.7 and 31.3.
 inline bool warp_joins_row(int64_t rows, int64_t partial) { return rows > 1200 && (partial < 12 || rows > 4800); }
 
 Plan plan_of(const jq_pages* p, int elem, int heads, int64_t tokens, int64_t sequences, int64_t prefix_length) {
