@@ -11,7 +11,8 @@
 namespace jq {
 namespace {
 
-// Other head sizes than the stream kernel's: one thread block per row and query head. 128 keys at a time, a thread has a key's score, then elements of the output.
+// Other head sizes than the stream kernel's: one thread block per row and query head. 128 keys at a time, a thread has a key's score, then elements of the output. Nothing
+// is shared among the rows and heads that read the same keys: 16 sequences of one row of 32 heads of 96 on 8 against up to 1000 keys, bf16, 405 us, where heads of 128 take 17.
 template <typename T, typename C>
 __global__ void __launch_bounds__(128) attend_row_kernel(AttendArgs a) {
     __shared__ float qs[256], sc[128], red[8];

@@ -14,8 +14,8 @@
 // towards zero (4e-6 of the result at 8192 keys): it only adds up a chunk, smallest parts first, and the chunks are added with rounding by the multiplication that a new
 // maximum takes anyway; of the scores the products of the first parts are added up apart from the small ones.
 //
-// Measured: 48 sequences of up to 4096 own keys, bf16, 32 heads of 128 on 8, 84 us with the joining kernel's for 0.50 GB, 6.0 TB/s (91 % of a copy's). FP32 pages are bound by the six products and by splitting:
-// 15 sequences of 8 rows of those heads behind 3900 keys 221 us. One row against 577 keys, FP32, 12 us in all: the chain of lookup, keys, values and the joining kernel's.
+// Measured: 48 sequences of up to 4096 own keys, bf16, 32 heads of 128 on 8, 86 us with the joining kernel's for 0.50 GB, 5.9 TB/s (90 % of a copy's). FP32 pages are bound by the six products and by splitting:
+// 15 sequences of 8 rows of those heads behind 3900 keys 211 us. One row against 577 keys, FP32, 13 us in all: the chain of lookup, keys, values and the joining kernel's.
 #pragma once
 
 #include "jq_pages_attention.cuh"

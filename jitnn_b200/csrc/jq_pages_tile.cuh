@@ -15,7 +15,7 @@
 // are cleared in shared memory, and the rows that do see such a key add it by themselves. Sums that are not finite in the end are worked out once more from the values that are not.
 //
 // Bound per tile and SM: the products' 1024 clocks at head size 128 (times the parts), the threads' 128 exponentials (1024 clocks at 16 a clock) and about 700 instructions a
-// warp, or 2800 clocks for 64 KB of pages where they come from memory. Measured, all launches of a call: 280 tokens of 32 heads of 128 on 8 behind 7182 keys, FP16, 81 us, 407 TFLOP/s; 48 tokens of
+// warp, or 2800 clocks for 64 KB of pages where they come from memory. Measured, all launches of a call: 280 tokens of 32 heads of 128 on 8 behind 7182 keys, bf16, 82 us, 401 TFLOP/s (FP16, whose sums are scaled more often, 87 us); 48 tokens of
 // 64 heads behind 2048 keys, bf16, 30 us. What bounds it is one tile's chain: scores, maximum of both halves, weights, sums are 3.8 us, two of which share an SM.
 #pragma once
 
