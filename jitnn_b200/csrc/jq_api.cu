@@ -22,6 +22,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) {
+    cudaGetLastError();  // (told here: the next launch's check is not to find it)
     int code = e == cudaErrorMemoryAllocation ? JQ_ERR_OOM : JQ_ERR_CUDA;
     return fail(code, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
 }
