@@ -48,6 +48,34 @@ def test_waits_that_run_out(short_waits, act, cache, hd, rows, lengths, prefix):
     assert torch.equal(whole[last + 1:], part[last + 1:]) and not torch.equal(whole[last], part[last])
 
 
+@pytest.mark.parametrize("act,cache", [(F16, F16), (BF16, BF16), (F32, F16), (F32, BF16)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("limit", [2, 3, 4, 6, 9, 14])
+def test_waits_that_run_out_anywhere(short_waits, act, cache, hd, limit):
+    """Limits that the first waits keep and later ones do not, with missing pages and values that are not finite under the rows' masks: whatever gave up, the call behind it is right."""
+    t = Setup([130, 150, 5], [900, 1500, 60], 2, hd, 16, cache, prefix=700, hole=float("nan"), seed=33)
+    q = normal(t.tokens, 32, hd, dtype=act, seed=33).cuda()
+    t.cache.v[int(t.tables[1, 90]), :, 3] = float("inf")  # (a key that some of the second sequence's rows see)
+    table = t.batch.tables.clone()
+    table[0, 5] = table[1, 70] = -1
+    missing = PagedBatch(table, t.batch.starts, t.batch.lengths, prefix=t.batch.prefix, prefix_length=700)
+    _lib.check(_lib.load().jq_set_option(b"wait_limit_us", limit))
+    for _ in range(10):
+        t.cache.attention(q, t.batch)
+        t.cache.attention(q, missing)
+    torch.cuda.synchronize()
+    code = device_status(0)
+    assert code == 96 or 10 <= code <= 19
+    short_waits()
+    for batch, after in ((t.batch, 0), (missing, 96)):
+        first = t.cache.attention(q, batch)
+        bits = torch.int32 if act is F32 else torch.int16
+        assert torch.equal(t.cache.attention(q, batch).view(bits), first.view(bits))
+        assert torch.isfinite(first[: t.starts[1]]).all() and not torch.isfinite(first[t.starts[2] - 1]).any()
+        torch.cuda.synchronize()
+        assert device_status(0) == after
+
+
 @pytest.mark.parametrize("act,cache", [(F32, F32), (F32, F16), (BF16, BF16)])
 @pytest.mark.parametrize("hd,rows", [(40, [2, 1]), (96, [1, 1]), (64, [2, 1]), (256, [1, 2]), (128, [40, 1])])
 @pytest.mark.parametrize("prefix", [0, 20])
