@@ -160,8 +160,9 @@ inline int stream_rows(int head_dim, int64_t own, int64_t kv_heads, int64_t shar
     const bool sixteen = own > 8 ? head_dim == 128 || own >= 32 || products > 1e8 : shared >= 96 && products > 1.5e8;
     return head_dim <= 128 && sixteen ? 16 : 8;
 }
-// What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with 64 own keys behind 4096,
-// heads of 128, FP32 on half precision, with the tile kernel 115 us (with 1, 2, 3 and 5 units 72, 62, 63 and 72); with the stream kernel heads of 64 130 us (with 2 and 4 units 80 and 64).
+// What beginning and ending an item takes, in units (128 and 16 keys). Without it whoever had many short items was late: 24 sequences of 5 rows with up to
+// 64 own keys behind 4096, heads of 128, with the tile kernel, bf16 59 us (with 1, 3 and 5 units 41, 37 and 40), FP32 on half precision 55 (54, 51 and 51); with the stream kernel heads of 64, a row each, FP32 on half
+// precision 45 us (with 2 and 4 units 24.2 and 22.4), 5 rows behind 1000, half precision, 58 (29 and 25).
 constexpr int TILE_OVER = 3, STREAM_OVER = 4;
 
 // Whether one warp joins a row, or four do. bf16, in all, us with one and with four: 8 tokens of 64 heads of 128 against up to 1000 keys 17.1 and 13.7, 16 tokens 18.5 and 17.3, 24 tokens 21.2 and 21.6, 100 tokens
